@@ -1,0 +1,41 @@
+// Arguments shared by the attention_tree kernels (attention_tree.cu has the
+// operator's definition).
+#pragma once
+#include <cmath>
+
+#include "common.cuh"
+#include "internal.hpp"
+
+namespace jade {
+
+struct TreeArgs {
+    const void *q, *k, *v;
+    const int *lengths;
+    const uint32_t *tree;  // [batch, seq, words]
+    void *out;
+    float *weights;
+    float2 *stats;    // per row of q: the maximum score and 1 / the sum of e^(s - maximum)
+    float2 *part_ml;  // per row and split: maximum and sum
+    float *part_o;    // per row and split: dim unnormalised sums
+    int batch, kv_heads, group, seq, words, dim, capacity, rows;  // rows = group * seq
+    float scale_log2;  // log2(e) / sqrt(dim): scores to exponents of 2
+    int *err;
+};
+
+inline TreeArgs tree_args(Context *ctx, const Spec &s) {
+    TreeArgs a{};
+    a.batch = s.batch, a.kv_heads = s.kv_heads, a.group = s.heads / s.kv_heads, a.seq = s.seq, a.words = (s.seq + 31) / 32;
+    a.dim = s.dim, a.capacity = s.capacity, a.rows = a.group * a.seq;
+    a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)s.dim));
+    a.err = ctx->err_dev;
+    return a;
+}
+// the spec's bindings: q, k, v, lengths, tree, out, weights
+inline TreeArgs tree_bind(TreeArgs a, void **b, bool weights) {
+    a.q = b[0], a.k = b[1], a.v = b[2], a.lengths = static_cast<const int *>(b[3]), a.tree = static_cast<const uint32_t *>(b[4]);
+    a.out = b[5];
+    a.weights = weights ? static_cast<float *>(b[6]) : nullptr;
+    return a;
+}
+
+}  // namespace jade

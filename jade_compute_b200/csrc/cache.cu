@@ -1,0 +1,228 @@
+// cache_evict and cache_commit: which entries of a key/value cache stay, and
+// moving them together. k, v are [batch, kv_heads, capacity, dim]; entry j of a
+// sequence is slot j < length. Rows are moved as 16-byte vectors whatever their
+// type (dim is a multiple of 8).
+//
+// cache_evict keeps, for every (sequence, head), the `recent` newest entries and
+// of the others those of largest accumulated weight up to `keep` in all (equal
+// weights: the lower slot; NaN counts as largest, -0 as 0), in slot order, and
+// writes them to another cache from slot 0 on. kept: their old slots, then -1.
+//
+// cache_commit: after attention_tree over seq drafted tokens in slots length ..,
+// moves the accepted ones, path[0 .. count) ascending, to slots length + 0, 1, ...
+// in place; their accumulated weights too, the rest of the drafts' weights to 0.
+#include <algorithm>
+#include <climits>
+
+#include "common.cuh"
+#include "internal.hpp"
+
+namespace jade {
+namespace {
+
+// ------------------------------------------------------------------ cache_evict
+struct EvictArgs {
+    const uint4 *k, *v;
+    const float *weights;
+    const int *lengths;
+    uint4 *k_out, *v_out;
+    float *weights_out;
+    int *kept, *lengths_out;
+    int kv_heads, capacity, keep, recent, vecs;  // vecs: 16-byte vectors of a row
+    int *err;
+};
+
+// Unsigned keys in the order of the weights.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (w != w) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(w == 0.0f ? 0.0f : w);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelectThreads = 1024;
+
+// Exclusive prefix sum of one flag per thread over the block, in thread order, and the total.
+__device__ __forceinline__ int block_rank(bool flag, int *warp_sums, int &total) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ballot = __ballot_sync(0xffffffffu, flag);
+    __syncthreads();
+    if (lane == 0) warp_sums[warp] = __popc(ballot);
+    __syncthreads();
+    int v = warp_sums[lane], sum = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int n = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += n;
+    }
+    total = __shfl_sync(0xffffffffu, sum, 31);
+    const int before = __shfl_sync(0xffffffffu, sum - v, warp);
+    return before + __popc(ballot & ((1u << lane) - 1));
+}
+
+// One block per (sequence, head): the need-th largest key among the entries that
+// may go, digit by digit (8 bits, from the top), then the kept slots in order.
+__global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
+    __shared__ int hist[256], warp_sums[32], chosen[2];
+    const int bh = blockIdx.x, b = bh / a.kv_heads;
+    const int n = a.lengths[b];
+    int *kept = a.kept + (size_t)bh * a.keep;
+    float *w_out = a.weights_out + (size_t)bh * a.capacity;
+    if (n < 0 || n > a.capacity) {
+        if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrCacheLength);
+        return;
+    }
+    const float *w = a.weights + (size_t)bh * a.capacity;
+    const int count = min(n, a.keep), last = max(0, n - a.recent);
+    int need = count - (n - last);  // of the first `last` entries
+    uint32_t prefix = 0;
+    const bool all = need >= last;
+    for (int shift = 24; shift >= 0 && !all && need > 0; shift -= 8) {
+        for (int i = threadIdx.x; i < 256; i += kSelectThreads) hist[i] = 0;
+        __syncthreads();
+        for (int j = threadIdx.x; j < last; j += kSelectThreads) {
+            const uint32_t key = weight_key(w[j]);
+            if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&hist[key >> shift & 255], 1);
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int above = 0, d = 255;
+            while (above + hist[d] < need) above += hist[d--];
+            chosen[0] = d, chosen[1] = need - above;
+        }
+        __syncthreads();
+        prefix = prefix << 8 | (uint32_t)chosen[0];
+        need = chosen[1];
+    }
+    // prefix: the smallest kept key; need: how many entries with exactly it are kept
+    int ties = 0, written = 0;
+    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
+        const int j = j0 + threadIdx.x;
+        bool take = j < n && (all || j >= last), tie = false;
+        if (!all && j < last && need > 0) {
+            const uint32_t key = weight_key(w[j]);
+            take = key > prefix;
+            tie = key == prefix;
+        }
+        int total;
+        if (!all && need > 0) {
+            const int rank = block_rank(tie, warp_sums, total);
+            take = take || (tie && ties + rank < need);
+            ties += total;
+        }
+        const int at = written + block_rank(take, warp_sums, total);
+        if (take) {
+            kept[at] = j;
+            w_out[at] = w[j];
+        }
+        written += total;
+    }
+    for (int i = count + threadIdx.x; i < a.keep; i += kSelectThreads) kept[i] = -1;
+    for (int i = count + threadIdx.x; i < a.capacity; i += kSelectThreads) w_out[i] = 0.0f;
+    if (bh % a.kv_heads == 0 && threadIdx.x == 0) a.lengths_out[b] = count;
+}
+
+__global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
+    const int bh = blockIdx.y, n = a.lengths[bh / a.kv_heads], count = min(n, a.keep);
+    const int *kept = a.kept + (size_t)bh * a.keep;
+    const size_t base = (size_t)bh * a.capacity;
+    const long long total = (long long)count * a.vecs;
+    if (n < 0 || n > a.capacity) return;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+        const int row = (int)(i / a.vecs), vec = (int)(i - (long long)row * a.vecs);
+        const size_t from = (base + kept[row]) * a.vecs + vec, to = (base + row) * a.vecs + vec;
+        a.k_out[to] = __ldg(a.k + from);
+        a.v_out[to] = __ldg(a.v + from);
+    }
+}
+
+// ------------------------------------------------------------------ cache_commit
+struct CommitArgs {
+    const int *path, *counts, *lengths;
+    uint4 *k, *v;
+    float *weights;
+    int *lengths_out;
+    int kv_heads, capacity, seq, vecs;
+    int *err;
+};
+
+constexpr int kCommitThreads = 256, kCommitVecs = 4;
+
+// One block per (sequence, head). Paths ascend, so path[i] >= i: rows are moved in
+// order, a block's worth at a time (all read before any is written), and no later
+// row's source is overwritten.
+__global__ void __launch_bounds__(kCommitThreads) commit_kernel(const CommitArgs a) {
+    const int bh = blockIdx.x, b = bh / a.kv_heads, n = a.lengths[b], count = a.counts[b];
+    const int *path = a.path + (size_t)b * a.seq;
+    const int i = threadIdx.x;
+    bool good = n >= 0 && n <= a.capacity - a.seq;
+    if (!good && i == 0) atomicCAS(a.err, 0, kErrCacheLength);
+    bool path_good = count >= 0 && count <= a.seq;
+    if (path_good && i < count) path_good = path[i] >= 0 && path[i] < a.seq && (i == 0 || path[i] > path[i - 1]);
+    path_good = __syncthreads_and(path_good);
+    if (!path_good && i == 0) atomicCAS(a.err, 0, kErrCommitPath);
+    if (!good || !path_good) return;
+    const size_t base = (size_t)bh * a.capacity + n;
+    if (bh % a.kv_heads == 0 && i == 0) a.lengths_out[b] = n + count;
+    if (a.weights) {
+        float moved = 0.0f;
+        if (i < count) moved = a.weights[base + path[i]];
+        __syncthreads();
+        if (i < a.seq) a.weights[base + i] = moved;
+    }
+    const int total = count * a.vecs;
+    for (int j0 = 0; j0 < total; j0 += kCommitThreads * kCommitVecs) {
+        uint4 kr[kCommitVecs], vr[kCommitVecs];
+#pragma unroll
+        for (int u = 0; u < kCommitVecs; ++u) {
+            const int j = j0 + u * kCommitThreads + i;
+            if (j < total) {
+                const size_t from = (base + path[j / a.vecs]) * a.vecs + j % a.vecs;
+                kr[u] = a.k[from], vr[u] = a.v[from];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < kCommitVecs; ++u) {
+            const int j = j0 + u * kCommitThreads + i;
+            if (j < total) a.k[base * a.vecs + j] = kr[u], a.v[base * a.vecs + j] = vr[u];
+        }
+        __syncthreads();
+    }
+}
+
+}  // namespace
+
+LaunchFn make_cache_op(Context *ctx, const Spec &s, std::string &impl) {
+    impl = std::string(spec_name(s)) + "_" + dtype_name(s.dtype);
+    const int heads = (int)(s.batch * s.kv_heads), vecs = (int)(s.dim * dtype_size(s.dtype) / 16);
+    if (s.op == Op::CacheCommit) {
+        CommitArgs base{};
+        base.kv_heads = s.kv_heads, base.capacity = s.capacity, base.seq = s.seq, base.vecs = vecs, base.err = ctx->err_dev;
+        const bool weights = s.weights;
+        return [=](cudaStream_t st, void **b) {
+            CommitArgs a = base;
+            a.path = static_cast<const int *>(b[0]), a.counts = static_cast<const int *>(b[1]), a.lengths = static_cast<const int *>(b[2]);
+            a.k = static_cast<uint4 *>(b[3]), a.v = static_cast<uint4 *>(b[4]);
+            a.weights = weights ? static_cast<float *>(b[5]) : nullptr;
+            a.lengths_out = static_cast<int *>(b[weights ? 6 : 5]);
+            commit_kernel<<<heads, kCommitThreads, 0, st>>>(a);
+            return cudaGetLastError();
+        };
+    }
+    if (heads > 65535) throw IrError("cache_evict: batch * kv_heads must be at most 65535");
+    EvictArgs base{};
+    base.kv_heads = s.kv_heads, base.capacity = s.capacity, base.keep = s.keep, base.recent = s.recent, base.vecs = vecs;
+    base.err = ctx->err_dev;
+    const int blocks = (int)std::min<long long>(((long long)s.keep * vecs + 1023) / 1024, std::max(1, 16 * ctx->sm_count / heads));
+    return [=](cudaStream_t st, void **b) {
+        EvictArgs a = base;
+        a.k = static_cast<const uint4 *>(b[0]), a.v = static_cast<const uint4 *>(b[1]), a.weights = static_cast<const float *>(b[2]);
+        a.lengths = static_cast<const int *>(b[3]), a.k_out = static_cast<uint4 *>(b[4]), a.v_out = static_cast<uint4 *>(b[5]);
+        a.weights_out = static_cast<float *>(b[6]), a.kept = static_cast<int *>(b[7]), a.lengths_out = static_cast<int *>(b[8]);
+        evict_select_kernel<<<heads, kSelectThreads, 0, st>>>(a);
+        evict_move_kernel<<<dim3(blocks, heads), 256, 0, st>>>(a);
+        return cudaGetLastError();
+    };
+}
+
+}  // namespace jade

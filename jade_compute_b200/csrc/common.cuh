@@ -29,6 +29,9 @@ enum DeviceError : int {
     kErrWaitDrain = 8,      // exit path waiting for copies in flight
     kErrBadLaunch = 9,      // launch geometry mismatch detected on device
     kErrWaitProbe = 10,     // wait_probe: a wait that nothing satisfies, expired as designed
+    // checks of input values that only the device sees (the kernel skips the sequence)
+    kErrCacheLength = 11,   // a sequence's cache length (or first slot) leaves no room for its new tokens
+    kErrCommitPath = 12,    // cache_commit: count or path outside the drafted tokens, or path not ascending
 };
 
 __device__ __forceinline__ uint64_t globaltimer() {

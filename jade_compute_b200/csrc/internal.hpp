@@ -97,6 +97,12 @@ inline bool attention_prefers_pair(const Spec &s, int sm_count) {
     auto efficiency = [&](double workers) { return items / (std::ceil(items / workers) * workers); };
     return efficiency(sm_count) < 0.92 * efficiency(sm_count / 2);
 }
+// Cached attention (rope.cu, attention_tree.cu, cache.cu)
+LaunchFn make_qk_norm_rope(Context *ctx, const Spec &s, std::string &impl);  // and its gradient
+LaunchFn make_attention_tree(Context *ctx, const Spec &s, std::string &impl, std::string &path);
+LaunchFn make_cache_op(Context *ctx, const Spec &s, std::string &impl);  // cache_evict, cache_commit
+// Device memory, zero-filled, that a kernel keeps from its compilation to its release.
+std::shared_ptr<void> kernel_workspace(size_t bytes, const char *what);
 LaunchFn make_elementwise_rtc(Context *ctx, const Spec &s, std::string &impl);
 LaunchFn make_misc_kernel(Context *ctx, const Spec &s, std::string &impl);  // fill, l2_flush
 LaunchFn make_cublas_gemm(Context *ctx, const Spec &s, std::string &impl);

@@ -107,6 +107,11 @@ void matrix(uint64_t x, uint64_t y) {
     ensure(x * y <= (uint64_t)INT_MAX, "tensor exceeds checked 31-bit indexing");
 }
 
+// the operators of a cached attention step
+bool is_cached_attention(Op op) {
+    return op == Op::QkNormRope || op == Op::QkNormRopeGrad || op == Op::AttentionTree || op == Op::CacheEvict || op == Op::CacheCommit;
+}
+
 bool is16(DType d) { return d == DType::BF16 || d == DType::F16; }
 
 void check_dtype(const Spec &s, std::initializer_list<DType> allowed) {
@@ -120,7 +125,7 @@ std::string u(uint64_t v) { return std::to_string(v) + "u"; }
 
 size_t dtype_size(DType d) {
     switch (d) {
-        case DType::F32: case DType::TF32: return 4;
+        case DType::F32: case DType::TF32: case DType::I32: return 4;
         case DType::BF16: case DType::F16: return 2;
         case DType::U8: return 1;
     }
@@ -133,6 +138,7 @@ const char *dtype_name(DType d) {
         case DType::BF16: return "bf16";
         case DType::F16: return "fp16";
         case DType::U8: return "u8";
+        case DType::I32: return "i32";
     }
     return "?";
 }
@@ -147,7 +153,7 @@ DType parse_dtype(const std::string &s) {
 bool Spec::extended() const {
     return has_dtype || has_out_dtype || has_batch || has_b_layout || epilogue != "none" || row_scale || sm_limit ||
            op == Op::RmsInv || op == Op::AllReduce || op == Op::Copy || op == Op::L2Flush || op == Op::Fill || op == Op::WaitProbe ||
-           op == Op::ShardReduce || op == Op::ShardGather || ranks;
+           op == Op::ShardReduce || op == Op::ShardGather || ranks || is_cached_attention(op);
 }
 
 const char *spec_name(const Spec &s) {
@@ -172,6 +178,11 @@ const char *spec_name(const Spec &s) {
         case Op::ShardReduce: return "shard_reduce";
         case Op::ShardGather: return "shard_gather";
         case Op::Fill: return "fill";
+        case Op::QkNormRope: return "qk_norm_rope";
+        case Op::QkNormRopeGrad: return "qk_norm_rope_grad";
+        case Op::AttentionTree: return "attention_tree";
+        case Op::CacheEvict: return "cache_evict";
+        case Op::CacheCommit: return "cache_commit";
     }
     return "?";
 }
@@ -223,10 +234,37 @@ Spec parse_spec(const Json &j) {
         if (j.has("lo")) s.lo = get_f32(j, "lo");
         if (j.has("hi")) s.hi = get_f32(j, "hi");
         if (j.has("offset")) s.offset = get_uint(j, "offset", UINT64_MAX);
+    } else if (op == "qk_norm_rope" || op == "qk_norm_rope_grad") {
+        s.op = op == "qk_norm_rope" ? Op::QkNormRope : Op::QkNormRopeGrad;
+        s.heads = get_u32(j, "heads"); s.kv_heads = get_u32(j, "kv_heads"); s.seq = get_u32(j, "seq"); s.dim = get_u32(j, "dim");
+        if (j.has("norm")) s.norm = get_bool(j, "norm");
+        if (s.norm) s.epsilon = get_f32(j, "epsilon");
+        s.rotary = j.has("rotary") ? get_u32(j, "rotary") : s.dim;
+        if (j.has("interleaved")) s.interleaved = get_bool(j, "interleaved");
+        if (j.has("base")) s.base = get_f32(j, "base");
+        if (j.has("scaling")) s.scaling = get_str(j, "scaling");
+        if (s.scaling != "none") s.factor = get_f32(j, "factor");
+        if (s.scaling == "yarn") s.original = get_u32(j, "original");
+        if (j.has("capacity")) { s.capacity = get_u32(j, "capacity"); ensure(s.capacity > 0, "capacity must be positive"); }
+    } else if (op == "attention_tree") {
+        s.op = Op::AttentionTree;
+        s.heads = get_u32(j, "heads"); s.kv_heads = get_u32(j, "kv_heads"); s.seq = get_u32(j, "seq"); s.dim = get_u32(j, "dim");
+        s.capacity = get_u32(j, "capacity");
+        if (j.has("weights")) s.weights = get_bool(j, "weights");
+    } else if (op == "cache_evict") {
+        s.op = Op::CacheEvict;
+        s.kv_heads = get_u32(j, "kv_heads"); s.dim = get_u32(j, "dim"); s.capacity = get_u32(j, "capacity");
+        s.keep = get_u32(j, "keep");
+        if (j.has("recent")) s.recent = get_u32(j, "recent");
+    } else if (op == "cache_commit") {
+        s.op = Op::CacheCommit;
+        s.kv_heads = get_u32(j, "kv_heads"); s.dim = get_u32(j, "dim"); s.capacity = get_u32(j, "capacity"); s.seq = get_u32(j, "seq");
+        if (j.has("weights")) s.weights = get_bool(j, "weights");
     } else {
         bail("unknown variant `" + op + "`, expected one of `elementwise`, `axpy`, `add`, `gemm`, `gemm_simd`, `gemm_mps`, "
              "`attention_scores`, `attention_apply`, `attention_online`, `rms_norm`, `swi_glu`, `softmax`, "
-             "`rms_inv`, `all_reduce`, `copy`, `l2_flush`, `fill`, `wait_probe`, `shard_reduce`, `shard_gather`");
+             "`rms_inv`, `all_reduce`, `copy`, `l2_flush`, `fill`, `wait_probe`, `shard_reduce`, `shard_gather`, "
+             "`qk_norm_rope`, `qk_norm_rope_grad`, `attention_tree`, `cache_evict`, `cache_commit`");
     }
     if (const Json *d = j.get("dtype")) {
         if (d->kind != Json::String) bail("invalid type for `dtype`");
@@ -299,6 +337,27 @@ Json spec_to_json(const Spec &s) {
                 .set("stream", U(s.stream_id)).set("lo", Json::f32(s.lo)).set("hi", Json::f32(s.hi));
             if (s.offset) j.set("offset", U(s.offset));
             break;
+        case Op::QkNormRope: case Op::QkNormRopeGrad:
+            j.set("op", Json::str(spec_name(s))).set("heads", U(s.heads)).set("kv_heads", U(s.kv_heads)).set("seq", U(s.seq)).set("dim", U(s.dim));
+            j.set("norm", Json::boolean(s.norm));
+            if (s.norm) j.set("epsilon", Json::f32(s.epsilon));
+            j.set("rotary", U(s.rotary)).set("interleaved", Json::boolean(s.interleaved)).set("base", Json::f32(s.base)).set("scaling", Json::str(s.scaling));
+            if (s.scaling != "none") j.set("factor", Json::f32(s.factor));
+            if (s.scaling == "yarn") j.set("original", U(s.original));
+            if (s.capacity) j.set("capacity", U(s.capacity));
+            break;
+        case Op::AttentionTree:
+            j.set("op", Json::str("attention_tree")).set("heads", U(s.heads)).set("kv_heads", U(s.kv_heads)).set("seq", U(s.seq)).set("dim", U(s.dim))
+                .set("capacity", U(s.capacity)).set("weights", Json::boolean(s.weights));
+            break;
+        case Op::CacheEvict:
+            j.set("op", Json::str("cache_evict")).set("kv_heads", U(s.kv_heads)).set("dim", U(s.dim)).set("capacity", U(s.capacity)).set("keep", U(s.keep))
+                .set("recent", U(s.recent));
+            break;
+        case Op::CacheCommit:
+            j.set("op", Json::str("cache_commit")).set("kv_heads", U(s.kv_heads)).set("dim", U(s.dim)).set("capacity", U(s.capacity)).set("seq", U(s.seq))
+                .set("weights", Json::boolean(s.weights));
+            break;
     }
     if (s.has_dtype) j.set("dtype", Json::str(dtype_name(s.dtype)));
     if (s.has_out_dtype) j.set("out_dtype", Json::str(dtype_name(s.out_dtype)));
@@ -310,6 +369,53 @@ Json spec_to_json(const Spec &s) {
     if (s.ranks) j.set("ranks", U(s.ranks)).set("rank", U(s.rank));
     return j;
 }
+
+namespace {
+
+// Head rows move as 16-byte vectors in every type, so dim is a multiple of 8; a
+// warp holds one row of up to 256 elements. Activations keep the 31-bit limit of
+// the other operators; a cache may be longer than that (its kernels index in 64
+// bits), its slots and lengths are 31-bit.
+void validate_cached_attention(const Spec &s) {
+    check_dtype(s, {DType::F32, DType::BF16, DType::F16});
+    const std::string name = spec_name(s);
+    ensure(s.out_dtype == s.dtype, name + " writes its input type");
+    ensure(s.batch >= 1 && s.batch <= 65535, "attention batch must be 1..=65535");
+    ensure(s.kv_heads >= 1 && s.kv_heads <= 1024, "attention kv_heads must be 1..=1024");
+    ensure(s.dim >= 8 && s.dim <= 256 && s.dim % 8 == 0, name + " head dimension must be a multiple of 8 in 8..=256");
+    const uint64_t heads_total = (uint64_t)s.batch * s.kv_heads;
+    ensure(heads_total <= (uint64_t)INT_MAX, "tensor exceeds checked 31-bit indexing");
+    if (s.op == Op::QkNormRope || s.op == Op::QkNormRopeGrad || s.op == Op::AttentionTree) {
+        ensure(s.heads >= 1 && s.heads <= 1024 && s.heads % s.kv_heads == 0, "attention heads must be 1..=1024 and a multiple of kv_heads");
+        const uint32_t most = s.op == Op::AttentionTree ? 128 : 131072;
+        ensure(s.seq >= 1 && s.seq <= most, name + " sequence must be 1..=" + std::to_string(most));
+        ensure((uint64_t)s.batch * s.seq * (s.heads + 2ull * s.kv_heads) <= (uint64_t)INT_MAX / s.dim, "tensor exceeds checked 31-bit indexing");
+    }
+    if (s.op == Op::QkNormRope || s.op == Op::QkNormRopeGrad) {
+        ensure(!s.norm || (std::isfinite(s.epsilon) && s.epsilon > 0.0f), "epsilon must be finite and positive");
+        ensure(s.rotary % 2 == 0 && s.rotary <= s.dim, "rotary must be even and at most dim");
+        ensure(std::isfinite(s.base) && s.base >= 1.0f, "base must be finite and at least 1");
+        ensure(s.scaling == "none" || s.scaling == "linear" || s.scaling == "ntk" || s.scaling == "yarn",
+               "scaling must be none, linear, ntk or yarn");
+        ensure(std::isfinite(s.factor) && s.factor >= 1.0f, "factor must be finite and at least 1");
+        ensure(s.scaling != "ntk" || s.rotary > 2, "ntk scaling needs rotary above 2");
+        ensure(s.scaling != "yarn" || s.original >= 1, "yarn scaling needs the original context length");
+        ensure(s.op == Op::QkNormRope || !s.capacity, "qk_norm_rope_grad has no cache (capacity)");
+    }
+    if (s.op == Op::CacheCommit) ensure(s.seq >= 1 && s.seq <= 128, "cache_commit sequence must be 1..=128");
+    if (s.op == Op::CacheEvict) {
+        ensure(s.keep >= 1 && s.keep <= s.capacity, "keep must be 1..=capacity");
+        ensure(s.recent <= s.keep, "recent must be at most keep");
+        ensure(heads_total <= (uint64_t)INT_MAX / s.keep, "tensor exceeds checked 31-bit indexing");
+    }
+    if (s.capacity || (s.op != Op::QkNormRope && s.op != Op::QkNormRopeGrad)) {
+        ensure(s.capacity >= 1 && s.capacity <= (1u << 30), "capacity must be 1..=2^30");
+        ensure(s.op == Op::CacheEvict || s.capacity >= s.seq, "capacity must hold the sequence");
+        ensure(heads_total <= (1ull << 40) / ((uint64_t)s.capacity * s.dim), "cache exceeds 2^40 elements");
+    }
+}
+
+}  // namespace
 
 void validate(const Spec &s) {  // ir.rs:193-268 plus the extensions
     switch (s.op) {
@@ -403,13 +509,18 @@ void validate(const Spec &s) {  // ir.rs:193-268 plus the extensions
             ensure(std::isfinite(s.lo) && std::isfinite(s.hi), "fill parameters must be finite");
             check_dtype(s, {DType::F32, DType::BF16, DType::F16});
             break;
+        case Op::QkNormRope: case Op::QkNormRopeGrad: case Op::AttentionTree: case Op::CacheEvict: case Op::CacheCommit:
+            validate_cached_attention(s);
+            break;
     }
     if (s.op != Op::Gemm) {
         ensure(!s.has_b_layout && s.epilogue == "none" && !s.row_scale, std::string(spec_name(s)) + " has no GEMM fusion fields");
         ensure(!s.ranks || s.op == Op::ShardReduce || s.op == Op::ShardGather,
                std::string(spec_name(s)) + " has no ranks (gemm scatter and the shard collectives only)");
     }
-    if (s.has_batch) ensure(s.op == Op::AttentionOnline || s.op == Op::AttentionScores || s.op == Op::AttentionApply, "batch applies to attention only");
+    if (s.has_batch)
+        ensure(s.op == Op::AttentionOnline || s.op == Op::AttentionScores || s.op == Op::AttentionApply || is_cached_attention(s.op),
+               "batch applies to attention only");
 }
 
 std::vector<Binding> bindings(const Spec &s) {  // ir.rs:269-339
@@ -480,6 +591,53 @@ std::vector<Binding> bindings(const Spec &s) {  // ir.rs:269-339
             r = {b("out", (uint64_t)s.rows * s.cols, true, d), b("flags", kPeerFlagBytes, true, DType::U8)};
             break;
         case Op::Fill: r = {b("out", s.len, true, d)}; break;
+        case Op::QkNormRope: case Op::QkNormRopeGrad: {
+            const uint64_t tokens = (uint64_t)s.batch * s.seq, rows = (uint64_t)s.batch * s.kv_heads * (s.capacity ? s.capacity : s.seq);
+            const uint64_t packed = tokens * (s.heads + 2ull * s.kv_heads) * s.dim;
+            r.push_back(b("qkv", packed, false, d));
+            if (s.norm) {
+                r.push_back(b("q_weight", s.dim, false, d));
+                r.push_back(b("k_weight", s.dim, false, d));
+            }
+            r.push_back(b("positions", tokens, false, DType::I32));
+            if (s.capacity) r.push_back(b("starts", s.batch, false, DType::I32));
+            const bool forward = s.op == Op::QkNormRope;
+            r.push_back(b(forward ? "q" : "dq", tokens * s.heads * s.dim, forward, d));
+            r.push_back(b(forward ? "k" : "dk", rows * s.dim, forward, d));
+            r.push_back(b(forward ? "v" : "dv", rows * s.dim, forward, d));
+            if (!forward) {
+                r.push_back(b("dqkv", packed, true, d));
+                if (s.norm) {
+                    r.push_back(b("dq_weight", s.dim, true, DType::F32));
+                    r.push_back(b("dk_weight", s.dim, true, DType::F32));
+                }
+            }
+            break;
+        }
+        case Op::AttentionTree: {
+            const uint64_t tokens = (uint64_t)s.batch * s.seq, slots = (uint64_t)s.batch * s.kv_heads * s.capacity;
+            r = {b("q", tokens * s.heads * s.dim, false, d), b("k", slots * s.dim, false, d), b("v", slots * s.dim, false, d),
+                 b("lengths", s.batch, false, DType::I32), b("tree", tokens * ((s.seq + 31) / 32), false, DType::I32),
+                 b("out", tokens * s.heads * s.dim, true, d)};
+            if (s.weights) r.push_back(b("weights", slots, true, DType::F32));
+            break;
+        }
+        case Op::CacheEvict: {
+            const uint64_t heads = (uint64_t)s.batch * s.kv_heads, slots = heads * s.capacity;
+            r = {b("k", slots * s.dim, false, d), b("v", slots * s.dim, false, d), b("weights", slots, false, DType::F32),
+                 b("lengths", s.batch, false, DType::I32), b("k_out", slots * s.dim, true, d), b("v_out", slots * s.dim, true, d),
+                 b("weights_out", slots, true, DType::F32), b("kept", heads * s.keep, true, DType::I32),
+                 b("lengths_out", s.batch, true, DType::I32)};
+            break;
+        }
+        case Op::CacheCommit: {
+            const uint64_t slots = (uint64_t)s.batch * s.kv_heads * s.capacity;
+            r = {b("path", (uint64_t)s.batch * s.seq, false, DType::I32), b("counts", s.batch, false, DType::I32),
+                 b("lengths", s.batch, false, DType::I32), b("k", slots * s.dim, true, d), b("v", slots * s.dim, true, d)};
+            if (s.weights) r.push_back(b("weights", slots, true, DType::F32));
+            r.push_back(b("lengths_out", s.batch, true, DType::I32));
+            break;
+        }
     }
     return r;
 }

@@ -12,7 +12,14 @@
 //   "epilogue"   none | swiglu | residual   (GEMM epilogue fusion)
 //   "row_scale"  bool, GEMM output rows scaled by a per-row FP32 vector
 //   "batch"      attention batch (layout [batch, heads, seq, dim])
-// and ops of this backend: rms_inv, all_reduce, copy, l2_flush, fill.
+// and ops of this backend: rms_inv, all_reduce, copy, l2_flush, fill, and those of
+// a cached attention step:
+//   qk_norm_rope       packed projection rows -> RMS-normalised, rotated queries and
+//                      keys, keys and values in their cache slots
+//   qk_norm_rope_grad  its gradient
+//   attention_tree     new tokens (one, or a drafted tree) attend to their cache
+//   cache_evict        the cache entries of largest accumulated attention weight
+//   cache_commit       the accepted branch of a drafted tree
 #pragma once
 #include <cstdint>
 #include <memory>
@@ -28,7 +35,7 @@ struct IrError : std::runtime_error {
     using std::runtime_error::runtime_error;
 };
 
-enum class DType { F32, TF32, BF16, F16, U8 };
+enum class DType { F32, TF32, BF16, F16, U8, I32 };  // U8 and I32: buffers only, not a spec's dtype
 size_t dtype_size(DType d);
 const char *dtype_name(DType d);
 DType parse_dtype(const std::string &s);
@@ -43,7 +50,8 @@ struct Expr {
 enum class Op {
     Elementwise, Axpy, Add, Gemm, GemmSimd, GemmMps, AttentionScores, AttentionApply,
     AttentionOnline, RmsNorm, SwiGlu, Softmax,
-    RmsInv, AllReduce, Copy, L2Flush, Fill, WaitProbe, ShardReduce, ShardGather
+    RmsInv, AllReduce, Copy, L2Flush, Fill, WaitProbe, ShardReduce, ShardGather,
+    QkNormRope, QkNormRopeGrad, AttentionTree, CacheEvict, CacheCommit
 };
 
 // Words of the per-rank flag buffer that the peer collectives share (arrivals
@@ -80,6 +88,18 @@ struct Spec {
     uint64_t limit_ns = 0;  // wait_probe: the bounded wait's time limit
     uint32_t ranks = 0, rank = 0;  // peer collectives and the gemm "scatter" epilogue
     bool residual = false;         // shard_reduce: add a residual to the reduced rows
+    // cached attention
+    uint32_t kv_heads = 0;         // heads of k and v; `heads` is a multiple
+    uint32_t capacity = 0;         // cache slots of a sequence (0: k and v hold the seq tokens alone)
+    uint32_t rotary = 0;           // leading elements of a head that are rotated
+    bool interleaved = false;      // rotated pairs are neighbours (else the two halves)
+    bool norm = true;              // qk_norm_rope: RMS norm of the query and key heads
+    float base = 10000.0f;         // rotation frequencies base^(-2i / rotary)
+    std::string scaling = "none";  // none | linear | ntk | yarn
+    float factor = 1.0f;           // how many times longer the scaled context is
+    uint32_t original = 0;         // yarn: the context length before scaling
+    bool weights = false;          // accumulated attention weight of every cache slot
+    uint32_t keep = 0, recent = 0; // cache_evict: entries kept, of which the newest always
     bool extended() const;
 };
 

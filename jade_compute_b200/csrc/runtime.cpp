@@ -25,6 +25,7 @@
 
 #include "../../include/jade_runtime.h"
 #include "cabi.hpp"
+#include "common.cuh"
 #include "internal.hpp"
 
 using jade::check_cuda;
@@ -40,6 +41,25 @@ void *driver_entry(const char *name) {
     if (cudaGetDriverEntryPointByVersion(name, &fn, 12000, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
         return nullptr;
     return fn;
+}
+std::shared_ptr<void> kernel_workspace(size_t bytes, const char *what) {
+    void *p = nullptr;
+    const cudaError_t st = cudaMalloc(&p, bytes);
+    if (st != cudaSuccess) {
+        cudaGetLastError();
+        raise(st == cudaErrorMemoryAllocation ? JR_ENOMEM : JR_ECUDA, "%s (%zu bytes): %s (%d)", what, bytes, cudaGetErrorString(st), (int)st);
+    }
+    int device = 0;
+    cudaGetDevice(&device);
+    std::shared_ptr<void> owned(p, [device](void *q) {
+        cudaSetDevice(device);
+        cudaFree(q);
+    });
+    // zeroed on the legacy stream, so waited for: contexts run non-blocking streams
+    cudaError_t zero = cudaMemsetAsync(p, 0, bytes, nullptr);
+    if (zero == cudaSuccess) zero = cudaStreamSynchronize(nullptr);
+    check_cuda(zero, what);
+    return owned;
 }
 void comm_poll_abort(Context *ctx);  // comm.cpp: throws JR_ETIMEOUT on an asynchronous NCCL error
 }  // namespace jade
@@ -128,8 +148,9 @@ void blocking_copy(Context &ctx, void *dst, const void *src, size_t bytes, cudaM
     check_cuda(done, (std::string(name) + " synchronization").c_str());
 }
 
-// Reads and clears the error word the kernels' bounded waits write (first
-// expiry wins), as JR_ETIMEOUT naming the wait that gave up.
+// Reads and clears the error word that kernels write (first error wins): a
+// bounded wait that expired is JR_ETIMEOUT naming the wait, an input value that
+// only the device could check is JR_EINVAL.
 void raise_device_wait_error(Context &ctx) {
     if (!ctx.err_host) return;
     volatile int *word = reinterpret_cast<volatile int *>(ctx.err_host);
@@ -147,6 +168,8 @@ void raise_device_wait_error(Context &ctx) {
                                        "exit wait for copies in flight",
                                        "launch geometry mismatch",
                                        "wait probe (a wait that nothing satisfies)"};
+    if (code == jade::kErrCacheLength) raise(JR_EINVAL, "a sequence's cache length is negative or leaves no room for its tokens in the capacity");
+    if (code == jade::kErrCommitPath) raise(JR_EINVAL, "cache_commit: a path must ascend within the drafted tokens, its count be at most their number");
     const bool known = code > 0 && code < (int)(sizeof site / sizeof site[0]);
     raise(JR_ETIMEOUT, "device-side bounded wait expired: %s (code %d)", known ? site[code] : "unknown", code);
 }
@@ -414,6 +437,17 @@ void select_implementation(Context *ctx, jr_kernel &k) {
             } else {
                 k.run = jade::make_attention_tc(ctx, s, k.impl);
             }
+            return;
+        case Op::QkNormRope: case Op::QkNormRopeGrad:
+            k.run = jade::make_qk_norm_rope(ctx, s, k.impl);
+            k.path = "simt";
+            return;
+        case Op::AttentionTree:
+            k.run = jade::make_attention_tree(ctx, s, k.impl, k.path);
+            return;
+        case Op::CacheEvict: case Op::CacheCommit:
+            k.run = jade::make_cache_op(ctx, s, k.impl);
+            k.path = "simt";
             return;
         case Op::Fill: case Op::L2Flush: case Op::WaitProbe:
             k.run = jade::make_misc_kernel(ctx, s, k.impl);
