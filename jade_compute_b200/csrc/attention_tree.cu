@@ -16,7 +16,8 @@
 // never multiplied (a NaN or infinity there cannot reach the row), slots from
 // lengths[b] + seq on are not read.
 //
-// This file: the FP32 path, any type and dim up to 256, on FFMA; weights; dispatch.
+// This file: FP32, and 16-bit types with dim above 128, on FFMA; weights; dispatch.
+// attention_tree_tc.cu: 16-bit types with dim up to 128, on tcgen05.
 #include <algorithm>
 #include <climits>
 
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const TreeArgs a, int sp
     const float shift = m == -INFINITY ? 0.0f : m;
     for (int s = 0; s < splits; ++s) l += ml[s].y * exp2f((ml[s].x - shift) * a.scale_log2);
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (lane == 0 && a.stats) a.stats[row] = make_float2(shift, inv);
+    if (lane == 0 && a.stats) a.stats[row] = make_float2(shift * a.scale_log2, inv);
     const int g = rr / a.seq, t = rr - g * a.seq;
     T *out = static_cast<T *>(a.out) + (((size_t)b * a.seq + t) * a.kv_heads * a.group + hk * a.group + g) * a.dim;
     for (int d = lane * 4; d < a.dim; d += 128) {
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(kThreads) tree_weights_simt_kernel(const TreeA
             const float2 st = a.stats[(size_t)bh * a.rows + r0 + r];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (sees(a, b, r0 + r, j0 + c + 8 * u, length)) acc[u] += exp2f((s[u] - st.x) * a.scale_log2) * st.y;
+                if (sees(a, b, r0 + r, j0 + c + 8 * u, length)) acc[u] += exp2f(fmaf(s[u], a.scale_log2, -st.x)) * st.y;
         }
         __syncthreads();
 #pragma unroll
@@ -212,6 +213,20 @@ __global__ void __launch_bounds__(kThreads) tree_weights_simt_kernel(const TreeA
             a.weights[(size_t)bh * a.capacity + j0 + threadIdx.x] += s;
         }
     }
+}
+
+template <typename T>
+TreeWeightsFn weights_simt(Context *ctx, const Spec &s) {
+    const int heads = (int)(s.batch * s.kv_heads);
+    if (s.weights && heads > 65535) throw IrError("attention_tree: batch * kv_heads must be at most 65535");
+    const int smem = (int)((kRows + kKeys) * q_stride(s.dim) * 4 + kRows * kKeys * 4);
+    if (cudaFuncSetAttribute(tree_weights_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        throw IrError("cannot reserve shared memory for attention_tree");
+    const int blocks = (int)std::min<long long>((s.capacity + kKeys - 1) / kKeys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
+    return [=](cudaStream_t st, const TreeArgs &a) {
+        tree_weights_simt_kernel<T><<<dim3(blocks, heads), kThreads, smem, st>>>(a);
+        return cudaGetLastError();
+    };
 }
 
 template <typename T>
@@ -228,24 +243,31 @@ LaunchFn simt_launch(Context *ctx, const Spec &s) {
     base.part_ml = base.stats + total_rows;
     base.part_o = reinterpret_cast<float *>(base.part_ml + (size_t)total_rows * splits);
     const size_t row = (size_t)q_stride(s.dim) * 4;
-    const size_t smem = (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4, smem_w = (kRows + kKeys) * row + kRows * kKeys * 4;
-    if (cudaFuncSetAttribute(tree_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaFuncSetAttribute(tree_weights_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_w) != cudaSuccess)
+    const size_t smem = (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4;
+    if (cudaFuncSetAttribute(tree_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         throw IrError("cannot reserve shared memory for attention_tree");
     const bool weights = s.weights;
-    const int key_blocks = (int)std::min<long long>((s.capacity + kKeys - 1) / kKeys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
+    const TreeWeightsFn add_weights = weights_simt<T>(ctx, s);
     return [=, keep = ws](cudaStream_t st, void **b) {
         const TreeArgs a = tree_bind(base, b, weights);
         tree_simt_kernel<T><<<dim3(row_blocks, splits, heads), kThreads, smem, st>>>(a, splits);
         tree_join_kernel<T><<<(total_rows + 3) / 4, 128, 0, st>>>(a, splits, total_rows);
-        if (weights) tree_weights_simt_kernel<T><<<dim3(key_blocks, heads), kThreads, smem_w, st>>>(a);
-        return cudaGetLastError();
+        return weights ? add_weights(st, a) : cudaGetLastError();
     };
 }
 
 }  // namespace
 
+TreeWeightsFn tree_weights(Context *ctx, const Spec &s) {
+    return s.dtype == DType::BF16 ? weights_simt<__nv_bfloat16>(ctx, s) : weights_simt<__half>(ctx, s);
+}
+
 LaunchFn make_attention_tree(Context *ctx, const Spec &s, std::string &impl, std::string &path) {
+    if (s.dtype != DType::F32 && s.dim <= 128) {
+        impl = std::string("attention_tree_tcgen05_d") + std::to_string(s.dim) + "_" + dtype_name(s.dtype);
+        path = "tcgen05";
+        return make_attention_tree_tc(ctx, s);
+    }
     impl = std::string("attention_tree_simt_d") + std::to_string(s.dim) + "_" + dtype_name(s.dtype);
     path = "simt";
     if (s.dtype == DType::BF16) return simt_launch<__nv_bfloat16>(ctx, s);

@@ -14,7 +14,7 @@ struct TreeArgs {
     const uint32_t *tree;  // [batch, seq, words]
     void *out;
     float *weights;
-    float2 *stats;    // per row of q: the maximum score and 1 / the sum of e^(s - maximum)
+    float2 *stats;    // for the weights, per row of q: p_j = 2^(s_j scale_log2 - x) y
     float2 *part_ml;  // per row and split: maximum and sum
     float *part_o;    // per row and split: dim unnormalised sums
     int batch, kv_heads, group, seq, words, dim, capacity, rows;  // rows = group * seq
@@ -37,5 +37,10 @@ inline TreeArgs tree_bind(TreeArgs a, void **b, bool weights) {
     a.weights = weights ? static_cast<float *>(b[6]) : nullptr;
     return a;
 }
+
+// Adds the rows' p_j (from their stats) to the weights of every cache slot.
+using TreeWeightsFn = std::function<cudaError_t(cudaStream_t, const TreeArgs &)>;
+TreeWeightsFn tree_weights(Context *ctx, const Spec &s);
+LaunchFn make_attention_tree_tc(Context *ctx, const Spec &s);  // 16-bit types, dim up to 128
 
 }  // namespace jade

@@ -1,0 +1,715 @@
+// attention_tree on tcgen05 for BF16/FP16 and dim up to 128 (attention_tree.cu has
+// the operator's definition).
+//
+// The M = group * seq rows of a (sequence, kv head) are one operand of the tensor
+// core, 128 to a tile, so a key is read from HBM once whatever the number of query
+// heads and drafted tokens; the kernel is bound by that stream up to M = 256
+// (256 FLOP per byte of a 16-bit cache). dim is padded to 64 or 128 by the TMA
+// loads' zero fill.
+//
+// Work: an item is a (sequence, kv head, row block); its keys are tiles of 128. The
+// tiles of all items form one list (lengths are read on the device), cut into equal
+// ranges, one per CTA: sequences of any mix of lengths load every SM alike. A range
+// is a run of segments, each a part of one item. A CTA writes the rows of an item
+// that it has whole; of an item that it shares it writes the unnormalised sums with
+// their maxima, and tree_join_tc joins them in range order.
+//   warp 0     TMA: Q of each segment, then K and V tiles through one ring of stages
+//              in the order in which the MMA warp takes them
+//   warp 1     MMA: S = Q K^T, O += P V, two chains t = 0, 1 so that the tensor core
+//              works for one while the other's softmax runs
+//   warps 2-5, 6-9  softmax of chain 0 / 1, one thread per row: scores out of TMEM,
+//              running maximum and sum in FP32, P rounded to the input type back into
+//              TMEM (relative error 2^-9 / 2^-12 per weight; the sum is of unrounded
+//              weights), O rescaled only when a maximum grows by more than 2^8
+// M <= 128: the chains take alternate key tiles of the same rows and are joined at
+// the segment's end, both sums being in the same TMEM lanes. M > 128: the chains are
+// two row tiles that share each K and V tile.
+//
+// A tile that reaches beyond the committed slots is masked per row by the drafts'
+// bits. Its V rows from lengths + seq on are zeroed in shared memory before the
+// product; non-finite elements of drafted V rows are zeroed too and added to the
+// rows that see them at the end, so that they reach no other row.
+#include <climits>
+#include <mutex>
+#include <type_traits>
+
+#include "attention_softmax.cuh"
+#include "attention_tree.cuh"
+
+namespace jade {
+namespace {
+
+constexpr int kThreads = 10 * 32, kTileKeys = 128, kTileRows = 128;
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
+
+template <int DP>
+struct Layout {
+    static constexpr uint32_t kChunk = 128 * 128;  // 128 rows x 64 elements, 128-byte swizzle
+    static constexpr uint32_t kTile = (DP / 64) * kChunk;
+    static constexpr int kStages = DP == 128 ? 5 : 10;  // 160 KB of K and V in flight per SM
+    static constexpr uint32_t kQ = 0;                   // two tiles
+    static constexpr uint32_t kRing = 2 * kTile;
+    static constexpr uint32_t kExchange = kRing + kStages * kTile;  // chain 1's (maximum, sum) per row
+    static constexpr uint32_t kBar = kExchange + 128 * 8;
+    static constexpr uint32_t kSmem = kBar + 512 + 1024;
+};
+
+struct TcArgs {
+    TreeArgs t;
+    int row_blocks, ctas;
+};
+
+// ------------------------------------------------------------------ work ranges
+__device__ __forceinline__ int tiles_of(const TreeArgs &t, int b, int &length) {
+    length = __ldg(t.lengths + b);
+    if (length < 0 || length > t.capacity - t.seq) return 0;
+    return (length + t.seq + kTileKeys - 1) / kTileKeys;
+}
+__device__ __forceinline__ long long range_tiles(long long total, int ctas) { return max(1ll, (total + ctas - 1) / ctas); }
+
+struct Segment {
+    int b, hk, rb, first, last, tiles, length;  // key tiles [first, last) of the item's `tiles`
+    __device__ __forceinline__ int count() const { return last - first; }
+};
+
+// The segments of a CTA's range, in order; every role walks the same sequence.
+struct Segments {
+    int b, sub, tile;
+    long long left;
+    __device__ __forceinline__ bool next(const TcArgs &a, Segment &s) {
+        if (left <= 0) return false;
+        int length, tiles = tiles_of(a.t, b, length);
+        if (tile >= tiles) {
+            tile = 0;
+            if (++sub >= a.t.kv_heads * a.row_blocks || tiles == 0) {
+                sub = 0;
+                do {
+                    if (++b >= a.t.batch) return false;
+                    tiles = tiles_of(a.t, b, length);
+                } while (tiles == 0);
+            }
+        }
+        s.b = b, s.hk = sub / a.row_blocks, s.rb = sub - s.hk * a.row_blocks;
+        s.first = tile, s.last = (int)min((long long)tiles, tile + left), s.tiles = tiles, s.length = length;
+        left -= s.last - s.first;
+        tile = s.last;
+        return true;
+    }
+};
+
+// Sum over the whole block of every thread's value (all threads get it). scratch: one long long per warp.
+__device__ __forceinline__ long long block_total(long long v, long long *scratch) {
+    const int warps = blockDim.x >> 5;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+    __syncthreads();
+    long long s = 0;
+    for (int w = 0; w < warps; ++w) s += scratch[w];
+    return s;
+}
+
+// Tiles of all items, and of the items of sequences before `b`.
+__device__ __forceinline__ void count_tiles(const TcArgs &a, int b, long long *scratch, long long &total, long long &before) {
+    long long all = 0, less = 0;
+    for (int i = threadIdx.x; i < a.t.batch; i += blockDim.x) {
+        int length;
+        const int n = tiles_of(a.t, i, length);
+        all += n;
+        if (i < b) less += n;
+    }
+    const long long per = (long long)a.t.kv_heads * a.row_blocks;
+    total = block_total(all, scratch) * per;
+    before = b > 0 ? block_total(less, scratch) * per : 0;
+}
+
+// ------------------------------------------------------------------ masks
+// Bit c of the result: the row sees column c of the tile whose first key lies `off`
+// slots before the first draft (off may be negative: the tile starts among the drafts).
+__device__ __forceinline__ void column_mask(const uint32_t (&bits)[4], int off, uint32_t (&mask)[4]) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int i0 = 32 * w - off;  // draft of column 32 w
+        uint32_t m = 0;
+        if (i0 <= -32) m = 0xffffffffu;
+        else if (i0 < 0) m = (1u << -i0) - 1 | bits[0] << -i0;
+        else if (i0 < 128) {
+            const int q = i0 >> 5, r = i0 & 31;
+            uint32_t lo = 0, hi = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (x == q) lo = bits[x];
+                if (x == q + 1) hi = bits[x];
+            }
+            m = __funnelshift_r(lo, hi, r);
+        }
+        mask[w] = m;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t exponent_bits() { return std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u; }
+
+// Zeroes V rows that hold no entry, and the non-finite elements of drafted rows
+// (whose drafts are noted in `bad`). Thread `key` owns one row of the tile.
+template <int DP, typename T>
+__device__ __forceinline__ void clean_v(uint8_t *v, int key, int j0, int length, int seq, uint32_t *bad) {
+    using L = Layout<DP>;
+    const int draft = j0 + key - length;
+    if (draft < 0) return;
+    bool found = false;
+#pragma unroll 1
+    for (uint32_t at = key * 128; at < L::kTile; at += L::kChunk)
+#pragma unroll 1
+        for (int u = 0; u < 8; ++u) {
+            uint4 *p = reinterpret_cast<uint4 *>(v + at) + u;
+            if (draft >= seq) {
+                *p = make_uint4(0, 0, 0, 0);
+                continue;
+            }
+            uint4 x = *p;
+            uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+            const uint32_t e = exponent_bits<T>();
+            bool hit = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if ((w[i] & e) == e) w[i] &= 0xffff0000u, hit = true;
+                if ((w[i] >> 16 & e) == e) w[i] &= 0x0000ffffu, hit = true;
+            }
+            if (hit) *p = x, found = true;
+        }
+    if (found) atomicOr(&bad[draft >> 5], 1u << (draft & 31));
+}
+
+// ------------------------------------------------------------------ kernel
+template <int DP, typename T, bool kTwoTiles>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const TcArgs args) {
+    using L = Layout<DP>;
+    constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr uint32_t kIdescS = idesc_f32acc(kFmt, kFmt, false, false, kTileRows, kTileKeys);
+    constexpr uint32_t kIdescO = idesc_f32acc(kFmt, kFmt, false, true, kTileRows, DP);
+    constexpr int kDChunks = DP / 64, kStages = L::kStages;
+
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
+    uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8, *o_free = bars + 10;
+    uint64_t *x_full = bars + 12, *x_empty = bars + 13, *mma_done = bars + 14;
+    uint64_t *full = bars + 16, *empty = bars + 16 + kStages;  // ring stages
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 36);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    uint32_t *bad = tmem_slot + 4;  // [3][4]: drafts with non-finite V, by segment number modulo 3
+    int *plan = reinterpret_cast<int *>(tmem_slot + 16);  // the range's first b, sub, tile and (64 bits) length
+    float2 *exchange = reinterpret_cast<float2 *>(smem + L::kExchange);
+
+    const TreeArgs &ta = args.t;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *err = ta.err;
+    int ring_loads = 0, q_loads = 0;  // issued by the producer (read on the abort path, after every role ended)
+
+    if (threadIdx.x == 0) {
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&q_full[t], 1); mbar_init(&q_empty[t], 1);
+            mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 128);
+            mbar_init(&o_full[t], 1); mbar_init(&o_free[t], 128);
+        }
+        mbar_init(x_full, 128); mbar_init(x_empty, 128); mbar_init(mma_done, 1);
+        for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
+        *abort_flag = 0;
+        for (int i = 0; i < 12; ++i) bad[i] = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    if (warp == 0) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    long long total, none;
+    count_tiles(args, 0, reinterpret_cast<long long *>(exchange), total, none);
+    const long long per = range_tiles(total, args.ctas), begin = per * blockIdx.x;
+    if (warp == 0) {  // the first sequence whose tiles reach beyond `begin`
+        const long long items = (long long)ta.kv_heads * args.row_blocks;
+        long long base = 0;
+        for (int b0 = 0; b0 < ta.batch && begin < total; b0 += 32) {
+            int length = 0;
+            const long long n = b0 + lane < ta.batch ? tiles_of(ta, b0 + lane, length) * items : 0;
+            long long upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > begin);
+            if (beyond && lane == __ffs(beyond) - 1) {
+                const long long into = begin - (base + upto - n);
+                const int tiles = (int)(n / items);
+                plan[0] = b0 + lane, plan[1] = (int)(into / tiles), plan[2] = (int)(into % tiles);
+            }
+            if (beyond) break;
+            base += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (blockIdx.x == 0)
+            for (int b = lane; b < ta.batch; b += 32) {
+                int length;
+                if (tiles_of(ta, b, length) == 0) atomicCAS(err, 0, kErrCacheLength);
+            }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem_s[2] = {tmem, tmem + 128};
+    const uint32_t tmem_o[2] = {tmem + 256, tmem + 384};
+    Segments segments{plan[0], plan[1], plan[2], begin < total ? min(per, total - begin) : 0};
+    Segment s;
+
+    if (warp == 0) {
+        if (lane == 0) {  // ------------------------------------- TMA producer
+            tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmK);
+            tma_prefetch_desc(&tmV);
+            bool ok = true;
+            while (ok && segments.next(args, s)) {
+                const int bh = s.b * ta.kv_heads + s.hk, n = s.count();
+                auto load = [&](const CUtensorMap &map, int tile) {
+                    const int st = ring_loads % kStages;
+                    if (!(ok = ok && mbar_wait(&empty[st], (ring_loads / kStages & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) return;
+                    mbar_arrive_expect_tx(&full[st], L::kTile);
+                    for (int c = 0; c < kDChunks; ++c)
+                        tma_load_3d(smem + L::kRing + st * L::kTile + c * L::kChunk, &map, &full[st], c * 64, (s.first + tile) * kTileKeys, bh);
+                    ++ring_loads;
+                };
+                auto load_q = [&](int buffer, int tile, int use) {
+                    if (!(ok = ok && mbar_wait(&q_empty[buffer], (use & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) return;
+                    mbar_arrive_expect_tx(&q_full[buffer], L::kTile);
+                    for (int c = 0; c < kDChunks; ++c)
+                        tma_load_3d(smem + L::kQ + buffer * L::kTile + c * L::kChunk, &tmQ, &q_full[buffer], c * 64, tile * kTileRows, bh);
+                };
+                if constexpr (kTwoTiles) {  // row tiles 2 rb and 2 rb + 1 (which may lie beyond the rows: zeros)
+                    load_q(0, 2 * s.rb, q_loads);
+                    load_q(1, 2 * s.rb + 1, q_loads);
+                    if (ok) ++q_loads;
+                    load(tmK, 0);
+                    for (int i = 0; i < n; ++i) {
+                        load(tmV, i);
+                        if (i + 1 < n) load(tmK, i + 1);
+                    }
+                } else {  // Q buffers alternate between segments
+                    load_q(q_loads & 1, 0, q_loads >> 1);
+                    if (ok) ++q_loads;
+                    load(tmK, 0);
+                    if (n > 1) load(tmK, 1);
+                    for (int i = 0; i < n; ++i) {
+                        load(tmV, i);
+                        if (i + 2 < n) load(tmK, i + 2);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------- MMA issuer (whole warp, one elected lane issues)
+        auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+        };
+        const uint64_t dq0 = sdesc_sw128(smem_u32(smem + L::kQ), 16, 1024);
+        const uint64_t dk0 = sdesc_sw128(smem_u32(smem + L::kRing), 16, 1024);
+        const uint64_t dv0 = sdesc_sw128(smem_u32(smem + L::kRing), L::kChunk, 1024);
+        auto issue_s = [&](int t, int q_buffer, int stage) {
+            uint64_t a[DP / 16], b[DP / 16];
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t off = ((k >> 2) * L::kChunk + (k & 3) * 32) >> 4;
+                a[k] = dq0 + ((q_buffer * L::kTile) >> 4) + off;
+                b[k] = dk0 + ((stage * L::kTile) >> 4) + off;
+            }
+            umma_ss_group<DP / 16>(tmem_s[t], a, b, kIdescS, 0);
+            umma_commit(&s_full[t]);
+        };
+        auto issue_pv = [&](int t, int stage, bool accumulate) {
+            uint64_t b[kTileKeys / 16];
+#pragma unroll
+            for (int k = 0; k < kTileKeys / 16; ++k) b[k] = dv0 + ((stage * L::kTile) >> 4) + ((k * 16 * 128) >> 4);
+            umma_ts_group8(tmem_o[t], tmem_s[t], b, kIdescO, accumulate);
+        };
+        // pos: ring loads consumed; qn: segments begun; cp: P tiles consumed; on: segments whose O_t was used
+        int pos = 0, qn = 0, cp[2] = {0, 0}, on[2] = {0, 0};
+        bool ok = true;
+        auto ready = [&] {  // the ring's next stage has landed
+            ok = ok && wait(&full[pos % kStages], pos / kStages & 1, kErrWaitTmaFull);
+            return ok;
+        };
+        auto release = [&] { umma_commit(&empty[pos++ % kStages]); };
+        auto p_ready = [&](int t, bool first) {  // P_t is written; for an item's first P V also: the last segment's O_t is read out
+            ok = ok && wait(&p_full[t], cp[t]++ & 1, kErrWaitProb);
+            if (first) {
+                if (on[t] > 0) ok = ok && wait(&o_free[t], (on[t] - 1) & 1, kErrWaitAccEmpty);
+                ++on[t];
+            }
+            return ok;
+        };
+        while (ok && segments.next(args, s)) {
+            const int n = s.count();
+            if constexpr (kTwoTiles) {
+                ok = wait(&q_full[0], qn & 1, kErrWaitTmaFull) && wait(&q_full[1], qn & 1, kErrWaitTmaFull);
+                ++qn;
+                if (!ready()) break;
+                tc_fence_after();
+                for (int t = 0; t < 2; ++t) issue_s(t, t, pos % kStages);
+                release();
+                for (int i = 0; i < n && ready(); ++i) {
+                    const int v = pos % kStages, k = (pos + 1) % kStages;
+                    for (int t = 0; t < 2 && p_ready(t, i == 0); ++t) {
+                        tc_fence_after();
+                        issue_pv(t, v, i > 0);  // reads P_t(i) from TMEM: must precede S_t(i + 1)
+                        if (i + 1 < n) {
+                            if (t == 0 && !(ok = wait(&full[k], (pos + 1) / kStages & 1, kErrWaitTmaFull))) break;
+                            tc_fence_after();
+                            issue_s(t, t, k);
+                        } else {
+                            umma_commit(&o_full[t]);
+                        }
+                    }
+                    if (!ok) break;
+                    release();
+                    if (i + 1 < n) release();
+                }
+                for (int t = 0; t < 2; ++t) umma_commit(&q_empty[t]);
+            } else {
+                const int q = qn & 1;
+                ok = wait(&q_full[q], qn >> 1 & 1, kErrWaitTmaFull);
+                ++qn;
+                for (int i = 0; i < 2 && i < n && ready(); ++i) {
+                    tc_fence_after();
+                    issue_s(i, q, pos % kStages);
+                    release();
+                }
+                if (n <= 2) umma_commit(&q_empty[q]);
+                for (int i = 0; i < n && ready() && p_ready(i & 1, i < 2); ++i) {
+                    const int t = i & 1;
+                    tc_fence_after();
+                    issue_pv(t, pos % kStages, i >= 2);
+                    release();
+                    if (i + 2 < n) {
+                        if (!ready()) break;
+                        tc_fence_after();
+                        issue_s(t, q, pos % kStages);
+                        release();
+                        if (i + 3 == n) umma_commit(&q_empty[q]);
+                    } else {
+                        umma_commit(&o_full[t]);
+                    }
+                }
+            }
+        }
+        umma_commit(mma_done);
+        mbar_wait_drain(mma_done, 0, err);
+    } else {
+        // ----------------------------------------------------- softmax (warps 2-5: chain 0, 6-9: chain 1)
+        const int t = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+        const uint32_t ts = tmem_s[t] + lane_off, to = tmem_o[t] + lane_off;
+        const float c = ta.scale_log2;
+        // cs: S tiles consumed; on: segments with O_t; xn: exchanges; ring: loads before the segment; sn: segments
+        int cs = 0, on[2] = {0, 0}, xn = 0, ring = 0, sn = 0;
+        bool ok = true;
+        for (; ok && segments.next(args, s); ++sn) {
+            const int n = s.count(), bh = s.b * ta.kv_heads + s.hk;
+            const int item_row = kTwoTiles ? s.rb * 256 + t * 128 + row : row;  // row of the item's M
+            const bool live = __any_sync(0xffffffffu, item_row < ta.rows);      // some row of this warp is one
+            uint32_t bits[4] = {0, 0, 0, 0};
+            uint32_t *bad_now = bad + (sn % 3) * 4;
+            if (threadIdx.x == 64)
+                for (int i = 0; i < 4; ++i) bad[((sn + 1) % 3) * 4 + i] = 0;
+            if (item_row < ta.rows)
+                for (int w = 0; w < 4; ++w)
+                    if (w < ta.words)  // no bits beyond the drafts: the slots behind them hold no entries
+                        bits[w] = __ldg(ta.tree + ((size_t)s.b * ta.seq + item_row % ta.seq) * ta.words + w) & (0xffffffffu >> max(0, 32 * (w + 1) - ta.seq));
+            float m_used = -INFINITY, l_run = 0.0f;
+            const int step = kTwoTiles ? 1 : 2;
+            bool first = true;
+            for (int i = kTwoTiles ? 0 : t; i < n; i += step, first = false) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], cs++ & 1, abort_flag, err, kErrWaitScore));
+                if (!ok) break;
+                tc_fence_after();
+                const int j0 = (s.first + i) * kTileKeys;
+                const bool masked = j0 + kTileKeys > s.length;
+                if (masked && (!kTwoTiles || t == 0)) {  // V(i) in place of what no row may multiply
+                    const int at = ring + (kTwoTiles ? 1 + 2 * i : min(2, n) + i + max(0, min(i, n - 2)));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&full[at % kStages], at / kStages & 1, abort_flag, err, kErrWaitTmaFull));
+                    if (!ok) break;
+                    clean_v<DP, T>(smem + L::kRing + (at % kStages) * L::kTile, row, j0, s.length, ta.seq, bad_now);
+                    fence_proxy_async();
+                }
+                if (live) {
+                    float sv[128];
+                    tmem_ld32f(ts, sv);
+                    tmem_ld32f(ts + 32, sv + 32);
+                    tmem_ld32f(ts + 64, sv + 64);
+                    tmem_ld32f(ts + 96, sv + 96);
+                    tmem_wait_ld();
+                    if (masked) {
+                        uint32_t mask[4];
+                        column_mask(bits, s.length - j0, mask);
+#pragma unroll
+                        for (int k = 0; k < 128; ++k) sv[k] = mask[k >> 5] >> (k & 31) & 1 ? sv[k] : -INFINITY;
+                    }
+                    float mx[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx[e] = max3(sv[e], sv[e + 8], sv[e + 16]);
+#pragma unroll
+                    for (int k = 24; k < 120; k += 16)
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], sv[k + e], sv[k + 8 + e]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], sv[120 + e]);
+                    const float m_tile = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
+                    float m_new = m_used, alpha = 1.0f;
+                    if (first) m_new = m_tile;
+                    else if (m_tile > m_used + kRescaleThreshold) {
+                        m_new = m_tile;
+                        alpha = mufu_exp2(m_used - m_new);
+                    }
+                    m_used = m_new;
+                    // a row that has seen nothing yet has maximum -inf: its weights are e^-inf = 0
+                    const float psum = store_p<kFmt, false, 128>(sv, c, m_used == -INFINITY ? 0.0f : m_used, ts);
+                    if (!first && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll 1
+                        for (int oc = 0; oc < DP; oc += 32) {
+                            float ov[32];
+                            tmem_ld32f(to + oc, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) ov[k] *= alpha;
+                            tmem_st32f(to + oc, ov);
+                        }
+                    }
+                    l_run = l_run * alpha + psum;
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                mbar_arrive(&p_full[t]);
+            }
+            ring += 2 * n;
+            if (!ok) break;
+            // ------------------------------------------------- the segment's rows
+            const bool both = !kTwoTiles && n > 1;  // chain 1 has sums to hand over
+            if (!kTwoTiles && t == 1) {
+                if (!both) continue;
+                ok = __all_sync(0xffffffffu, mbar_wait(x_empty, (xn++ & 1) ^ 1, abort_flag, err, kErrWaitAccEmpty));
+                if (!ok) break;
+                exchange[row] = make_float2(m_used, l_run);
+                mbar_arrive(x_full);
+                continue;
+            }
+            float f0 = 1.0f, f1 = 0.0f;  // factors of the two chains' sums
+            if (both) {
+                ok = __all_sync(0xffffffffu, mbar_wait(x_full, xn++ & 1, abort_flag, err, kErrWaitPv));
+                if (!ok) break;
+                const float2 other = exchange[row];
+                mbar_arrive(x_empty);
+                const float m = fmaxf(m_used, other.x), shift = m == -INFINITY ? 0.0f : m;
+                f0 = mufu_exp2(m_used - shift), f1 = mufu_exp2(other.x - shift);
+                l_run = l_run * f0 + other.y * f1;
+                m_used = m;
+            }
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], on[t]++ & 1, abort_flag, err, kErrWaitPv));
+            if (ok && both) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[1], on[1]++ & 1, abort_flag, err, kErrWaitPv));
+            if (!ok) break;
+            tc_fence_after();
+            const bool whole = s.first == 0 && s.last == s.tiles, valid = item_row < ta.rows;
+            const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;
+            if (whole) f0 *= inv, f1 *= inv;
+            uint32_t extra[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) extra[w] = valid ? bad_now[w] & bits[w] : 0;
+            const size_t slot = (size_t)blockIdx.x * 2 + (s.first == 0);
+            const int g = item_row / ta.seq, tok = item_row - g * ta.seq;
+            T *out = static_cast<T *>(ta.out) + (((size_t)s.b * ta.seq + tok) * ta.kv_heads * ta.group + s.hk * ta.group + g) * ta.dim;
+            constexpr int kSlotRows = kTwoTiles ? 256 : 128;
+            const int slot_row = kTwoTiles ? t * 128 + row : row;
+            float4 *part = reinterpret_cast<float4 *>(ta.part_o) + slot * (DP / 4) * kSlotRows + slot_row;
+            if (live) {
+#pragma unroll 1
+                for (int oc = 0; oc < DP; oc += 32) {
+                    float r[32];
+                    tmem_ld32f(to + oc, r);
+                    tmem_wait_ld();
+                    if (both) {
+                        float x[32];
+                        tmem_ld32f(tmem_o[1] + lane_off + oc, x);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) r[k] = f0 * r[k] + f1 * x[k];
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) r[k] *= f0;
+                    }
+                    if (extra[0] | extra[1] | extra[2] | extra[3]) {  // non-finite values that this row sees
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+#pragma unroll 1
+                            for (uint32_t left = extra[w]; left; left &= left - 1) {
+                                const int d = 32 * w + __ffs(left) - 1;
+                                const T *v = static_cast<const T *>(ta.v) + ((size_t)bh * ta.capacity + s.length + d) * ta.dim + oc;
+#pragma unroll
+                                for (int k = 0; k < 32; ++k)
+                                    if (oc + k < ta.dim) {
+                                        const float x = to_f32<T>(v[k]);
+                                        if (!isfinite(x)) r[k] += x;
+                                    }
+                            }
+                    }
+                    if (valid && whole) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8)
+                            if (oc + k < ta.dim)
+                                *reinterpret_cast<uint4 *>(out + oc + k) = make_uint4(pack16<kFmt>(r[k], r[k + 1]), pack16<kFmt>(r[k + 2], r[k + 3]),
+                                                                                      pack16<kFmt>(r[k + 4], r[k + 5]), pack16<kFmt>(r[k + 6], r[k + 7]));
+                    } else if (valid) {  // [dim / 4][row] so that a warp's rows are one run of memory
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            part[(size_t)((oc + k) / 4) * kSlotRows] = make_float4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            mbar_arrive(&o_free[t]);
+            if (both) mbar_arrive(&o_free[1]);
+            if (valid) {
+                if (!whole) ta.part_ml[slot * kSlotRows + slot_row] = make_float2(m_used, l_run);
+                else if (ta.stats) ta.stats[(size_t)bh * ta.rows + item_row] = make_float2(m_used == -INFINITY ? 0.0f : m_used, inv);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        if (lane == 0 && *abort_flag) {  // TMA loads still in flight land before the CTA exits
+            for (int i = max(0, ring_loads - kStages); i < ring_loads; ++i) mbar_wait_drain(&full[i % kStages], i / kStages & 1, err);
+            for (int i = max(0, q_loads - (kTwoTiles ? 1 : 2)); i < q_loads; ++i) {
+                if (kTwoTiles) mbar_wait_drain(&q_full[0], i & 1, err), mbar_wait_drain(&q_full[1], i & 1, err);
+                else mbar_wait_drain(&q_full[i & 1], i >> 1 & 1, err);
+            }
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// Joins the parts of items that several CTAs share: a block takes 32 rows of an
+// item, a thread one row and four columns; parts in range order.
+template <int DP, typename T, int kSlotRows>
+__global__ void __launch_bounds__(8 * DP) tree_join_tc(const TcArgs a) {
+    __shared__ long long scratch[32];
+    const TreeArgs &t = a.t;
+    const int subs = t.kv_heads * a.row_blocks, blocks = kSlotRows / 32;
+    const int item = blockIdx.x / blocks, b = item / subs, sub = item - b * subs, hk = sub / a.row_blocks, rb = sub - hk * a.row_blocks;
+    const int lane = threadIdx.x & 31, col = threadIdx.x >> 5, slot_row = (blockIdx.x - item * blocks) * 32 + lane, row = rb * kSlotRows + slot_row;
+    int length;
+    const int tiles = tiles_of(t, b, length);
+    long long total, before;
+    count_tiles(a, b, scratch, total, before);
+    if (tiles == 0 || row >= t.rows) return;
+    const long long per = range_tiles(total, a.ctas), begin = before + (long long)sub * tiles;
+    const int c0 = (int)(begin / per), c1 = (int)((begin + tiles - 1) / per);
+    if (c0 == c1) return;  // written whole
+    auto slot = [&](int c) { return (size_t)c * 2 + (c == c0); };
+    float m = -INFINITY, l = 0.0f;
+    for (int c = c0; c <= c1; ++c) m = fmaxf(m, t.part_ml[slot(c) * kSlotRows + slot_row].x);
+    const float shift = m == -INFINITY ? 0.0f : m;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 *part = reinterpret_cast<const float4 *>(t.part_o) + (size_t)col * kSlotRows + slot_row;
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+        const float2 ml = t.part_ml[slot(c) * kSlotRows + slot_row];
+        const float4 x = part[slot(c) * (DP / 4) * kSlotRows];
+        const float w = exp2f(ml.x - shift);
+        l = fmaf(ml.y, w, l);
+        o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    }
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    if (col == 0 && t.stats) t.stats[((size_t)b * t.kv_heads + hk) * t.rows + row] = make_float2(shift, inv);
+    if (col * 4 >= t.dim) return;
+    constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const int g = row / t.seq, tok = row - g * t.seq;
+    T *out = static_cast<T *>(t.out) + (((size_t)b * t.seq + tok) * t.kv_heads * t.group + hk * t.group + g) * t.dim + col * 4;
+    *reinterpret_cast<uint2 *>(out) = make_uint2(pack16<kFmt>(o.x * inv, o.y * inv), pack16<kFmt>(o.z * inv, o.w * inv));
+}
+
+// ------------------------------------------------------------------ host side
+using EncodeFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                              const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+    static EncodeFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] { fn = reinterpret_cast<EncodeFn>(driver_entry("cuTensorMapEncodeTiled")); });
+    return fn;
+}
+
+// [heads, rows, dim] tensor, box {64, 128, 1}, 128-byte swizzle; elements beyond dim or rows read as 0.
+bool row_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, uint64_t heads, uint64_t rows, uint64_t dim) {
+    const cuuint64_t dims[3] = {dim, rows, heads};
+    const cuuint64_t strides[2] = {dim * 2, rows * dim * 2};
+    const cuuint32_t box[3] = {64, 128, 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    return encoder()(map, dt, 3, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP, typename T, bool kTwoTiles>
+LaunchFn tc_launch(Context *ctx, const Spec &s) {
+    using L = Layout<DP>;
+    auto kernel = tree_tc_kernel<DP, T, kTwoTiles>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem) != cudaSuccess)
+        throw IrError("cannot reserve shared memory for the tcgen05 attention_tree");
+    constexpr int kSlotRows = kTwoTiles ? 256 : 128;
+    TcArgs base{};
+    base.t = tree_args(ctx, s);
+    const uint64_t heads = (uint64_t)s.batch * s.kv_heads, capacity = s.capacity, dim = s.dim, rows = base.t.rows;
+    base.row_blocks = (int)((rows + kSlotRows - 1) / kSlotRows);
+    // one CTA per SM, none for which even full caches have no tile
+    const unsigned __int128 most = (unsigned __int128)heads * base.row_blocks * ((capacity + kTileKeys - 1) / kTileKeys);
+    base.ctas = most < (unsigned __int128)ctx->sm_count ? (int)most : ctx->sm_count;
+    const long long join_blocks = (long long)heads * base.row_blocks * (kSlotRows / 32);
+    if (join_blocks > INT_MAX) throw IrError("attention_tree too large for one launch");
+    const bool weights = s.weights;
+    const size_t stats = (heads * rows * sizeof(float2) + 255) / 256 * 256, slots = (size_t)base.ctas * 2 * kSlotRows;
+    auto ws = kernel_workspace(stats + slots * (sizeof(float2) + DP * sizeof(float)), "attention_tree partial results");
+    base.t.stats = weights ? static_cast<float2 *>(ws.get()) : nullptr;
+    base.t.part_o = reinterpret_cast<float *>(static_cast<char *>(ws.get()) + stats);
+    base.t.part_ml = reinterpret_cast<float2 *>(base.t.part_o + slots * DP);
+    const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const TreeWeightsFn add_weights = tree_weights(ctx, s);
+    return [=, keep = ws](cudaStream_t st, void **b) {
+        TcArgs a = base;
+        a.t = tree_bind(base.t, b, weights);
+        CUtensorMap mq, mk, mv;
+        if (!row_map(&mq, dt, b[0], heads, rows, dim) || !row_map(&mk, dt, b[1], heads, capacity, dim) || !row_map(&mv, dt, b[2], heads, capacity, dim))
+            return cudaErrorInvalidValue;
+        kernel<<<a.ctas, kThreads, L::kSmem, st>>>(mq, mk, mv, a);
+        tree_join_tc<DP, T, kSlotRows><<<(int)join_blocks, 8 * DP, 0, st>>>(a);
+        return weights ? add_weights(st, a.t) : cudaGetLastError();
+    };
+}
+
+}  // namespace
+
+LaunchFn make_attention_tree_tc(Context *ctx, const Spec &s) {
+    if (!encoder()) throw IrError("cuTensorMapEncodeTiled unavailable");
+    const bool two = (uint64_t)s.heads / s.kv_heads * s.seq > kTileRows, wide = s.dim > 64;
+    auto pick = [&](auto type) {
+        using T = decltype(type);
+        if (wide) return two ? tc_launch<128, T, true>(ctx, s) : tc_launch<128, T, false>(ctx, s);
+        return two ? tc_launch<64, T, true>(ctx, s) : tc_launch<64, T, false>(ctx, s);
+    };
+    return s.dtype == DType::BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
+}
+
+}  // namespace jade
