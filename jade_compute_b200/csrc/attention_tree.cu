@@ -216,20 +216,6 @@ __global__ void __launch_bounds__(kThreads) tree_weights_simt_kernel(const TreeA
 }
 
 template <typename T>
-TreeWeightsFn weights_simt(Context *ctx, const Spec &s) {
-    const int heads = (int)(s.batch * s.kv_heads);
-    if (s.weights && heads > 65535) throw IrError("attention_tree: batch * kv_heads must be at most 65535");
-    const int smem = (int)((kRows + kKeys) * q_stride(s.dim) * 4 + kRows * kKeys * 4);
-    if (cudaFuncSetAttribute(tree_weights_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        throw IrError("cannot reserve shared memory for attention_tree");
-    const int blocks = (int)std::min<long long>((s.capacity + kKeys - 1) / kKeys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
-    return [=](cudaStream_t st, const TreeArgs &a) {
-        tree_weights_simt_kernel<T><<<dim3(blocks, heads), kThreads, smem, st>>>(a);
-        return cudaGetLastError();
-    };
-}
-
-template <typename T>
 LaunchFn simt_launch(Context *ctx, const Spec &s) {
     TreeArgs base = tree_args(ctx, s);
     const int heads = (int)(s.batch * s.kv_heads), rows = base.rows, row_blocks = (rows + kRows - 1) / kRows, total_rows = heads * rows;
@@ -243,24 +229,22 @@ LaunchFn simt_launch(Context *ctx, const Spec &s) {
     base.part_ml = base.stats + total_rows;
     base.part_o = reinterpret_cast<float *>(base.part_ml + (size_t)total_rows * splits);
     const size_t row = (size_t)q_stride(s.dim) * 4;
-    const size_t smem = (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4;
-    if (cudaFuncSetAttribute(tree_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    const size_t smem = (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4, smem_w = (kRows + kKeys) * row + kRows * kKeys * 4;
+    if (cudaFuncSetAttribute(tree_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaFuncSetAttribute(tree_weights_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_w) != cudaSuccess)
         throw IrError("cannot reserve shared memory for attention_tree");
     const bool weights = s.weights;
-    const TreeWeightsFn add_weights = weights_simt<T>(ctx, s);
+    const int key_blocks = (int)std::min<long long>((s.capacity + kKeys - 1) / kKeys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
     return [=, keep = ws](cudaStream_t st, void **b) {
         const TreeArgs a = tree_bind(base, b, weights);
         tree_simt_kernel<T><<<dim3(row_blocks, splits, heads), kThreads, smem, st>>>(a, splits);
         tree_join_kernel<T><<<(total_rows + 3) / 4, 128, 0, st>>>(a, splits, total_rows);
-        return weights ? add_weights(st, a) : cudaGetLastError();
+        if (weights) tree_weights_simt_kernel<T><<<dim3(key_blocks, heads), kThreads, smem_w, st>>>(a);
+        return cudaGetLastError();
     };
 }
 
 }  // namespace
-
-TreeWeightsFn tree_weights(Context *ctx, const Spec &s) {
-    return s.dtype == DType::BF16 ? weights_simt<__nv_bfloat16>(ctx, s) : weights_simt<__half>(ctx, s);
-}
 
 LaunchFn make_attention_tree(Context *ctx, const Spec &s, std::string &impl, std::string &path) {
     if (s.dtype != DType::F32 && s.dim <= 128) {

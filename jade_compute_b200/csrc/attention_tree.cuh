@@ -38,9 +38,6 @@ inline TreeArgs tree_bind(TreeArgs a, void **b, bool weights) {
     return a;
 }
 
-// Adds the rows' p_j (from their stats) to the weights of every cache slot.
-using TreeWeightsFn = std::function<cudaError_t(cudaStream_t, const TreeArgs &)>;
-TreeWeightsFn tree_weights(Context *ctx, const Spec &s);
 LaunchFn make_attention_tree_tc(Context *ctx, const Spec &s);  // 16-bit types, dim up to 128
 
 }  // namespace jade

@@ -54,6 +54,9 @@ struct Layout {
     static constexpr uint32_t kSmem = kBar + 512 + 1024;
 };
 
+// Rows of stats per item: whole groups of 16 columns of the weights' MMA, the last ones zero.
+__host__ __device__ constexpr size_t stats_stride(int rows) { return ((size_t)rows + 15) / 16 * 16; }
+
 struct TcArgs {
     TreeArgs t;
     int row_blocks, ctas;
@@ -122,6 +125,46 @@ __device__ __forceinline__ void count_tiles(const TcArgs &a, int b, long long *s
     const long long per = (long long)a.t.kv_heads * a.row_blocks;
     total = block_total(all, scratch) * per;
     before = b > 0 ? block_total(less, scratch) * per : 0;
+}
+
+// The CTA's range (whole block; also the barrier behind its set-up, TMEM allocation included).
+__device__ __forceinline__ Segments open_range(const TcArgs &a, int *plan, long long *scratch) {
+    const TreeArgs &t = a.t;
+    const int lane = threadIdx.x & 31;
+    long long total, none;
+    count_tiles(a, 0, scratch, total, none);
+    const long long per = range_tiles(total, a.ctas), begin = per * blockIdx.x;
+    if (threadIdx.x < 32) {  // the first sequence whose tiles reach beyond `begin`
+        const long long items = (long long)t.kv_heads * a.row_blocks;
+        long long base = 0;
+        for (int b0 = 0; b0 < t.batch && begin < total; b0 += 32) {
+            int length = 0;
+            const long long n = b0 + lane < t.batch ? tiles_of(t, b0 + lane, length) * items : 0;
+            long long upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > begin);
+            if (beyond && lane == __ffs(beyond) - 1) {
+                const long long into = begin - (base + upto - n);
+                const int tiles = (int)(n / items);
+                plan[0] = b0 + lane, plan[1] = (int)(into / tiles), plan[2] = (int)(into % tiles);
+            }
+            if (beyond) break;
+            base += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        if (blockIdx.x == 0)
+            for (int b = lane; b < t.batch; b += 32) {
+                int length;
+                if (tiles_of(t, b, length) == 0) atomicCAS(t.err, 0, kErrCacheLength);
+            }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    return Segments{plan[0], plan[1], plan[2], begin < total ? min(per, total - begin) : 0};
 }
 
 // ------------------------------------------------------------------ masks
@@ -227,43 +270,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(tmem_slot, 512);
         tmem_relinquish();
     }
-    long long total, none;
-    count_tiles(args, 0, reinterpret_cast<long long *>(exchange), total, none);
-    const long long per = range_tiles(total, args.ctas), begin = per * blockIdx.x;
-    if (warp == 0) {  // the first sequence whose tiles reach beyond `begin`
-        const long long items = (long long)ta.kv_heads * args.row_blocks;
-        long long base = 0;
-        for (int b0 = 0; b0 < ta.batch && begin < total; b0 += 32) {
-            int length = 0;
-            const long long n = b0 + lane < ta.batch ? tiles_of(ta, b0 + lane, length) * items : 0;
-            long long upto = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-                if (lane >= o) upto += x;
-            }
-            const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > begin);
-            if (beyond && lane == __ffs(beyond) - 1) {
-                const long long into = begin - (base + upto - n);
-                const int tiles = (int)(n / items);
-                plan[0] = b0 + lane, plan[1] = (int)(into / tiles), plan[2] = (int)(into % tiles);
-            }
-            if (beyond) break;
-            base += __shfl_sync(0xffffffffu, upto, 31);
-        }
-        if (blockIdx.x == 0)
-            for (int b = lane; b < ta.batch; b += 32) {
-                int length;
-                if (tiles_of(ta, b, length) == 0) atomicCAS(err, 0, kErrCacheLength);
-            }
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
+    Segments segments = open_range(args, plan, reinterpret_cast<long long *>(exchange));
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_s[2] = {tmem, tmem + 128};
     const uint32_t tmem_o[2] = {tmem + 256, tmem + 384};
-    Segments segments{plan[0], plan[1], plan[2], begin < total ? min(per, total - begin) : 0};
     Segment s;
 
     if (warp == 0) {
@@ -581,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (both) mbar_arrive(&o_free[1]);
             if (valid) {
                 if (!whole) ta.part_ml[slot * kSlotRows + slot_row] = make_float2(m_used, l_run);
-                else if (ta.stats) ta.stats[(size_t)bh * ta.rows + item_row] = make_float2(m_used == -INFINITY ? 0.0f : m_used, inv);
+                else if (ta.stats) ta.stats[(size_t)bh * stats_stride(ta.rows) + item_row] = make_float2(m_used == -INFINITY ? 0.0f : m_used, inv);
             }
         }
     }
@@ -633,12 +643,201 @@ __global__ void __launch_bounds__(8 * DP) tree_join_tc(const TcArgs a) {
         o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (col == 0 && t.stats) t.stats[((size_t)b * t.kv_heads + hk) * t.rows + row] = make_float2(shift, inv);
+    if (col == 0 && t.stats) t.stats[((size_t)b * t.kv_heads + hk) * stats_stride(t.rows) + row] = make_float2(shift, inv);
     if (col * 4 >= t.dim) return;
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const int g = row / t.seq, tok = row - g * t.seq;
     T *out = static_cast<T *>(t.out) + (((size_t)b * t.seq + tok) * t.kv_heads * t.group + hk * t.group + g) * t.dim + col * 4;
     *reinterpret_cast<uint2 *>(out) = make_uint2(pack16<kFmt>(o.x * inv, o.y * inv), pack16<kFmt>(o.z * inv, o.w * inv));
+}
+
+// ------------------------------------------------------------------ weights
+// weights[j] += sum over the item's M rows of p_j = 2^(s_j c - x) y, (x, y) the
+// rows' stats from the pass before. Transposed, S^T = K Q^T with 128 keys in the TMEM
+// lanes and up to 256 rows of Q in the columns, so that a thread owns a key and adds
+// its row of p in order: no sums between threads, no atomics. Ranges of key tiles per
+// CTA as above; more than 256 rows take several passes over the segment's keys.
+// Bound by K's second read and by one exponential per (row, key).
+//   warp 0 TMA (Q rows and their stats per segment, K tiles through a ring),
+//   warp 1 MMA into two buffers, warps 2-5 and 6-9 take the tiles in turn.
+constexpr int kWeightRows = 256;
+
+template <int DP>
+struct WeightsLayout {
+    static constexpr uint32_t kRows64 = kWeightRows * 128;  // 64 elements of every row of Q
+    static constexpr uint32_t kTile = (DP / 64) * 128 * 128;
+    static constexpr int kStages = DP == 128 ? 4 : 8;
+    static constexpr uint32_t kRing = (DP / 64) * kRows64;
+    static constexpr uint32_t kStats = kRing + kStages * kTile;
+    static constexpr uint32_t kBar = kStats + kWeightRows * 8;
+    static constexpr uint32_t kSmem = kBar + 512 + 1024;
+};
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    tree_weights_tc(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const TcArgs args) {
+    using L = WeightsLayout<DP>;
+    constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    constexpr int kDChunks = DP / 64, kStages = L::kStages;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
+    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *s_empty = bars + 4, *mma_done = bars + 6;
+    uint64_t *full = bars + 8, *empty = bars + 8 + kStages;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    int *plan = reinterpret_cast<int *>(tmem_slot + 2);
+    long long *scratch = reinterpret_cast<long long *>(tmem_slot + 6);
+    const float2 *stats = reinterpret_cast<const float2 *>(smem + L::kStats);
+
+    const TreeArgs &ta = args.t;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *err = ta.err;
+    int ring_loads = 0, q_loads = 0;
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1); mbar_init(q_empty, 1 + 256); mbar_init(mma_done, 1);
+        for (int t = 0; t < 2; ++t) mbar_init(&s_full[t], 1), mbar_init(&s_empty[t], 128);
+        for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    if (warp == 0) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    Segments segments = open_range(args, plan, scratch);
+    const uint32_t tmem = *tmem_slot;
+    Segment s;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            tma_prefetch_desc(&tmQ);
+            tma_prefetch_desc(&tmK);
+            bool ok = true;
+            while (ok && segments.next(args, s)) {
+                const int bh = s.b * ta.kv_heads + s.hk;
+                for (int r0 = 0; ok && r0 < ta.rows; r0 += kWeightRows) {
+                    if (!(ok = mbar_wait(q_empty, (q_loads & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) break;
+                    const int boxes = min(2, (ta.rows - r0 + 127) / 128), padded = min(kWeightRows, (ta.rows - r0 + 15) & ~15);
+                    mbar_arrive_expect_tx(q_full, boxes * L::kTile + padded * 8);
+                    for (int t = 0; t < boxes; ++t)
+                        for (int c = 0; c < kDChunks; ++c)
+                            tma_load_3d(smem + c * L::kRows64 + t * 128 * 128, &tmQ, q_full, c * 64, r0 + t * 128, bh);
+                    bulk_load(smem + L::kStats, ta.stats + (size_t)bh * stats_stride(ta.rows) + r0, padded * 8, q_full);
+                    ++q_loads;
+                    for (int i = s.first; i < s.last; ++i, ++ring_loads) {
+                        const int st = ring_loads % kStages;
+                        if (!(ok = mbar_wait(&empty[st], (ring_loads / kStages & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) break;
+                        mbar_arrive_expect_tx(&full[st], L::kTile);
+                        for (int c = 0; c < kDChunks; ++c)
+                            tma_load_3d(smem + L::kRing + st * L::kTile + c * 128 * 128, &tmK, &full[st], c * 64, i * kTileKeys, bh);
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
+            return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
+        };
+        const uint64_t dq0 = sdesc_sw128(smem_u32(smem), 16, 1024), dk0 = sdesc_sw128(smem_u32(smem + L::kRing), 16, 1024);
+        int pos = 0, qn = 0;
+        bool ok = true;
+        while (ok && segments.next(args, s))
+            for (int r0 = 0; ok && r0 < ta.rows; r0 += kWeightRows) {
+                const uint32_t idesc = idesc_f32acc(kFmt, kFmt, false, false, kTileKeys, min(kWeightRows, (ta.rows - r0 + 15) & ~15));
+                ok = wait(q_full, qn++ & 1, kErrWaitTmaFull);
+                for (int i = s.first; ok && i < s.last; ++i, ++pos) {
+                    const int st = pos % kStages, t = pos & 1;
+                    ok = wait(&full[st], pos / kStages & 1, kErrWaitTmaFull) && wait(&s_empty[t], (pos >> 1 & 1) ^ 1, kErrWaitAccEmpty);
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint64_t a[DP / 16], b[DP / 16];
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        a[k] = dk0 + ((st * L::kTile + (k >> 2) * 128 * 128 + (k & 3) * 32) >> 4);
+                        b[k] = dq0 + (((k >> 2) * L::kRows64 + (k & 3) * 32) >> 4);
+                    }
+                    umma_ss_group<DP / 16>(tmem + t * kWeightRows, a, b, idesc, 0);
+                    umma_commit(&s_full[t]);
+                    umma_commit(&empty[st]);
+                }
+                umma_commit(q_empty);
+            }
+        umma_commit(mma_done);
+        mbar_wait_drain(mma_done, 0, err);
+    } else {
+        const int t = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane;
+        const uint32_t ts = tmem + t * kWeightRows + ((uint32_t)(quarter * 32) << 16);
+        const float c = ta.scale_log2;
+        int pos = 0, qn = 0;
+        bool ok = true;
+        while (ok && segments.next(args, s)) {
+            float *weights = ta.weights + ((size_t)s.b * ta.kv_heads + s.hk) * ta.capacity;
+            for (int r0 = 0; ok && r0 < ta.rows; r0 += kWeightRows) {
+                ok = __all_sync(0xffffffffu, mbar_wait(q_full, qn++ & 1, abort_flag, err, kErrWaitTmaFull));
+                const int count = min(kWeightRows, ta.rows - r0);
+                for (int i = s.first; ok && i < s.last; ++i, ++pos) {
+                    if ((pos & 1) != t) continue;
+                    const int j = i * kTileKeys + key, draft = j - s.length;
+                    const float old = draft < ta.seq ? weights[j] : 0.0f;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], pos >> 1 & 1, abort_flag, err, kErrWaitScore));
+                    if (!ok) break;
+                    tc_fence_after();
+                    float sum = 0.0f;
+                    if (i * kTileKeys + kTileKeys <= s.length) {
+                        float sums[4] = {};
+#pragma unroll 1
+                        for (int n = 0; n < count; n += 32) {
+                            float sv[32];
+                            tmem_ld32f(ts + n, sv);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; k += 2) {
+                                const float4 st = *reinterpret_cast<const float4 *>(stats + n + k);
+                                if (n + k < count) {
+                                    sums[k & 2] = fmaf(mufu_exp2(fmaf(sv[k], c, -st.x)), st.y, sums[k & 2]);
+                                    sums[(k & 2) + 1] = fmaf(mufu_exp2(fmaf(sv[k + 1], c, -st.z)), st.w, sums[(k & 2) + 1]);
+                                }
+                            }
+                        }
+                        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                    } else {
+                        const uint32_t *tree = ta.tree + (size_t)s.b * ta.seq * ta.words + (max(draft, 0) >> 5);
+                        int tok = r0 % ta.seq;
+#pragma unroll 1
+                        for (int n = 0; n < count; n += 16) {
+                            uint32_t raw[16];
+                            tmem_ld16(ts + n, raw);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) {
+                                const bool sees = n + k < count && (draft < 0 || (draft < ta.seq && __ldg(tree + (size_t)tok * ta.words) >> (draft & 31) & 1));
+                                const float2 st = stats[min(n + k, kWeightRows - 1)];
+                                if (sees) sum = fmaf(mufu_exp2(fmaf(__uint_as_float(raw[k]), c, -st.x)), st.y, sum);
+                                if (++tok == ta.seq) tok = 0;
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    mbar_arrive(&s_empty[t]);
+                    if (draft < ta.seq) weights[j] = old + sum;
+                }
+                mbar_arrive(q_empty);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) {
+        if (lane == 0 && *abort_flag) {
+            for (int i = max(0, ring_loads - kStages); i < ring_loads; ++i) mbar_wait_drain(&full[i % kStages], i / kStages & 1, err);
+            if (q_loads) mbar_wait_drain(q_full, (q_loads - 1) & 1, err);
+        }
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -680,13 +879,16 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
     const long long join_blocks = (long long)heads * base.row_blocks * (kSlotRows / 32);
     if (join_blocks > INT_MAX) throw IrError("attention_tree too large for one launch");
     const bool weights = s.weights;
-    const size_t stats = (heads * rows * sizeof(float2) + 255) / 256 * 256, slots = (size_t)base.ctas * 2 * kSlotRows;
+    const size_t stats = (heads * stats_stride((int)rows) * sizeof(float2) + 255) / 256 * 256, slots = (size_t)base.ctas * 2 * kSlotRows;
     auto ws = kernel_workspace(stats + slots * (sizeof(float2) + DP * sizeof(float)), "attention_tree partial results");
     base.t.stats = weights ? static_cast<float2 *>(ws.get()) : nullptr;
     base.t.part_o = reinterpret_cast<float *>(static_cast<char *>(ws.get()) + stats);
     base.t.part_ml = reinterpret_cast<float2 *>(base.t.part_o + slots * DP);
     const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    const TreeWeightsFn add_weights = tree_weights(ctx, s);
+    auto weights_kernel = tree_weights_tc<DP, T>;
+    using W = WeightsLayout<DP>;
+    if (weights && cudaFuncSetAttribute(weights_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)W::kSmem) != cudaSuccess)
+        throw IrError("cannot reserve shared memory for the tcgen05 attention_tree");
     return [=, keep = ws](cudaStream_t st, void **b) {
         TcArgs a = base;
         a.t = tree_bind(base.t, b, weights);
@@ -695,7 +897,11 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
             return cudaErrorInvalidValue;
         kernel<<<a.ctas, kThreads, L::kSmem, st>>>(mq, mk, mv, a);
         tree_join_tc<DP, T, kSlotRows><<<(int)join_blocks, 8 * DP, 0, st>>>(a);
-        return weights ? add_weights(st, a.t) : cudaGetLastError();
+        if (weights) {
+            a.row_blocks = 1;
+            weights_kernel<<<a.ctas, kThreads, W::kSmem, st>>>(mq, mk, a);
+        }
+        return cudaGetLastError();
     };
 }
 
