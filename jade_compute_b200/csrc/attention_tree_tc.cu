@@ -41,17 +41,23 @@ namespace {
 
 constexpr int kThreads = 10 * 32, kTileKeys = 128, kTileRows = 128;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
+// An item's end in tiles (see "work ranges"): measured on B200 with 16 sequences of
+// 1,000 to 8,000 tokens, 128 items of 9 to 63 tiles: 73.8 us with 0, 67.3 with 2, 65.7
+// with 4, 64.6 with 6, 64.5 with 8
+constexpr int kBoundary = 6;
 
-template <int DP>
+template <int DP, bool kTwoTiles>
 struct Layout {
     static constexpr uint32_t kChunk = 128 * 128;  // 128 rows x 64 elements, 128-byte swizzle
     static constexpr uint32_t kTile = (DP / 64) * kChunk;
-    static constexpr int kStages = DP == 128 ? 5 : 10;  // 160 KB of K and V in flight per SM
-    static constexpr uint32_t kQ = 0;                   // two tiles
-    static constexpr uint32_t kRing = 2 * kTile;
-    static constexpr uint32_t kExchange = kRing + kStages * kTile;  // chain 1's (maximum, sum) per row
-    static constexpr uint32_t kBar = kExchange + 128 * 8;
-    static constexpr uint32_t kSmem = kBar + 512 + 1024;
+    static constexpr uint32_t kRing = 2 * kTile;                         // behind Q: two row tiles, or this segment's and the next one's
+    static constexpr int kStages = (224 * 1024 - kRing) / kTile;         // 160 KB of K and V in flight per SM (192 KB for DP = 64)
+    static constexpr uint32_t kExchange = kRing + kStages * kTile;               // (maximum, sum) of every row and chain
+    static constexpr uint32_t kBar = kExchange + 2 * 128 * 8;
+    static constexpr uint32_t kBytes = kBar + 512;
+    // dynamic shared memory starts on a 1024-byte boundary in practice (checked in
+    // the kernel); the slack covers the alignment where the layout leaves room for it
+    static constexpr uint32_t kSmem = kBytes + 1024 < 227 * 1024 ? kBytes + 1024 : 227 * 1024;
 };
 
 // Rows of stats per item: whole groups of 16 columns of the weights' MMA, the last ones zero.
@@ -59,88 +65,85 @@ __host__ __device__ constexpr size_t stats_stride(int rows) { return ((size_t)ro
 
 struct TcArgs {
     TreeArgs t;
-    int row_blocks, ctas;
+    int row_blocks, ctas, boundary, slot_rows;  // slot_rows: rows of a partial result
 };
 
 // ------------------------------------------------------------------ work ranges
-__device__ __forceinline__ int tiles_of(const TreeArgs &t, int b, int &length) {
-    length = __ldg(t.lengths + b);
+// An item counts as its tiles and `boundary` more, the time that a CTA loses at an
+// item's end (epilogue, new Q, an emptied pipeline) in tiles, so that ranges with
+// more ends hold fewer tiles.
+__device__ __forceinline__ int length_of(const TreeArgs &t, int b) { return b < t.batch ? __ldg(t.lengths + b) : 0; }
+__device__ __forceinline__ int tiles_of(const TreeArgs &t, int length) {
     if (length < 0 || length > t.capacity - t.seq) return 0;
     return (length + t.seq + kTileKeys - 1) / kTileKeys;
 }
-__device__ __forceinline__ long long range_tiles(long long total, int ctas) { return max(1ll, (total + ctas - 1) / ctas); }
+__device__ __forceinline__ int units_of(const TcArgs &a, int b) {
+    const int tiles = tiles_of(a.t, length_of(a.t, b));
+    return tiles ? tiles + a.boundary : 0;
+}
+// Units of a CTA's range; total: of all sequences' items.
+__device__ __forceinline__ long long range_units(const TcArgs &a, long long total) { return max(1ll, (total + a.ctas - 1) / a.ctas); }
 
 struct Segment {
     int b, hk, rb, first, last, tiles, length;  // key tiles [first, last) of the item's `tiles`
     __device__ __forceinline__ int count() const { return last - first; }
 };
 
-// The segments of a CTA's range, in order; every role walks the same sequence.
+// The segments of a CTA's range, in order; every role walks the same sequence. The
+// next sequence's length is read one sequence ahead: under the stream of K and V a
+// load takes microseconds.
 struct Segments {
-    int b, sub, tile;
+    int b, sub, unit, length, next_length;
     long long left;
     __device__ __forceinline__ bool next(const TcArgs &a, Segment &s) {
-        if (left <= 0) return false;
-        int length, tiles = tiles_of(a.t, b, length);
-        if (tile >= tiles) {
-            tile = 0;
-            if (++sub >= a.t.kv_heads * a.row_blocks || tiles == 0) {
-                sub = 0;
-                do {
+        while (left > 0) {
+            const int tiles = tiles_of(a.t, length), units = tiles ? tiles + a.boundary : 0;
+            if (unit >= units) {
+                unit = 0;
+                if (tiles == 0 || ++sub >= a.t.kv_heads * a.row_blocks) {
+                    sub = 0;
                     if (++b >= a.t.batch) return false;
-                    tiles = tiles_of(a.t, b, length);
-                } while (tiles == 0);
+                    length = next_length;
+                    next_length = length_of(a.t, b + 1);
+                }
+                continue;
             }
+            const int upto = (int)min((long long)units, unit + left);
+            s.b = b, s.hk = sub / a.row_blocks, s.rb = sub - s.hk * a.row_blocks;
+            s.first = min(unit, tiles), s.last = min(upto, tiles), s.tiles = tiles, s.length = length;
+            left -= upto - unit;
+            unit = upto;
+            if (s.count() > 0) return true;
         }
-        s.b = b, s.hk = sub / a.row_blocks, s.rb = sub - s.hk * a.row_blocks;
-        s.first = tile, s.last = (int)min((long long)tiles, tile + left), s.tiles = tiles, s.length = length;
-        left -= s.last - s.first;
-        tile = s.last;
-        return true;
+        return false;
     }
 };
 
-// Sum over the whole block of every thread's value (all threads get it). scratch: one long long per warp.
-__device__ __forceinline__ long long block_total(long long v, long long *scratch) {
-    const int warps = blockDim.x >> 5;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    long long s = 0;
-    for (int w = 0; w < warps; ++w) s += scratch[w];
-    return s;
-}
-
-// Tiles of all items, and of the items of sequences before `b`.
-__device__ __forceinline__ void count_tiles(const TcArgs &a, int b, long long *scratch, long long &total, long long &before) {
-    long long all = 0, less = 0;
-    for (int i = threadIdx.x; i < a.t.batch; i += blockDim.x) {
-        int length;
-        const int n = tiles_of(a.t, i, length);
-        all += n;
-        if (i < b) less += n;
-    }
-    const long long per = (long long)a.t.kv_heads * a.row_blocks;
-    total = block_total(all, scratch) * per;
-    before = b > 0 ? block_total(less, scratch) * per : 0;
-}
-
-// The CTA's range (whole block; also the barrier behind its set-up, TMEM allocation included).
+// The CTA's range (whole block; also the barrier behind its set-up, TMEM allocation
+// included). plan: 4 ints, scratch: a long long per warp.
 __device__ __forceinline__ Segments open_range(const TcArgs &a, int *plan, long long *scratch) {
     const TreeArgs &t = a.t;
-    const int lane = threadIdx.x & 31;
-    long long total, none;
-    count_tiles(a, 0, scratch, total, none);
-    const long long per = range_tiles(total, a.ctas), begin = per * blockIdx.x;
-    if (threadIdx.x < 32) {  // the first sequence whose tiles reach beyond `begin`
-        const long long items = (long long)t.kv_heads * a.row_blocks;
+    const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    long long mine = 0;
+    for (int i = threadIdx.x; i < t.batch; i += blockDim.x) {
+        const int units = units_of(a, i);
+        mine += units;
+        if (blockIdx.x == 0 && units == 0) atomicCAS(t.err, 0, kErrCacheLength);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) scratch[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    const long long items = (long long)t.kv_heads * a.row_blocks;
+    long long total = 0;
+    for (int w = 0; w < warps; ++w) total += scratch[w];
+    total *= items;
+    const long long per = range_units(a, total), begin = per * blockIdx.x;
+    if (threadIdx.x < 32) {  // the first sequence whose units reach beyond `begin`
         long long base = 0;
         for (int b0 = 0; b0 < t.batch && begin < total; b0 += 32) {
-            int length = 0;
-            const long long n = b0 + lane < t.batch ? tiles_of(t, b0 + lane, length) * items : 0;
-            long long upto = n;
+            const int units = b0 + lane < t.batch ? units_of(a, b0 + lane) : 0;
+            long long upto = units * items;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long x = __shfl_up_sync(0xffffffffu, upto, o);
@@ -148,26 +151,26 @@ __device__ __forceinline__ Segments open_range(const TcArgs &a, int *plan, long 
             }
             const uint32_t beyond = __ballot_sync(0xffffffffu, base + upto > begin);
             if (beyond && lane == __ffs(beyond) - 1) {
-                const long long into = begin - (base + upto - n);
-                const int tiles = (int)(n / items);
-                plan[0] = b0 + lane, plan[1] = (int)(into / tiles), plan[2] = (int)(into % tiles);
+                const long long into = begin - (base + upto - units * items);
+                plan[0] = b0 + lane, plan[1] = (int)(into / units), plan[2] = (int)(into % units);
             }
             if (beyond) break;
             base += __shfl_sync(0xffffffffu, upto, 31);
         }
-        if (blockIdx.x == 0)
-            for (int b = lane; b < t.batch; b += 32) {
-                int length;
-                if (tiles_of(t, b, length) == 0) atomicCAS(t.err, 0, kErrCacheLength);
-            }
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    return Segments{plan[0], plan[1], plan[2], begin < total ? min(per, total - begin) : 0};
+    if (begin >= total) return Segments{0, 0, 0, 0, 0, 0};
+    return Segments{plan[0], plan[1], plan[2], length_of(t, plan[0]), length_of(t, plan[0] + 1), min(per, total - begin)};
 }
 
 // ------------------------------------------------------------------ masks
+// The bits of word w that stand for drafts: bits beyond them may be anything.
+__device__ __forceinline__ uint32_t draft_bits(int w, int seq) {
+    const int n = seq - 32 * w;
+    return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
+}
 // Bit c of the result: the row sees column c of the tile whose first key lies `off`
 // slots before the first draft (off may be negative: the tile starts among the drafts).
 __device__ __forceinline__ void column_mask(const uint32_t (&bits)[4], int off, uint32_t (&mask)[4]) {
@@ -195,23 +198,18 @@ template <typename T>
 __device__ __forceinline__ uint32_t exponent_bits() { return std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u; }
 
 // Zeroes V rows that hold no entry, and the non-finite elements of drafted rows
-// (whose drafts are noted in `bad`). Thread `key` owns one row of the tile.
+// (whose drafts are noted in `bad`). A row's 64 elements are 128 contiguous bytes
+// (the swizzle permutes 16-byte units within them), so both are runs of memory that
+// the chain's 128 threads take 16 bytes at a time.
 template <int DP, typename T>
-__device__ __forceinline__ void clean_v(uint8_t *v, int key, int j0, int length, int seq, uint32_t *bad) {
-    using L = Layout<DP>;
-    const int draft = j0 + key - length;
-    if (draft < 0) return;
-    bool found = false;
+__device__ __forceinline__ void clean_v(uint8_t *v, int thread, int j0, int length, int seq, uint32_t *bad) {
+    const int draft0 = j0 - length;  // draft of the tile's first row
+    const int from = max(0, -draft0), upto = min(kTileKeys, seq - draft0);
 #pragma unroll 1
-    for (uint32_t at = key * 128; at < L::kTile; at += L::kChunk)
-#pragma unroll 1
-        for (int u = 0; u < 8; ++u) {
-            uint4 *p = reinterpret_cast<uint4 *>(v + at) + u;
-            if (draft >= seq) {
-                *p = make_uint4(0, 0, 0, 0);
-                continue;
-            }
-            uint4 x = *p;
+    for (uint32_t at = 0; at < (DP / 64) * 128 * 128; at += 128 * 128) {
+        for (int u = upto * 8 + thread; u < kTileKeys * 8; u += 128) *reinterpret_cast<uint4 *>(v + at + u * 16) = make_uint4(0, 0, 0, 0);
+        for (int u = from * 8 + thread; u < upto * 8; u += 128) {
+            uint4 x = *reinterpret_cast<uint4 *>(v + at + u * 16);
             uint32_t *w = reinterpret_cast<uint32_t *>(&x);
             const uint32_t e = exponent_bits<T>();
             bool hit = false;
@@ -220,9 +218,13 @@ __device__ __forceinline__ void clean_v(uint8_t *v, int key, int j0, int length,
                 if ((w[i] & e) == e) w[i] &= 0xffff0000u, hit = true;
                 if ((w[i] >> 16 & e) == e) w[i] &= 0x0000ffffu, hit = true;
             }
-            if (hit) *p = x, found = true;
+            if (hit) {
+                *reinterpret_cast<uint4 *>(v + at + u * 16) = x;
+                const int draft = draft0 + (u >> 3);
+                atomicOr(&bad[draft >> 5], 1u << (draft & 31));
+            }
         }
-    if (found) atomicOr(&bad[draft >> 5], 1u << (draft & 31));
+    }
 }
 
 // ------------------------------------------------------------------ kernel
@@ -230,7 +232,7 @@ template <int DP, typename T, bool kTwoTiles>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const TcArgs args) {
-    using L = Layout<DP>;
+    using L = Layout<DP, kTwoTiles>;
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t kIdescS = idesc_f32acc(kFmt, kFmt, false, false, kTileRows, kTileKeys);
     constexpr uint32_t kIdescO = idesc_f32acc(kFmt, kFmt, false, true, kTileRows, DP);
@@ -238,15 +240,20 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    if (smem + L::kBytes > smem_raw + L::kSmem) {
+        if (threadIdx.x == 0) atomicCAS(args.t.err, 0, kErrBadLaunch);
+        return;
+    }
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8, *o_free = bars + 10;
     uint64_t *x_full = bars + 12, *x_empty = bars + 13, *mma_done = bars + 14;
     uint64_t *full = bars + 16, *empty = bars + 16 + kStages;  // ring stages
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 36);
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 44);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     uint32_t *bad = tmem_slot + 4;  // [3][4]: drafts with non-finite V, by segment number modulo 3
     int *plan = reinterpret_cast<int *>(tmem_slot + 16);  // the range's first b, sub, tile and (64 bits) length
-    float2 *exchange = reinterpret_cast<float2 *>(smem + L::kExchange);
+    float2 *exchange = reinterpret_cast<float2 *>(smem + L::kExchange);  // [chain][row]
+    static_assert(16 + 2 * kStages <= 44, "barriers");
 
     const TreeArgs &ta = args.t;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -257,9 +264,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int t = 0; t < 2; ++t) {
             mbar_init(&q_full[t], 1); mbar_init(&q_empty[t], 1);
             mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 128);
-            mbar_init(&o_full[t], 1); mbar_init(&o_free[t], 128);
+            mbar_init(&o_full[t], 1); mbar_init(&o_free[t], kTwoTiles ? 128 : 256);
         }
-        mbar_init(x_full, 128); mbar_init(x_empty, 128); mbar_init(mma_done, 1);
+        mbar_init(x_full, 256); mbar_init(x_empty, 256); mbar_init(mma_done, 1);
         for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
         *abort_flag = 0;
         for (int i = 0; i < 12; ++i) bad[i] = 0;
@@ -271,6 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_relinquish();
     }
     Segments segments = open_range(args, plan, reinterpret_cast<long long *>(exchange));
+    grid_dependency_trigger();
     const uint32_t tmem = *tmem_slot;
     const uint32_t tmem_s[2] = {tmem, tmem + 128};
     const uint32_t tmem_o[2] = {tmem + 256, tmem + 384};
@@ -296,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!(ok = ok && mbar_wait(&q_empty[buffer], (use & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) return;
                     mbar_arrive_expect_tx(&q_full[buffer], L::kTile);
                     for (int c = 0; c < kDChunks; ++c)
-                        tma_load_3d(smem + L::kQ + buffer * L::kTile + c * L::kChunk, &tmQ, &q_full[buffer], c * 64, tile * kTileRows, bh);
+                        tma_load_3d(smem + buffer * L::kTile + c * L::kChunk, &tmQ, &q_full[buffer], c * 64, tile * kTileRows, bh);
                 };
                 if constexpr (kTwoTiles) {  // row tiles 2 rb and 2 rb + 1 (which may lie beyond the rows: zeros)
                     load_q(0, 2 * s.rb, q_loads);
@@ -324,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
             return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, err, code));
         };
-        const uint64_t dq0 = sdesc_sw128(smem_u32(smem + L::kQ), 16, 1024);
+        const uint64_t dq0 = sdesc_sw128(smem_u32(smem), 16, 1024);
         const uint64_t dk0 = sdesc_sw128(smem_u32(smem + L::kRing), 16, 1024);
         const uint64_t dv0 = sdesc_sw128(smem_u32(smem + L::kRing), L::kChunk, 1024);
         auto issue_s = [&](int t, int q_buffer, int stage) {
@@ -389,8 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int t = 0; t < 2; ++t) umma_commit(&q_empty[t]);
             } else {
                 const int q = qn & 1;
-                ok = wait(&q_full[q], qn >> 1 & 1, kErrWaitTmaFull);
-                ++qn;
+                ok = wait(&q_full[q], qn++ >> 1 & 1, kErrWaitTmaFull);
                 for (int i = 0; i < 2 && i < n && ready(); ++i) {
                     tc_fence_after();
                     issue_s(i, q, pos % kStages);
@@ -407,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tc_fence_after();
                         issue_s(t, q, pos % kStages);
                         release();
-                        if (i + 3 == n) umma_commit(&q_empty[q]);
+                        if (i + 3 == n) umma_commit(&q_empty[q]);  // the segment's last S: Q may be replaced
                     } else {
                         umma_commit(&o_full[t]);
                     }
@@ -435,8 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int i = 0; i < 4; ++i) bad[((sn + 1) % 3) * 4 + i] = 0;
             if (item_row < ta.rows)
                 for (int w = 0; w < 4; ++w)
-                    if (w < ta.words)  // no bits beyond the drafts: the slots behind them hold no entries
-                        bits[w] = __ldg(ta.tree + ((size_t)s.b * ta.seq + item_row % ta.seq) * ta.words + w) & (0xffffffffu >> max(0, 32 * (w + 1) - ta.seq));
+                    if (w < ta.words) bits[w] = __ldg(ta.tree + ((size_t)s.b * ta.seq + item_row % ta.seq) * ta.words + w);
             float m_used = -INFINITY, l_run = 0.0f;
             const int step = kTwoTiles ? 1 : 2;
             bool first = true;
@@ -461,8 +467,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_ld32f(ts + 96, sv + 96);
                     tmem_wait_ld();
                     if (masked) {
-                        uint32_t mask[4];
-                        column_mask(bits, s.length - j0, mask);
+                        uint32_t seen[4], mask[4];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) seen[w] = bits[w] & draft_bits(w, ta.seq);
+                        column_mask(seen, s.length - j0, mask);
 #pragma unroll
                         for (int k = 0; k < 128; ++k) sv[k] = mask[k >> 5] >> (k & 31) & 1 ? sv[k] : -INFINITY;
                     }
@@ -484,7 +492,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     m_used = m_new;
                     // a row that has seen nothing yet has maximum -inf: its weights are e^-inf = 0
-                    const float psum = store_p<kFmt, false, 128>(sv, c, m_used == -INFINITY ? 0.0f : m_used, ts);
+                    const float psum = masked ? store_p<kFmt, false, 128>(sv, c, m_used == -INFINITY ? 0.0f : m_used, ts)
+                                              : store_p<kFmt, kTwoTiles, 128, 2>(sv, c, m_used, ts);
                     if (!first && __any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll 1
                         for (int oc = 0; oc < DP; oc += 32) {
@@ -505,27 +514,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             ring += 2 * n;
             if (!ok) break;
             // ------------------------------------------------- the segment's rows
-            const bool both = !kTwoTiles && n > 1;  // chain 1 has sums to hand over
-            if (!kTwoTiles && t == 1) {
-                if (!both) continue;
-                ok = __all_sync(0xffffffffu, mbar_wait(x_empty, (xn++ & 1) ^ 1, abort_flag, err, kErrWaitAccEmpty));
+            const bool both = !kTwoTiles && n > 1;  // chain 1 has sums too
+            float f0 = 1.0f, f1 = 0.0f;             // factors of the two chains' sums
+            if constexpr (!kTwoTiles) {             // both chains' threads write half of the columns each
+                ok = __all_sync(0xffffffffu, mbar_wait(x_empty, (xn & 1) ^ 1, abort_flag, err, kErrWaitAccEmpty));
                 if (!ok) break;
-                exchange[row] = make_float2(m_used, l_run);
+                exchange[t * 128 + row] = make_float2(m_used, l_run);
                 mbar_arrive(x_full);
-                continue;
-            }
-            float f0 = 1.0f, f1 = 0.0f;  // factors of the two chains' sums
-            if (both) {
                 ok = __all_sync(0xffffffffu, mbar_wait(x_full, xn++ & 1, abort_flag, err, kErrWaitPv));
                 if (!ok) break;
-                const float2 other = exchange[row];
+                const float2 e0 = exchange[row], e1 = exchange[128 + row];
                 mbar_arrive(x_empty);
-                const float m = fmaxf(m_used, other.x), shift = m == -INFINITY ? 0.0f : m;
-                f0 = mufu_exp2(m_used - shift), f1 = mufu_exp2(other.x - shift);
-                l_run = l_run * f0 + other.y * f1;
-                m_used = m;
+                m_used = fmaxf(e0.x, e1.x);
+                const float shift = m_used == -INFINITY ? 0.0f : m_used;
+                f0 = mufu_exp2(e0.x - shift), f1 = mufu_exp2(e1.x - shift);
+                l_run = e0.y * f0 + e1.y * f1;
             }
-            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], on[t]++ & 1, abort_flag, err, kErrWaitPv));
+            const int o0 = kTwoTiles ? t : 0;
+            ok = __all_sync(0xffffffffu, mbar_wait(&o_full[o0], on[o0]++ & 1, abort_flag, err, kErrWaitPv));
             if (ok && both) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[1], on[1]++ & 1, abort_flag, err, kErrWaitPv));
             if (!ok) break;
             tc_fence_after();
@@ -534,18 +540,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (whole) f0 *= inv, f1 *= inv;
             uint32_t extra[4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) extra[w] = valid ? bad_now[w] & bits[w] : 0;
+            for (int w = 0; w < 4; ++w) extra[w] = valid ? bad_now[w] & bits[w] & draft_bits(w, ta.seq) : 0;
             const size_t slot = (size_t)blockIdx.x * 2 + (s.first == 0);
             const int g = item_row / ta.seq, tok = item_row - g * ta.seq;
             T *out = static_cast<T *>(ta.out) + (((size_t)s.b * ta.seq + tok) * ta.kv_heads * ta.group + s.hk * ta.group + g) * ta.dim;
-            constexpr int kSlotRows = kTwoTiles ? 256 : 128;
-            const int slot_row = kTwoTiles ? t * 128 + row : row;
-            float4 *part = reinterpret_cast<float4 *>(ta.part_o) + slot * (DP / 4) * kSlotRows + slot_row;
+            const int slot_row = kTwoTiles ? t * 128 + row : row, slot_rows = args.slot_rows;
+            float4 *part = reinterpret_cast<float4 *>(ta.part_o) + slot * (DP / 4) * slot_rows + slot_row;
+            constexpr int kColumns = kTwoTiles ? DP : DP / 2;
+            const int first_column = kTwoTiles ? 0 : t * kColumns;
             if (live) {
 #pragma unroll 1
-                for (int oc = 0; oc < DP; oc += 32) {
+                for (int oc = first_column; oc < first_column + kColumns; oc += 32) {
                     float r[32];
-                    tmem_ld32f(to + oc, r);
+                    tmem_ld32f(tmem_o[o0] + lane_off + oc, r);
                     tmem_wait_ld();
                     if (both) {
                         float x[32];
@@ -581,16 +588,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                     } else if (valid) {  // [dim / 4][row] so that a warp's rows are one run of memory
 #pragma unroll
                         for (int k = 0; k < 32; k += 4)
-                            part[(size_t)((oc + k) / 4) * kSlotRows] = make_float4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+                            part[(size_t)((oc + k) / 4) * slot_rows] = make_float4(r[k], r[k + 1], r[k + 2], r[k + 3]);
                     }
                     __syncwarp();
                 }
             }
             tc_fence_before();
-            mbar_arrive(&o_free[t]);
+            mbar_arrive(&o_free[o0]);
             if (both) mbar_arrive(&o_free[1]);
-            if (valid) {
-                if (!whole) ta.part_ml[slot * kSlotRows + slot_row] = make_float2(m_used, l_run);
+            if (valid && (kTwoTiles || t == 0)) {
+                if (!whole) ta.part_ml[slot * slot_rows + slot_row] = make_float2(m_used, l_run);
                 else if (ta.stats) ta.stats[(size_t)bh * stats_stride(ta.rows) + item_row] = make_float2(m_used == -INFINITY ? 0.0f : m_used, inv);
             }
         }
@@ -611,33 +618,46 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Joins the parts of items that several CTAs share: a block takes 32 rows of an
-// item, a thread one row and four columns; parts in range order.
-template <int DP, typename T, int kSlotRows>
-__global__ void __launch_bounds__(8 * DP) tree_join_tc(const TcArgs a) {
-    __shared__ long long scratch[32];
+// Joins the parts of items that several CTAs share, in range order. A thread takes
+// one row and four columns: consecutive threads, consecutive memory of every part.
+constexpr int kJoinThreads = 256;
+
+template <int DP, typename T>
+__global__ void __launch_bounds__(kJoinThreads) tree_join_tc(const TcArgs a, int blocks) {
+    __shared__ long long counts[2];
     const TreeArgs &t = a.t;
-    const int subs = t.kv_heads * a.row_blocks, blocks = kSlotRows / 32;
+    const int subs = t.kv_heads * a.row_blocks;
     const int item = blockIdx.x / blocks, b = item / subs, sub = item - b * subs, hk = sub / a.row_blocks, rb = sub - hk * a.row_blocks;
-    const int lane = threadIdx.x & 31, col = threadIdx.x >> 5, slot_row = (blockIdx.x - item * blocks) * 32 + lane, row = rb * kSlotRows + slot_row;
-    int length;
-    const int tiles = tiles_of(t, b, length);
-    long long total, before;
-    count_tiles(a, b, scratch, total, before);
-    if (tiles == 0 || row >= t.rows) return;
-    const long long per = range_tiles(total, a.ctas), begin = before + (long long)sub * tiles;
+    grid_dependency_trigger();
+    if (threadIdx.x < 32) {
+        long long all = 0, before = 0;
+        for (int i = threadIdx.x; i < t.batch; i += 32) {
+            const int n = units_of(a, i);
+            all += n;
+            if (i < b) before += n;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o), before += __shfl_xor_sync(0xffffffffu, before, o);
+        if (threadIdx.x == 0) counts[0] = all, counts[1] = before;
+    }
+    __syncthreads();
+    const int at = (blockIdx.x - item * blocks) * kJoinThreads + threadIdx.x, col = at / a.slot_rows, slot_row = at - col * a.slot_rows;
+    const int row = rb * a.slot_rows + slot_row;
+    const int tiles = tiles_of(t, length_of(t, b));
+    grid_dependency_wait();  // in every block: this grid's end stands for the one's before it
+    const long long per = range_units(a, counts[0] * subs), begin = counts[1] * subs + (long long)sub * (tiles + a.boundary);
     const int c0 = (int)(begin / per), c1 = (int)((begin + tiles - 1) / per);
-    if (c0 == c1) return;  // written whole
+    if (tiles == 0 || c0 == c1 || row >= t.rows || col * 4 >= DP) return;  // c0 == c1: written whole
     auto slot = [&](int c) { return (size_t)c * 2 + (c == c0); };
     float m = -INFINITY, l = 0.0f;
-    for (int c = c0; c <= c1; ++c) m = fmaxf(m, t.part_ml[slot(c) * kSlotRows + slot_row].x);
+    for (int c = c0; c <= c1; ++c) m = fmaxf(m, t.part_ml[slot(c) * a.slot_rows + slot_row].x);
     const float shift = m == -INFINITY ? 0.0f : m;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4 *part = reinterpret_cast<const float4 *>(t.part_o) + (size_t)col * kSlotRows + slot_row;
+    const float4 *part = reinterpret_cast<const float4 *>(t.part_o) + at;
 #pragma unroll 4
     for (int c = c0; c <= c1; ++c) {
-        const float2 ml = t.part_ml[slot(c) * kSlotRows + slot_row];
-        const float4 x = part[slot(c) * (DP / 4) * kSlotRows];
+        const float2 ml = t.part_ml[slot(c) * a.slot_rows + slot_row];
+        const float4 x = part[slot(c) * (DP / 4) * a.slot_rows];
         const float w = exp2f(ml.x - shift);
         l = fmaf(ml.y, w, l);
         o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
@@ -660,7 +680,7 @@ __global__ void __launch_bounds__(8 * DP) tree_join_tc(const TcArgs a) {
 // Bound by K's second read and by one exponential per (row, key).
 //   warp 0 TMA (Q rows and their stats per segment, K tiles through a ring),
 //   warp 1 MMA into two buffers, warps 2-5 and 6-9 take the tiles in turn.
-constexpr int kWeightRows = 256;
+constexpr int kWeightRows = 256, kWeightsBoundary = 2;
 
 template <int DP>
 struct WeightsLayout {
@@ -715,6 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_prefetch_desc(&tmQ);
             tma_prefetch_desc(&tmK);
             bool ok = true;
+            grid_dependency_wait();  // the rows' stats
             while (ok && segments.next(args, s)) {
                 const int bh = s.b * ta.kv_heads + s.hk;
                 for (int r0 = 0; ok && r0 < ta.rows; r0 += kWeightRows) {
@@ -862,9 +883,22 @@ bool row_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, uint64_t
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Launches `kernel` so that its blocks may start, up to grid_dependency_wait, while
+// the kernel before it on the stream still runs.
+template <typename... P, typename... A>
+cudaError_t launch_after(cudaStream_t st, void (*kernel)(P...), int grid, int block, size_t smem, A &&...args) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(grid), config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = st;
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &early, config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, kernel, args...);
+}
+
 template <int DP, typename T, bool kTwoTiles>
 LaunchFn tc_launch(Context *ctx, const Spec &s) {
-    using L = Layout<DP>;
+    using L = Layout<DP, kTwoTiles>;
     auto kernel = tree_tc_kernel<DP, T, kTwoTiles>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem) != cudaSuccess)
         throw IrError("cannot reserve shared memory for the tcgen05 attention_tree");
@@ -876,10 +910,13 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
     // one CTA per SM, none for which even full caches have no tile
     const unsigned __int128 most = (unsigned __int128)heads * base.row_blocks * ((capacity + kTileKeys - 1) / kTileKeys);
     base.ctas = most < (unsigned __int128)ctx->sm_count ? (int)most : ctx->sm_count;
-    const long long join_blocks = (long long)heads * base.row_blocks * (kSlotRows / 32);
+    base.boundary = kBoundary;
+    base.slot_rows = rows >= (uint64_t)kSlotRows ? kSlotRows : (int)((rows + 7) / 8 * 8);
+    const int item_blocks = (base.slot_rows * (DP / 4) + kJoinThreads - 1) / kJoinThreads;
+    const long long join_blocks = (long long)heads * base.row_blocks * item_blocks;
     if (join_blocks > INT_MAX) throw IrError("attention_tree too large for one launch");
     const bool weights = s.weights;
-    const size_t stats = (heads * stats_stride((int)rows) * sizeof(float2) + 255) / 256 * 256, slots = (size_t)base.ctas * 2 * kSlotRows;
+    const size_t stats = (heads * stats_stride((int)rows) * sizeof(float2) + 255) / 256 * 256, slots = (size_t)base.ctas * 2 * base.slot_rows;
     auto ws = kernel_workspace(stats + slots * (sizeof(float2) + DP * sizeof(float)), "attention_tree partial results");
     base.t.stats = weights ? static_cast<float2 *>(ws.get()) : nullptr;
     base.t.part_o = reinterpret_cast<float *>(static_cast<char *>(ws.get()) + stats);
@@ -896,12 +933,13 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
         if (!row_map(&mq, dt, b[0], heads, rows, dim) || !row_map(&mk, dt, b[1], heads, capacity, dim) || !row_map(&mv, dt, b[2], heads, capacity, dim))
             return cudaErrorInvalidValue;
         kernel<<<a.ctas, kThreads, L::kSmem, st>>>(mq, mk, mv, a);
-        tree_join_tc<DP, T, kSlotRows><<<(int)join_blocks, 8 * DP, 0, st>>>(a);
-        if (weights) {
-            a.row_blocks = 1;
-            weights_kernel<<<a.ctas, kThreads, W::kSmem, st>>>(mq, mk, a);
+        cudaError_t e = launch_after(st, tree_join_tc<DP, T>, (int)join_blocks, kJoinThreads, 0, a, item_blocks);
+        if (weights && e == cudaSuccess) {
+            TcArgs w = a;
+            w.row_blocks = 1, w.boundary = kWeightsBoundary;
+            e = launch_after(st, weights_kernel, a.ctas, kThreads, W::kSmem, mq, mk, w);
         }
-        return cudaGetLastError();
+        return e == cudaSuccess ? cudaGetLastError() : e;
     };
 }
 
