@@ -883,19 +883,6 @@ bool row_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, uint64_t
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Launches `kernel` so that its blocks may start, up to grid_dependency_wait, while
-// the kernel before it on the stream still runs.
-template <typename... P, typename... A>
-cudaError_t launch_after(cudaStream_t st, void (*kernel)(P...), int grid, int block, size_t smem, A &&...args) {
-    cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid), config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = st;
-    cudaLaunchAttribute early{};
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.attrs = &early, config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, kernel, args...);
-}
-
 template <int DP, typename T, bool kTwoTiles>
 LaunchFn tc_launch(Context *ctx, const Spec &s) {
     using L = Layout<DP, kTwoTiles>;

@@ -20,6 +20,12 @@
 // a fraction of a turn in 64-bit fixed point (theta / 2 pi as a 0.64 fraction, times
 // the position, modulo 2^64): exact reduction at every position, where an FP32
 // product is off by 0.004 rad at position 100,000.
+//
+// Both kernels are bound by HBM (each row read and written once). A warp takes
+// heads of one token, 32 / kLanes rows at a time, 8 elements a lane, and forms the
+// token's sines and cosines once in registers for all of them; no block barrier, no
+// shared memory in the loop. Rows of several rounds are loaded before the first is
+// worked on, so that enough bytes are in flight.
 #include <cmath>
 #include <vector>
 
@@ -38,46 +44,144 @@ struct RopeArgs {
     void *q, *k, *v;        // outputs (gradient: dq, dk, dv, inputs)
     void *dqkv;
     float *partial;         // gradient: [block][2][dim] sums of the norm weights' gradients
-    int batch, seq, heads, kv_heads, dim, rotary, interleaved, norm, rows;  // rows: of k and v per head
+    int batch, seq, heads, kv_heads, dim, rotary, norm, rows;  // rows: of k and v per head
+    int parts;              // warps that share a token's heads
     float epsilon, gain;
     int *err;
 };
 
-// 8 consecutive elements: 16 bytes of a 16-bit type, 32 of FP32.
-__device__ __forceinline__ void load8(const float *p, float (&x)[8]) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(p)), b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+// How a lane's 8 elements lie in the head and find their partners.
+//   kHalves      rotated lanes hold 4 of the first half and their 4 partners of the
+//                second, two pieces rotary / 2 apart (rotary a multiple of 8); the
+//                others 8 in a row
+//   kNeighbours  8 in a row, partners beside each other
+//   kGeneral     8 in a row, partners through the warp's rows in shared memory
+//                (halves of any length)
+enum Pairing { kHalves, kNeighbours, kGeneral };
+
+template <typename T>
+struct Vec4;  // 4 elements as loaded
+template <>
+struct Vec4<float> { using type = float4; };
+template <>
+struct Vec4<__nv_bfloat16> { using type = uint2; };
+template <>
+struct Vec4<__half> { using type = uint2; };
+
+__device__ __forceinline__ void widen(const float4 &u, float *x, float) { x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w; }
+__device__ __forceinline__ void widen(const uint2 &u, float *x, __nv_bfloat16) {
+    x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
+    x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
 }
-__device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&x)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
-    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __bfloat1622float2(h[i]);
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
+__device__ __forceinline__ void widen(const uint2 &u, float *x, __half) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+__device__ __forceinline__ float4 narrow(const float *x, float) { return make_float4(x[0], x[1], x[2], x[3]); }
+__device__ __forceinline__ uint2 narrow(const float *x, __nv_bfloat16) { return make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])); }
+__device__ __forceinline__ uint2 narrow(const float *x, __half) { return make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3])); }
+
+// A lane's elements of a row: 4 from offset a, 4 from offset b.
+template <typename T>
+struct Row8 {
+    typename Vec4<T>::type lo, hi;
+};
+struct Place {
+    int a, b;
+    bool live;
+};
+template <typename T, Pairing kPair>
+__device__ __forceinline__ Row8<T> load_row(const T *p, Place at) {
+    using V = typename Vec4<T>::type;
+    Row8<T> r{};
+    if (!at.live) return r;
+    if constexpr (kPair != kHalves && sizeof(T) == 2) {
+        const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p + at.a));
+        r.lo = make_uint2(u.x, u.y), r.hi = make_uint2(u.z, u.w);
+    } else {
+        r.lo = __ldcs(reinterpret_cast<const V *>(p + at.a)), r.hi = __ldcs(reinterpret_cast<const V *>(p + at.b));
+    }
+    return r;
+}
+template <typename T, Pairing kPair>
+__device__ __forceinline__ void store_row(T *p, Place at, const Row8<T> &r) {
+    using V = typename Vec4<T>::type;
+    if (!at.live) return;
+    if constexpr (kPair != kHalves && sizeof(T) == 2) {
+        *reinterpret_cast<uint4 *>(p + at.a) = make_uint4(r.lo.x, r.lo.y, r.hi.x, r.hi.y);
+    } else {
+        *reinterpret_cast<V *>(p + at.a) = r.lo;
+        *reinterpret_cast<V *>(p + at.b) = r.hi;
     }
 }
-__device__ __forceinline__ void load8(const __half *p, float (&x)[8]) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(p));
-    const __half2 *h = reinterpret_cast<const __half2 *>(&u);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(h[i]);
-        x[2 * i] = f.x, x[2 * i + 1] = f.y;
-    }
+template <typename T>
+__device__ __forceinline__ void widen8(const Row8<T> &r, float (&x)[8]) {
+    widen(r.lo, x, T{});
+    widen(r.hi, x + 4, T{});
 }
-__device__ __forceinline__ void store8(float *p, const float (&x)[8]) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-}
-__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float (&x)[8]) {
-    *reinterpret_cast<uint4 *>(p) = make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
-}
-__device__ __forceinline__ void store8(__half *p, const float (&x)[8]) {
-    *reinterpret_cast<uint4 *>(p) = make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+template <typename T>
+__device__ __forceinline__ Row8<T> narrow8(const float (&x)[8]) {
+    return Row8<T>{narrow(x, T{}), narrow(x + 4, T{})};
 }
 
-// A warp holds 32 / kLanes head rows, kLanes lanes each, 8 elements a lane.
+template <Pairing kPair>
+__device__ __forceinline__ Place lane_place(int chunk, int dim, int rotary) {
+    Place at{8 * chunk, 8 * chunk + 4, 8 * chunk < dim};
+    if (kPair == kHalves && 8 * chunk < rotary) at.a = 4 * chunk, at.b = 4 * chunk + rotary / 2;
+    return at;
+}
+
+// Cosines and sines of the lane's pairs at a position; passed elements turn by 0.
+// kGeneral: for each of its 8 elements, y = x c + partner s.
+template <Pairing kPair>
+struct Angles {
+    static constexpr int kCount = kPair == kGeneral ? 8 : 4;
+    float c[kCount], s[kCount];
+    __device__ __forceinline__ void set(const RopeArgs &a, int chunk, int position, float sign) {
+        const int half = a.rotary / 2;
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            const int e = kCount * chunk + i;  // pair, or element
+            const int pair = kPair == kGeneral && e >= half ? e - half : e;
+            c[i] = 1.0f, s[i] = 0.0f;
+            if (pair < half) {
+                const uint64_t turn = (uint64_t)(int64_t)position * __ldg(a.turns + pair);
+                sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s[i], &c[i]);
+                c[i] *= a.gain, s[i] *= kPair == kGeneral && e < half ? -sign * a.gain : sign * a.gain;
+            }
+        }
+    }
+    // x: the lane's elements; row: the warp row's elements in shared memory (kGeneral)
+    __device__ __forceinline__ void turn(float (&x)[8], float *row, int chunk, int half) const {
+        if constexpr (kPair == kHalves) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = x[i] * c[i] - x[4 + i] * s[i];
+                x[4 + i] = x[i] * s[i] + x[4 + i] * c[i];
+                x[i] = u;
+            }
+        } else if constexpr (kPair == kNeighbours) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
+                x[2 * i + 1] = x[2 * i] * s[i] + x[2 * i + 1] * c[i];
+                x[2 * i] = u;
+            }
+        } else {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) row[8 * chunk + i] = x[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = 8 * chunk + i;
+                if (e < 2 * half) x[i] = x[i] * c[i] + row[e < half ? e + half : e - half] * s[i];
+            }
+        }
+    }
+};
+
+// Sum over the kLanes lanes of a row.
 template <int kLanes>
 __device__ __forceinline__ float row_sum(float v) {
 #pragma unroll
@@ -85,169 +189,168 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// Turns the lane's 8 elements (first: index of the first) by the token's angles;
-// sign -1 turns back. The halves' partners are fetched through the warp's rows in
-// shared memory.
+// The rounds of a warp: a token's heads in the order queries, keys, values, 32 /
+// kLanes heads of one kind a round, the rounds of a token dealt evenly to its `parts`
+// warps.
 template <int kLanes>
-__device__ __forceinline__ void turn8(const RopeArgs &a, const float2 *cs, float *warp_rows, int row, int first, float sign, float (&x)[8]) {
-    if (a.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 8; i += 2)
-            if (first + i < a.rotary) {
-                const float2 t = cs[(first + i) >> 1];
-                const float u = x[i] * t.x - sign * (x[i + 1] * t.y), w = sign * (x[i] * t.y) + x[i + 1] * t.x;
-                x[i] = u, x[i + 1] = w;
-            }
-        return;
+struct Rounds {
+    int q, k, total;  // rounds of queries, of queries and keys, of all
+    __device__ __forceinline__ Rounds(const RopeArgs &a) {
+        constexpr int per = 32 / kLanes;
+        q = (a.heads + per - 1) / per;
+        k = q + (a.kv_heads + per - 1) / per;
+        total = k + k - q;
     }
-    float *mine = warp_rows + row * (kLanes * 8);
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) mine[first + i] = x[i];
-    __syncwarp();
-    const int half = a.rotary >> 1;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int e = first + i;
-        if (e < half) {
-            const float2 t = cs[e];
-            x[i] = x[i] * t.x - sign * (mine[e + half] * t.y);
-        } else if (e < a.rotary) {
-            const float2 t = cs[e - half];
-            x[i] = x[i] * t.x + sign * (mine[e - half] * t.y);
-        }
-    }
-}
+};
 
-__device__ __forceinline__ void token_angles(const RopeArgs &a, int position, float2 *cs) {
-    for (int i = threadIdx.x; i < a.rotary / 2; i += kThreads) {
-        const uint64_t turn = (uint64_t)(int64_t)position * a.turns[i];
-        float s, c;
-        sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
-        cs[i] = make_float2(c * a.gain, s * a.gain);
-    }
-}
-
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
-    __shared__ float2 cs[128];
-    __shared__ float rows[kWarps][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane / kLanes, first = (lane % kLanes) * 8;
-    const bool live = first < a.dim;
-    const int total = a.heads + 2 * a.kv_heads;
-    float wq[8], wk[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) wq[i] = wk[i] = 1.0f;
-    if (a.norm && live) {
-        load8(static_cast<const T *>(a.q_weight) + first, wq);
-        load8(static_cast<const T *>(a.k_weight) + first, wk);
-    }
-    for (int token = blockIdx.x; token < a.batch * a.seq; token += gridDim.x) {
+template <typename T, int kLanes, Pairing kPair>
+__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
+    constexpr int kPer = 32 / kLanes, kAhead = 4;  // rounds loaded at a time
+    __shared__ float shared_rows[kPair == kGeneral ? kWarps : 1][256];
+    const int lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
+    const Place at = lane_place<kPair>(chunk, a.dim, a.rotary);
+    const Rounds<kLanes> rounds(a);
+    const int total_heads = a.heads + 2 * a.kv_heads;
+    float *row = shared_rows[kPair == kGeneral ? threadIdx.x >> 5 : 0] + sub * (kLanes * 8);
+    const long long items = (long long)a.batch * a.seq * a.parts;
+    for (long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * kWarps) {
+        const int token = (int)(item / a.parts), part = (int)(item - (long long)token * a.parts);
         const int b = token / a.seq, t = token - b * a.seq;
-        const int start = a.starts ? a.starts[b] : 0;
+        const int r0 = (int)((long long)rounds.total * part / a.parts), r1 = (int)((long long)rounds.total * (part + 1) / a.parts);
+        const int start = a.starts ? __ldg(a.starts + b) : 0, position = __ldg(a.positions + token);
         if (start < 0 || start > a.rows - a.seq) {
-            if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrCacheLength);
+            if (lane == 0) atomicCAS(a.err, 0, kErrCacheLength);
             continue;
         }
-        __syncthreads();
-        token_angles(a, a.positions[token], cs);
-        __syncthreads();
-        for (int h0 = warp * (32 / kLanes); h0 < total; h0 += kWarps * (32 / kLanes)) {
-            const int h = h0 + sub;
-            const bool on = live && h < total;
-            float x[8] = {};
-            if (on) load8(static_cast<const T *>(a.qkv) + ((size_t)token * total + h) * a.dim + first, x);
-            if (h0 < a.heads + a.kv_heads) {  // some row of the warp is a query or a key
-                float y[8], scale = 1.0f;
-                if (a.norm) {
-                    float ss = 0.0f;
+        const T *in = static_cast<const T *>(a.qkv) + (size_t)token * total_heads * a.dim;
+        // head of the packed row and its destination in round r; -1 where the round has no head for this lane
+        auto head_of = [&](int r, T *&out) {
+            int h;
+            if (r < rounds.q) {
+                h = r * kPer + sub;
+                out = static_cast<T *>(a.q) + (((size_t)b * a.heads + h) * a.seq + t) * a.dim;
+                return h < a.heads ? h : -1;
+            }
+            const bool key = r < rounds.k;
+            h = (r - (key ? rounds.q : rounds.k)) * kPer + sub;
+            out = static_cast<T *>(key ? a.k : a.v) + (((size_t)b * a.kv_heads + h) * a.rows + start + t) * a.dim;
+            return h < a.kv_heads ? a.heads + (key ? 0 : a.kv_heads) + h : -1;
+        };
+        Angles<kPair> angles;
+        float w[8];
+        int weights = -1;  // whose weights w holds: 0 queries, 1 keys
+        for (int r = r0; r < r1; r += kAhead) {
+            Row8<T> x[kAhead];
+            T *out[kAhead];
+            bool on[kAhead];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-                    scale = rsqrtf(row_sum<kLanes>(ss) / (float)a.dim + a.epsilon);
+            for (int u = 0; u < kAhead; ++u) {
+                const int h = head_of(min(r + u, r1 - 1), out[u]);
+                on[u] = h >= 0 && r + u < r1;
+                x[u] = load_row<T, kPair>(in + (size_t)max(h, 0) * a.dim, Place{at.a, at.b, at.live && on[u]});
+            }
+            if (r == r0 && r < rounds.k) angles.set(a, chunk, position, 1.0f);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (r + u >= r1) break;
+                if (r + u < rounds.k) {  // a query or a key
+                    const int kind = r + u < rounds.q ? 0 : 1;
+                    if (a.norm && kind != weights) {
+                        weights = kind;
+                        widen8(load_row<T, kPair>(static_cast<const T *>(kind ? a.k_weight : a.q_weight), at), w);
+                    }
+                    float y[8];
+                    widen8(x[u], y);
+                    if (a.norm) {
+                        float ss = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+                        const float scale = rsqrtf(row_sum<kLanes>(ss) / (float)a.dim + a.epsilon);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) y[i] *= scale * w[i];
+                    }
+                    angles.turn(y, row, chunk, a.rotary / 2);
+                    x[u] = narrow8<T>(y);
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = x[i] * scale * (h < a.heads ? wq[i] : wk[i]);
-                turn8<kLanes>(a, cs, rows[warp], sub, first, 1.0f, y);
-                if (h < a.heads + a.kv_heads)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = y[i];
+                store_row<T, kPair>(out[u], Place{at.a, at.b, at.live && on[u]}, x[u]);
             }
-            if (!on) continue;
-            T *out;
-            if (h < a.heads) out = static_cast<T *>(a.q) + (((size_t)b * a.heads + h) * a.seq + t) * a.dim;
-            else {
-                const bool key = h < a.heads + a.kv_heads;
-                const int hk = h - a.heads - (key ? 0 : a.kv_heads);
-                out = static_cast<T *>(key ? a.k : a.v) + (((size_t)b * a.kv_heads + hk) * a.rows + start + t) * a.dim;
-            }
-            store8(out + first, x);
         }
     }
 }
 
-template <typename T, int kLanes>
-__global__ void __launch_bounds__(kThreads) rope_grad_kernel(const RopeArgs a) {
-    __shared__ float2 cs[128];
-    __shared__ float rows[kWarps][256];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane / kLanes, first = (lane % kLanes) * 8;
-    const bool live = first < a.dim;
-    const int total = a.heads + 2 * a.kv_heads;
+template <typename T, int kLanes, Pairing kPair>
+__global__ void __launch_bounds__(kThreads, 2) rope_grad_kernel(const RopeArgs a) {
+    constexpr int kPer = 32 / kLanes, kAhead = 4;
+    __shared__ float shared_rows[kWarps][256];
+    const int lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
+    const Place at = lane_place<kPair>(chunk, a.dim, a.rotary);
+    const Rounds<kLanes> rounds(a);
+    const int total_heads = a.heads + 2 * a.kv_heads;
+    float *row = shared_rows[threadIdx.x >> 5] + sub * (kLanes * 8);
     float wq[8], wk[8], dwq[8] = {}, dwk[8] = {};
 #pragma unroll
     for (int i = 0; i < 8; ++i) wq[i] = wk[i] = 1.0f;
-    if (a.norm && live) {
-        load8(static_cast<const T *>(a.q_weight) + first, wq);
-        load8(static_cast<const T *>(a.k_weight) + first, wk);
+    if (a.norm) {
+        widen8(load_row<T, kPair>(static_cast<const T *>(a.q_weight), at), wq);
+        widen8(load_row<T, kPair>(static_cast<const T *>(a.k_weight), at), wk);
     }
-    for (int token = blockIdx.x; token < a.batch * a.seq; token += gridDim.x) {
+    const long long items = (long long)a.batch * a.seq * a.parts;
+    for (long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * kWarps) {
+        const int token = (int)(item / a.parts), part = (int)(item - (long long)token * a.parts);
         const int b = token / a.seq, t = token - b * a.seq;
-        __syncthreads();
-        token_angles(a, a.positions[token], cs);
-        __syncthreads();
-        for (int h0 = warp * (32 / kLanes); h0 < total; h0 += kWarps * (32 / kLanes)) {
-            const int h = h0 + sub;
-            const bool on = live && h < total, query = h < a.heads, value = h >= a.heads + a.kv_heads;
-            const size_t at = ((size_t)token * total + h) * a.dim + first;
-            float g[8] = {};
-            if (on) {
-                const void *from = query ? a.q : value ? a.v : a.k;
-                const int heads = query ? a.heads : a.kv_heads, index = query ? h : h - a.heads - (value ? a.kv_heads : 0);
-                load8(static_cast<const T *>(from) + (((size_t)b * heads + index) * a.seq + t) * a.dim + first, g);
+        const int r0 = (int)((long long)rounds.total * part / a.parts), r1 = (int)((long long)rounds.total * (part + 1) / a.parts);
+        const int position = __ldg(a.positions + token);
+        const size_t packed = (size_t)token * total_heads * a.dim;
+        Angles<kPair> angles;
+        for (int r = r0; r < r1; r += kAhead) {
+            Row8<T> g[kAhead], x[kAhead];
+            size_t to[kAhead];
+            bool on[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int rr = min(r + u, r1 - 1), kind = rr < rounds.q ? 0 : rr < rounds.k ? 1 : 2;
+                const int h = (rr - (kind == 0 ? 0 : kind == 1 ? rounds.q : rounds.k)) * kPer + sub, heads = kind ? a.kv_heads : a.heads;
+                on[u] = h < heads && r + u < r1;
+                const Place here{at.a, at.b, at.live && on[u]};
+                const T *from = static_cast<const T *>(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
+                to[u] = packed + (size_t)(h + (kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads)) * a.dim;
+                g[u] = load_row<T, kPair>(from + (((size_t)b * heads + h) * a.seq + t) * a.dim, here);
+                if (a.norm && kind < 2) x[u] = load_row<T, kPair>(static_cast<const T *>(a.qkv) + to[u], here);
             }
-            if (h0 < a.heads + a.kv_heads) {
-                float d[8];
+            if (r == r0 && r < rounds.k) angles.set(a, chunk, position, -1.0f);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) d[i] = g[i];
-                turn8<kLanes>(a, cs, rows[warp], sub, first, -1.0f, d);
-                if (a.norm) {
-                    float x[8] = {}, ss = 0.0f, ux = 0.0f;
-                    if (on && !value) load8(static_cast<const T *>(a.qkv) + at, x);
+            for (int u = 0; u < kAhead; ++u) {
+                if (r + u >= r1) break;
+                if (r + u < rounds.k) {
+                    const bool query = r + u < rounds.q;
+                    float d[8];
+                    widen8(g[u], d);
+                    angles.turn(d, row, chunk, a.rotary / 2);
+                    if (a.norm) {
+                        float y[8], ss = 0.0f, ux = 0.0f;
+                        widen8(x[u], y);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-                    const float scale = rsqrtf(row_sum<kLanes>(ss) / (float)a.dim + a.epsilon);
+                        for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+                        const float scale = rsqrtf(row_sum<kLanes>(ss) / (float)a.dim + a.epsilon);
+                        if (query) {  // lanes without a row hold zeros
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        x[i] *= scale;
-                        if (on && query) dwq[i] = fmaf(d[i], x[i], dwq[i]);
-                        if (on && !query && !value) dwk[i] = fmaf(d[i], x[i], dwk[i]);
-                        d[i] *= query ? wq[i] : wk[i];
-                        ux = fmaf(d[i], x[i], ux);
+                            for (int i = 0; i < 8; ++i) y[i] *= scale, dwq[i] = fmaf(d[i], y[i], dwq[i]), d[i] *= wq[i], ux = fmaf(d[i], y[i], ux);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) y[i] *= scale, dwk[i] = fmaf(d[i], y[i], dwk[i]), d[i] *= wk[i], ux = fmaf(d[i], y[i], ux);
+                        }
+                        const float mean = row_sum<kLanes>(ux) / (float)a.dim;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) d[i] = scale * (d[i] - y[i] * mean);
                     }
-                    const float mean = row_sum<kLanes>(ux) / (float)a.dim;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) d[i] = scale * (d[i] - x[i] * mean);
+                    g[u] = narrow8<T>(d);
                 }
-                if (!value)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) g[i] = d[i];
+                store_row<T, kPair>(static_cast<T *>(a.dqkv) + to[u], Place{at.a, at.b, at.live && on[u]}, g[u]);
             }
-            if (on) store8(static_cast<T *>(a.dqkv) + at, g);
         }
     }
     if (!a.norm) return;
-    // the block's sums, rows of the warp first, then warps, each in a fixed order
+    // the block's sums: rows of the warp first, then the warps, each in a fixed order
     for (int which = 0; which < 2; ++which) {
         float(&dw)[8] = which ? dwk : dwq;
         __syncthreads();
@@ -255,12 +358,13 @@ __global__ void __launch_bounds__(kThreads) rope_grad_kernel(const RopeArgs a) {
         for (int i = 0; i < 8; ++i) {
 #pragma unroll
             for (int o = kLanes; o < 32; o <<= 1) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-            if (sub == 0 && live) rows[warp][first + i] = dw[i];
+            if (sub == 0 && at.live) shared_rows[threadIdx.x >> 5][(i < 4 ? at.a : at.b) + (i & 3)] = dw[i];
         }
         __syncthreads();
         for (int e = threadIdx.x; e < a.dim; e += kThreads) {
             float s = 0.0f;
-            for (int w = 0; w < kWarps; ++w) s += rows[w][e];
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) s += shared_rows[w][e];
             a.partial[((size_t)blockIdx.x * 2 + which) * a.dim + e] = s;
         }
     }
@@ -271,13 +375,17 @@ __global__ void __launch_bounds__(kThreads) rope_grad_kernel(const RopeArgs a) {
 __global__ void __launch_bounds__(1024) rope_weight_grad_kernel(const float *partial, int blocks, int dim, float *dq, float *dk) {
     __shared__ float sums[32][33];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, col = blockIdx.x * 32 + lane;
+    grid_dependency_wait();
     float s = 0.0f;
-    if (col < 2 * dim)
+    if (col < 2 * dim) {
+#pragma unroll 8
         for (int i = warp; i < blocks; i += 32) s += partial[(size_t)i * 2 * dim + col];
+    }
     sums[warp][lane] = s;
     __syncthreads();
     if (warp == 0 && col < 2 * dim) {
         s = 0.0f;
+#pragma unroll
         for (int i = 0; i < 32; ++i) s += sums[i][lane];
         (col < dim ? dq : dk)[col < dim ? col : col - dim] = s;
     }
@@ -302,16 +410,21 @@ std::vector<uint64_t> turn_fractions(const Spec &s) {
     return out;
 }
 
-template <typename T, int kLanes>
+template <typename T, int kLanes, Pairing kPair>
 LaunchFn rope_launch(Context *ctx, const Spec &s) {
     RopeArgs base{};
     base.batch = s.batch, base.seq = s.seq, base.heads = s.heads, base.kv_heads = s.kv_heads, base.dim = s.dim, base.rotary = s.rotary;
-    base.interleaved = s.interleaved, base.norm = s.norm, base.rows = s.capacity ? s.capacity : s.seq;
+    base.norm = s.norm, base.rows = s.capacity ? s.capacity : s.seq;
     base.epsilon = s.epsilon;
     base.gain = s.scaling == "yarn" ? (float)(0.1 * std::log((double)s.factor) + 1.0) : 1.0f;
     base.err = ctx->err_dev;
     const bool grad = s.op == Op::QkNormRopeGrad, norm = s.norm, cached = s.capacity != 0;
-    const int blocks = std::min<int>(s.batch * s.seq, ctx->sm_count * (grad ? 4 : 8)), dim = s.dim;
+    // Resident warps get one token each where there are as many; fewer tokens share
+    // theirs among warps, down to one round of rows a warp.
+    const long long tokens = (long long)s.batch * s.seq, resident = (long long)ctx->sm_count * kWarps * (grad ? 2 : 4);
+    const int per = 32 / kLanes, rounds = (int)((s.heads + per - 1) / per + 2 * ((s.kv_heads + per - 1) / per));
+    base.parts = (int)std::max(1ll, std::min<long long>(rounds, resident / tokens));
+    const int blocks = (int)std::min((tokens * base.parts + kWarps - 1) / kWarps, grad ? resident / kWarps : 1ll << 30), dim = s.dim;
     // the frequencies, and behind them the gradient's partial sums
     const std::vector<uint64_t> turns = turn_fractions(s);
     const size_t table = (turns.size() * 8 + 255) / 256 * 256;
@@ -329,21 +442,27 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
         if (cached) a.starts = static_cast<const int *>(b[i++]);
         a.q = b[i++], a.k = b[i++], a.v = b[i++];
         if (!grad) {
-            rope_kernel<T, kLanes><<<blocks, kThreads, 0, st>>>(a);
+            rope_kernel<T, kLanes, kPair><<<blocks, kThreads, 0, st>>>(a);
             return cudaGetLastError();
         }
         a.dqkv = b[i++];
-        rope_grad_kernel<T, kLanes><<<blocks, kThreads, 0, st>>>(a);
-        if (norm)
-            rope_weight_grad_kernel<<<(2 * dim + 31) / 32, 1024, 0, st>>>(a.partial, blocks, dim, static_cast<float *>(b[i]), static_cast<float *>(b[i + 1]));
-        return cudaGetLastError();
+        rope_grad_kernel<T, kLanes, kPair><<<blocks, kThreads, 0, st>>>(a);
+        if (!norm) return cudaGetLastError();
+        const cudaError_t e = launch_after(st, rope_weight_grad_kernel, (2 * dim + 31) / 32, 1024, 0, static_cast<const float *>(a.partial), blocks,
+                                           dim, static_cast<float *>(b[i]), static_cast<float *>(b[i + 1]));
+        return e == cudaSuccess ? cudaGetLastError() : e;
     };
 }
 
+template <typename T, Pairing kPair>
+LaunchFn rope_lanes(Context *ctx, const Spec &s) {
+    if (s.dim <= 64) return rope_launch<T, 8, kPair>(ctx, s);
+    return s.dim <= 128 ? rope_launch<T, 16, kPair>(ctx, s) : rope_launch<T, 32, kPair>(ctx, s);
+}
 template <typename T>
 LaunchFn rope_pick(Context *ctx, const Spec &s) {
-    if (s.dim <= 64) return rope_launch<T, 8>(ctx, s);
-    return s.dim <= 128 ? rope_launch<T, 16>(ctx, s) : rope_launch<T, 32>(ctx, s);
+    if (s.interleaved) return rope_lanes<T, kNeighbours>(ctx, s);
+    return s.rotary % 8 == 0 ? rope_lanes<T, kHalves>(ctx, s) : rope_lanes<T, kGeneral>(ctx, s);
 }
 
 }  // namespace
