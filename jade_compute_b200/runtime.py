@@ -15,6 +15,7 @@ import ctypes
 import json
 import os
 import time
+from array import array
 from dataclasses import dataclass, field
 from typing import Iterable, Sequence
 
@@ -235,6 +236,7 @@ class Execution:
 
 
 class _Dispatch(ctypes.Structure):
+    """jr_dispatch, for direct calls of jr_execute2 (execute packs the same words)."""
     _fields_ = [("kernel", ctypes.c_void_p), ("buffers", ctypes.POINTER(ctypes.c_void_p)), ("buffer_count", ctypes.c_size_t)]
 
 
@@ -254,6 +256,7 @@ class Runtime:
         _check(L.jr_info(self.ctx, out, len(out), e, len(e)), e)
         self.device_info = out.value.decode()
         self._kernels: list[Kernel] = []
+        self._message = _err()  # of execute (a context is used serially)
 
     # -- lifetime
     def close(self) -> None:
@@ -356,26 +359,26 @@ class Runtime:
         jobs = list(jobs)
         if not jobs or repeats <= 0:
             raise JadeError(JR_EINVAL, "execution requires jobs and positive repeats")
-        arrays = []
-        disp = (_Dispatch * len(jobs))()
-        for i, (kernel, bufs) in enumerate(jobs):
+        # jr_dispatch records as machine words (kernel, buffer array, count): ctypes
+        # structures and pointer arrays cost several times as much host time per call
+        words, arrays = array("Q"), []
+        for kernel, bufs in jobs:
             if kernel.runtime is not self:
                 raise JadeError(JR_EINVAL, "kernel belongs to another runtime/device context")
             for b in bufs:
-                self._own(b)
-            arr = (ctypes.c_void_p * len(bufs))(*[b.ptr for b in bufs])
-            arrays.append(arr)
-            disp[i].kernel = kernel.handle
-            disp[i].buffers = ctypes.cast(arr, ctypes.POINTER(ctypes.c_void_p))
-            disp[i].buffer_count = len(bufs)
-        e = _err()
+                if b.freed or b.runtime is not self:
+                    self._own(b)  # raises
+            arrays.append(array("Q", [b.ptr for b in bufs]))
+            words.extend((kernel.handle, arrays[-1].buffer_info()[0], len(bufs)))
+        e = self._message
         gpu = ctypes.c_double(0)
         jm = (ctypes.c_double * len(jobs))() if per_job else None
-        t0 = time.perf_counter()
         flags = (JR_EXEC_GRAPH if graph else 0) | (JR_EXEC_STREAMS if streams else 0)
-        rc = lib().jr_execute2(self.ctx, disp, len(jobs), repeats, flags, ctypes.byref(gpu), jm, e, len(e))
+        t0 = time.perf_counter()
+        rc = lib().jr_execute2(self.ctx, words.buffer_info()[0], len(jobs), repeats, flags, ctypes.byref(gpu), jm, e, len(e))
         host_ms = (time.perf_counter() - t0) * 1e3
-        _check(rc, e)
+        if rc != JR_OK:
+            _check(rc, e)
         return Execution(host_ms, gpu.value if gpu.value > 0 else None, len(jobs) * repeats, repeats,
                          list(jm) if per_job else None)
 
