@@ -21,21 +21,26 @@
 // the position, modulo 2^64): exact reduction at every position, where an FP32
 // product is off by 0.004 rad at position 100,000.
 //
-// Both kernels are bound by HBM (each row read and written once). A warp takes
-// heads of one token, 32 / kLanes rows at a time, 8 elements a lane, and forms the
-// token's sines and cosines once in registers for all of them; no block barrier, no
-// shared memory in the loop. Rows of several rounds are loaded before the first is
-// worked on, so that enough bytes are in flight.
+// Both kernels are bound by HBM (each row read and written once), with the issue rate
+// close behind: 16 elements a lane, 32 / kLanes rows a warp (a round), packed FP32x2
+// arithmetic. A warp takes heads of one token, whose sines and cosines it forms once,
+// a few a lane, in shared memory; the rows of the next rounds load meanwhile. Angles
+// and norm weights are read from shared memory for every round: registers hold rows
+// only, so that enough warps are resident. No block barrier per token, so that warps
+// drift apart and memory stays busy.
+#include <climits>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
+#include "attention_softmax.cuh"
 #include "common.cuh"
 #include "internal.hpp"
 
 namespace jade {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kThreads = 128, kWarps = kThreads / 32;
 
 struct RopeArgs {
     const void *qkv, *q_weight, *k_weight;
@@ -46,140 +51,210 @@ struct RopeArgs {
     float *partial;         // gradient: [block][2][dim] sums of the norm weights' gradients
     int batch, seq, heads, kv_heads, dim, rotary, norm, rows;  // rows: of k and v per head
     int parts;              // warps that share a token's heads
-    float epsilon, gain;
+    float epsilon, gain, inv_dim;
     int *err;
 };
 
-// How a lane's 8 elements lie in the head and find their partners.
-//   kHalves      rotated lanes hold 4 of the first half and their 4 partners of the
-//                second, two pieces rotary / 2 apart (rotary a multiple of 8); the
-//                others 8 in a row
-//   kNeighbours  8 in a row, partners beside each other
-//   kGeneral     8 in a row, partners through the warp's rows in shared memory
+// How a lane's 16 elements, two pieces of 8, lie in the head and find their partners.
+//   kHalves      rotated lanes hold 8 of the first half and their 8 partners of the
+//                second, rotary / 2 apart (rotary a multiple of 16); the others 16 in
+//                a row
+//   kNeighbours  16 in a row, partners beside each other
+//   kGeneral     16 in a row, partners through the warp's rows in shared memory
 //                (halves of any length)
 enum Pairing { kHalves, kNeighbours, kGeneral };
 
-template <typename T>
-struct Vec4;  // 4 elements as loaded
-template <>
-struct Vec4<float> { using type = float4; };
-template <>
-struct Vec4<__nv_bfloat16> { using type = uint2; };
-template <>
-struct Vec4<__half> { using type = uint2; };
-
-__device__ __forceinline__ void widen(const float4 &u, float *x, float) { x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w; }
-__device__ __forceinline__ void widen(const uint2 &u, float *x, __nv_bfloat16) {
-    x[0] = __uint_as_float(u.x << 16), x[1] = __uint_as_float(u.x & 0xffff0000u);
-    x[2] = __uint_as_float(u.y << 16), x[3] = __uint_as_float(u.y & 0xffff0000u);
-}
-__device__ __forceinline__ void widen(const uint2 &u, float *x, __half) {
-    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-    x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-}
-__device__ __forceinline__ float4 narrow(const float *x, float) { return make_float4(x[0], x[1], x[2], x[3]); }
-__device__ __forceinline__ uint2 narrow(const float *x, __nv_bfloat16) { return make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])); }
-__device__ __forceinline__ uint2 narrow(const float *x, __half) { return make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3])); }
-
-// A lane's elements of a row: 4 from offset a, 4 from offset b.
-template <typename T>
-struct Row8 {
-    typename Vec4<T>::type lo, hi;
-};
 struct Place {
-    int a, b;
-    bool live;
+    int lo, hi;            // offsets of the pieces in the head
+    bool has_lo, has_hi;   // the head has them
 };
-template <typename T, Pairing kPair>
-__device__ __forceinline__ Row8<T> load_row(const T *p, Place at) {
-    using V = typename Vec4<T>::type;
-    Row8<T> r{};
-    if (!at.live) return r;
-    if constexpr (kPair != kHalves && sizeof(T) == 2) {
-        const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p + at.a));
-        r.lo = make_uint2(u.x, u.y), r.hi = make_uint2(u.z, u.w);
-    } else {
-        r.lo = __ldcs(reinterpret_cast<const V *>(p + at.a)), r.hi = __ldcs(reinterpret_cast<const V *>(p + at.b));
-    }
-    return r;
-}
-template <typename T, Pairing kPair>
-__device__ __forceinline__ void store_row(T *p, Place at, const Row8<T> &r) {
-    using V = typename Vec4<T>::type;
-    if (!at.live) return;
-    if constexpr (kPair != kHalves && sizeof(T) == 2) {
-        *reinterpret_cast<uint4 *>(p + at.a) = make_uint4(r.lo.x, r.lo.y, r.hi.x, r.hi.y);
-    } else {
-        *reinterpret_cast<V *>(p + at.a) = r.lo;
-        *reinterpret_cast<V *>(p + at.b) = r.hi;
-    }
-}
-template <typename T>
-__device__ __forceinline__ void widen8(const Row8<T> &r, float (&x)[8]) {
-    widen(r.lo, x, T{});
-    widen(r.hi, x + 4, T{});
-}
-template <typename T>
-__device__ __forceinline__ Row8<T> narrow8(const float (&x)[8]) {
-    return Row8<T>{narrow(x, T{}), narrow(x + 4, T{})};
-}
-
 template <Pairing kPair>
 __device__ __forceinline__ Place lane_place(int chunk, int dim, int rotary) {
-    Place at{8 * chunk, 8 * chunk + 4, 8 * chunk < dim};
-    if (kPair == kHalves && 8 * chunk < rotary) at.a = 4 * chunk, at.b = 4 * chunk + rotary / 2;
+    Place at{16 * chunk, 16 * chunk + 8, 16 * chunk < dim, 16 * chunk + 8 < dim};
+    if (kPair == kHalves && 16 * chunk < rotary) at.lo = 8 * chunk, at.hi = 8 * chunk + rotary / 2, at.has_hi = true;
     return at;
 }
 
-// Cosines and sines of the lane's pairs at a position; passed elements turn by 0.
-// kGeneral: for each of its 8 elements, y = x c + partner s.
-template <Pairing kPair>
-struct Angles {
-    static constexpr int kCount = kPair == kGeneral ? 8 : 4;
-    float c[kCount], s[kCount];
-    __device__ __forceinline__ void set(const RopeArgs &a, int chunk, int position, float sign) {
-        const int half = a.rotary / 2;
+// Pieces as they are loaded and stored, and as four pairs of FP32 each.
+template <typename T>
+struct Piece { uint4 u; };
+template <>
+struct Piece<float> { float4 a, b; };
+
+__device__ __forceinline__ void load_piece(Piece<float> &x, const float *p, bool on) {
+    x.a = x.b = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (on) x.a = __ldcs(reinterpret_cast<const float4 *>(p)), x.b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+}
+template <typename T>
+__device__ __forceinline__ void load_piece(Piece<T> &x, const T *p, bool on) {
+    x.u = make_uint4(0, 0, 0, 0);
+    if (on) x.u = __ldcs(reinterpret_cast<const uint4 *>(p));
+}
+__device__ __forceinline__ void store_piece(float *p, const Piece<float> &x) {
+    reinterpret_cast<float4 *>(p)[0] = x.a;
+    reinterpret_cast<float4 *>(p)[1] = x.b;
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(T *p, const Piece<T> &x) { *reinterpret_cast<uint4 *>(p) = x.u; }
+
+__device__ __forceinline__ void widen(const Piece<float> &x, uint64_t *v) {
+    v[0] = pack2f(x.a.x, x.a.y), v[1] = pack2f(x.a.z, x.a.w), v[2] = pack2f(x.b.x, x.b.y), v[3] = pack2f(x.b.z, x.b.w);
+}
+__device__ __forceinline__ void widen(const Piece<__nv_bfloat16> &x, uint64_t *v) {
+    const uint32_t w[4] = {x.u.x, x.u.y, x.u.z, x.u.w};
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) {
-            const int e = kCount * chunk + i;  // pair, or element
-            const int pair = kPair == kGeneral && e >= half ? e - half : e;
-            c[i] = 1.0f, s[i] = 0.0f;
-            if (pair < half) {
-                const uint64_t turn = (uint64_t)(int64_t)position * __ldg(a.turns + pair);
-                sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s[i], &c[i]);
-                c[i] *= a.gain, s[i] *= kPair == kGeneral && e < half ? -sign * a.gain : sign * a.gain;
+    for (int i = 0; i < 4; ++i) v[i] = pack2f(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void widen(const Piece<__half> &x, uint64_t *v) {
+    const uint32_t w[4] = {x.u.x, x.u.y, x.u.z, x.u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        v[i] = pack2f(f.x, f.y);
+    }
+}
+__device__ __forceinline__ void narrow(Piece<float> &x, const uint64_t *v) {
+    unpack2f(v[0], x.a.x, x.a.y), unpack2f(v[1], x.a.z, x.a.w), unpack2f(v[2], x.b.x, x.b.y), unpack2f(v[3], x.b.z, x.b.w);
+}
+template <typename T>
+__device__ __forceinline__ void narrow(Piece<T> &x, const uint64_t *v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float a, b;
+        unpack2f(v[i], a, b);
+        w[i] = std::is_same<T, __nv_bfloat16>::value ? pack_bf16(a, b) : pack_f16(a, b);
+    }
+    x.u = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+struct Row {  // a lane's share of a head
+    Piece<T> lo, hi;
+    __device__ __forceinline__ void load(const T *p, const Place &at, bool on) {
+        load_piece(lo, p + at.lo, on && at.has_lo);
+        load_piece(hi, p + at.hi, on && at.has_hi);
+    }
+    __device__ __forceinline__ void store(T *p, const Place &at, bool on) const {
+        if (on && at.has_lo) store_piece(p + at.lo, lo);
+        if (on && at.has_hi) store_piece(p + at.hi, hi);
+    }
+};
+
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t both(float x) { return pack2f(x, x); }
+
+// FP32 tables in shared memory, read 8 in a row by a lane (two 16-byte loads) without
+// bank conflicts: entry e lies at table_at(e).
+constexpr int kTable = 256;
+__device__ __forceinline__ int table_at(int e) { return (e >> 2 & 1) * (kTable / 2) + (e >> 3) * 4 + (e & 3); }
+__device__ __forceinline__ void table8(const float *table, int first, uint64_t *v) {
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(table + first / 2), b = *reinterpret_cast<const ulonglong2 *>(table + kTable / 2 + first / 2);
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
+}
+
+struct Elements {
+    uint64_t v[8];
+    template <typename T>
+    __device__ __forceinline__ void from(const Row<T> &r) { widen(r.lo, v), widen(r.hi, v + 4); }
+    template <typename T>
+    __device__ __forceinline__ void to(Row<T> &r) const { narrow(r.lo, v), narrow(r.hi, v + 4); }
+    // sum of the products with another row's elements
+    __device__ __forceinline__ float dot(const Elements &o) const {
+        uint64_t s[2] = {mul2(v[0], o.v[0]), mul2(v[1], o.v[1])};
+#pragma unroll
+        for (int i = 2; i < 8; ++i) s[i & 1] = fma2(v[i], o.v[i], s[i & 1]);
+        float x, y;
+        unpack2f(add2(s[0], s[1]), x, y);
+        return x + y;
+    }
+};
+
+// The token's cosines and sines, formed by the warp in its shared memory as the
+// pairing multiplies them; kBack turns back.
+//   kNeighbours  x' = x a + (x with its pairs swapped) b: a = c c .., b = -s s ..
+//   else         a = c, b = s, n = -s of each pair
+template <int kLanes, Pairing kPair, bool kBack>
+struct Turn {
+    float *a, *b, *n;
+    __device__ __forceinline__ explicit Turn(float *tables) : a(tables), b(tables + kTable), n(tables + 2 * kTable) {}
+    static constexpr int kFloats = (kPair == kNeighbours ? 2 : 3) * kTable;
+    __device__ __forceinline__ void form(const RopeArgs &args, int position, int lane) {
+        __syncwarp();  // the last token's have been read
+        for (int i = lane; i < 8 * kLanes; i += 32) {
+            float c = 1.0f, s = 0.0f;  // passed elements, and beyond the head: lanes read whole pieces
+            if (i < args.rotary / 2) {
+                const uint64_t turn = (uint64_t)(int64_t)position * __ldg(args.turns + i);
+                sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
+                c *= args.gain, s *= kBack ? -args.gain : args.gain;
+            }
+            if constexpr (kPair == kNeighbours) {
+                *reinterpret_cast<float2 *>(a + table_at(2 * i)) = make_float2(c, c);
+                *reinterpret_cast<float2 *>(b + table_at(2 * i)) = make_float2(-s, s);
+            } else {
+                a[table_at(i)] = c, b[table_at(i)] = s, n[table_at(i)] = -s;
             }
         }
+        __syncwarp();
     }
-    // x: the lane's elements; row: the warp row's elements in shared memory (kGeneral)
-    __device__ __forceinline__ void turn(float (&x)[8], float *row, int chunk, int half) const {
+    // row: the row's elements in shared memory (kGeneral)
+    __device__ __forceinline__ void apply(Elements &x, float *row, int chunk, int half) const {
         if constexpr (kPair == kHalves) {
+            uint64_t c[4], s[4], m[4];
+            table8(a, 8 * chunk, c), table8(b, 8 * chunk, s), table8(n, 8 * chunk, m);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = x[i] * c[i] - x[4 + i] * s[i];
-                x[4 + i] = x[i] * s[i] + x[4 + i] * c[i];
-                x[i] = u;
+                const uint64_t lo = x.v[i], hi = x.v[4 + i];
+                x.v[i] = fma2(lo, c[i], mul2(hi, m[i]));
+                x.v[4 + i] = fma2(hi, c[i], mul2(lo, s[i]));
             }
         } else if constexpr (kPair == kNeighbours) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float u = x[2 * i] * c[i] - x[2 * i + 1] * s[i];
-                x[2 * i + 1] = x[2 * i] * s[i] + x[2 * i + 1] * c[i];
-                x[2 * i] = u;
-            }
-        } else {
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 8; ++i) row[8 * chunk + i] = x[i];
-            __syncwarp();
+            uint64_t c[8], s[8];
+            table8(a, 16 * chunk, c), table8(a, 16 * chunk + 8, c + 4), table8(b, 16 * chunk, s), table8(b, 16 * chunk + 8, s + 4);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int e = 8 * chunk + i;
-                if (e < 2 * half) x[i] = x[i] * c[i] + row[e < half ? e + half : e - half] * s[i];
+                float p, q;
+                unpack2f(x.v[i], p, q);
+                x.v[i] = fma2(x.v[i], c[i], mul2(pack2f(q, p), s[i]));
             }
+        } else {
+            float y[16];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) unpack2f(x.v[i], y[2 * i], y[2 * i + 1]);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) row[16 * chunk + i] = y[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int e = 16 * chunk + i;
+                if (e >= 2 * half) continue;
+                const int pair = table_at(e < half ? e : e - half);
+                y[i] = y[i] * a[pair] + (e < half ? n : b)[pair] * row[e < half ? e + half : e - half];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x.v[i] = pack2f(y[2 * i], y[2 * i + 1]);
         }
     }
 };
+
+// The norm weights of queries and keys as tables (whole block; a barrier is due before their use).
+template <typename T>
+__device__ __forceinline__ void weight_tables(const RopeArgs &a, float (*w)[kTable]) {
+    if (!a.norm) return;
+    for (int e = threadIdx.x; e < kTable; e += kThreads) {  // 0 beyond the head: lanes read whole pieces
+        w[0][table_at(e)] = e < a.dim ? to_f32<T>(static_cast<const T *>(a.q_weight)[e]) : 0.0f;
+        w[1][table_at(e)] = e < a.dim ? to_f32<T>(static_cast<const T *>(a.k_weight)[e]) : 0.0f;
+    }
+}
+__device__ __forceinline__ void load_weights(Elements &w, const float *table, const Place &at) {
+    table8(table, at.lo, w.v);
+    table8(table, at.hi & (kTable - 1), w.v + 4);  // a piece that the head lacks is not stored
+}
 
 // Sum over the kLanes lanes of a row.
 template <int kLanes>
@@ -189,182 +264,190 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// The rounds of a warp: a token's heads in the order queries, keys, values, 32 /
-// kLanes heads of one kind a round, the rounds of a token dealt evenly to its `parts`
-// warps.
+// Rounds of a token: its heads in the order queries, keys, values, 32 / kLanes heads
+// of one kind a round; dealt evenly to the token's `parts` warps.
+__host__ __device__ constexpr int rounds_of(int heads, int per) { return (heads + per - 1) / per; }
 template <int kLanes>
 struct Rounds {
+    static constexpr int kPer = 32 / kLanes;
     int q, k, total;  // rounds of queries, of queries and keys, of all
     __device__ __forceinline__ Rounds(const RopeArgs &a) {
-        constexpr int per = 32 / kLanes;
-        q = (a.heads + per - 1) / per;
-        k = q + (a.kv_heads + per - 1) / per;
+        q = rounds_of(a.heads, kPer), k = q + rounds_of(a.kv_heads, kPer);
         total = k + k - q;
+    }
+    // kind (0 queries, 1 keys, 2 values) of round r and the lane's head of it; false: it has none
+    __device__ __forceinline__ bool at(const RopeArgs &a, int r, int sub, int &kind, int &h) const {
+        kind = r < q ? 0 : r < k ? 1 : 2;
+        h = (r - (kind == 0 ? 0 : kind == 1 ? q : k)) * kPer + sub;
+        return h < (kind ? a.kv_heads : a.heads);
     }
 };
 
 template <typename T, int kLanes, Pairing kPair>
 __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
-    constexpr int kPer = 32 / kLanes, kAhead = 4;  // rounds loaded at a time
-    __shared__ float shared_rows[kPair == kGeneral ? kWarps : 1][256];
-    const int lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
+    constexpr int kAhead = 2;  // rounds worked on, and as many loading
+    __shared__ __align__(16) float tables[kWarps][Turn<kLanes, kPair, false>::kFloats];
+    __shared__ __align__(16) float weights[2][kTable];
+    __shared__ float shared_rows[kPair == kGeneral ? kWarps : 1][512];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
     const Place at = lane_place<kPair>(chunk, a.dim, a.rotary);
     const Rounds<kLanes> rounds(a);
-    const int total_heads = a.heads + 2 * a.kv_heads;
-    float *row = shared_rows[kPair == kGeneral ? threadIdx.x >> 5 : 0] + sub * (kLanes * 8);
-    const long long items = (long long)a.batch * a.seq * a.parts;
-    for (long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * kWarps) {
-        const int token = (int)(item / a.parts), part = (int)(item - (long long)token * a.parts);
-        const int b = token / a.seq, t = token - b * a.seq;
-        const int r0 = (int)((long long)rounds.total * part / a.parts), r1 = (int)((long long)rounds.total * (part + 1) / a.parts);
-        const int start = a.starts ? __ldg(a.starts + b) : 0, position = __ldg(a.positions + token);
-        if (start < 0 || start > a.rows - a.seq) {
-            if (lane == 0) atomicCAS(a.err, 0, kErrCacheLength);
-            continue;
+    float *row = shared_rows[kPair == kGeneral ? warp : 0] + sub * (kLanes * 16);
+    Turn<kLanes, kPair, false> turn(tables[warp]);
+    weight_tables<T>(a, weights);
+    __syncthreads();
+    const int item = blockIdx.x * kWarps + warp;
+    if (item >= a.batch * a.seq * a.parts) return;
+    const int token = item / a.parts, part = item - token * a.parts, b = token / a.seq, t = token - b * a.seq;
+    const int r0 = rounds.total * part / a.parts, r1 = rounds.total * (part + 1) / a.parts;
+    const int position = __ldg(a.positions + token), start = a.starts ? __ldg(a.starts + b) : 0;
+    const T *in = static_cast<const T *>(a.qkv) + (size_t)token * (a.heads + 2 * a.kv_heads) * a.dim;
+    // first row of the token's queries, and its slot of the first head's keys and values
+    T *q = static_cast<T *>(a.q) + ((size_t)b * a.heads * a.seq + t) * a.dim;
+    const size_t slot = ((size_t)b * a.kv_heads * a.rows + start + t) * a.dim;
+    const int q_step = a.seq * a.dim;
+    const long long kv_step = (long long)a.rows * a.dim;
+    Row<T> next[kAhead];
+    auto load = [&](int r) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            int kind, h;
+            const bool on = rounds.at(a, r + u, sub, kind, h) && r + u < r1;
+            next[u].load(in + ((kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads) + h) * a.dim, at, on);
         }
-        const T *in = static_cast<const T *>(a.qkv) + (size_t)token * total_heads * a.dim;
-        // head of the packed row and its destination in round r; -1 where the round has no head for this lane
-        auto head_of = [&](int r, T *&out) {
-            int h;
-            if (r < rounds.q) {
-                h = r * kPer + sub;
-                out = static_cast<T *>(a.q) + (((size_t)b * a.heads + h) * a.seq + t) * a.dim;
-                return h < a.heads ? h : -1;
-            }
-            const bool key = r < rounds.k;
-            h = (r - (key ? rounds.q : rounds.k)) * kPer + sub;
-            out = static_cast<T *>(key ? a.k : a.v) + (((size_t)b * a.kv_heads + h) * a.rows + start + t) * a.dim;
-            return h < a.kv_heads ? a.heads + (key ? 0 : a.kv_heads) + h : -1;
-        };
-        Angles<kPair> angles;
-        float w[8];
-        int weights = -1;  // whose weights w holds: 0 queries, 1 keys
-        for (int r = r0; r < r1; r += kAhead) {
-            Row8<T> x[kAhead];
-            T *out[kAhead];
-            bool on[kAhead];
+    };
+    load(r0);
+    if (start < 0 || start > a.rows - a.seq) {
+        if (lane == 0) atomicCAS(a.err, 0, kErrCacheLength);
+        return;
+    }
+    if (r0 < rounds.k) turn.form(a, position, lane);
+    for (int r = r0; r < r1; r += kAhead) {
+        Row<T> x[kAhead];
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int h = head_of(min(r + u, r1 - 1), out[u]);
-                on[u] = h >= 0 && r + u < r1;
-                x[u] = load_row<T, kPair>(in + (size_t)max(h, 0) * a.dim, Place{at.a, at.b, at.live && on[u]});
-            }
-            if (r == r0 && r < rounds.k) angles.set(a, chunk, position, 1.0f);
+        for (int u = 0; u < kAhead; ++u) x[u] = next[u];
+        if (r + kAhead < r1) load(r + kAhead);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (r + u >= r1) break;
-                if (r + u < rounds.k) {  // a query or a key
-                    const int kind = r + u < rounds.q ? 0 : 1;
-                    if (a.norm && kind != weights) {
-                        weights = kind;
-                        widen8(load_row<T, kPair>(static_cast<const T *>(kind ? a.k_weight : a.q_weight), at), w);
-                    }
-                    float y[8];
-                    widen8(x[u], y);
-                    if (a.norm) {
-                        float ss = 0.0f;
+        for (int u = 0; u < kAhead; ++u) {
+            if (r + u >= r1) break;
+            int kind, h;
+            const bool on = rounds.at(a, r + u, sub, kind, h);
+            if (kind < 2) {
+                Elements y;
+                y.from(x[u]);
+                if (a.norm) {
+                    Elements w;
+                    load_weights(w, weights[kind], at);
+                    const uint64_t scale = both(rsqrtf(fmaf(row_sum<kLanes>(y.dot(y)), a.inv_dim, a.epsilon)));
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
-                        const float scale = rsqrtf(row_sum<kLanes>(ss) / (float)a.dim + a.epsilon);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] *= scale * w[i];
-                    }
-                    angles.turn(y, row, chunk, a.rotary / 2);
-                    x[u] = narrow8<T>(y);
+                    for (int i = 0; i < 8; ++i) y.v[i] = mul2(mul2(y.v[i], scale), w.v[i]);
                 }
-                store_row<T, kPair>(out[u], Place{at.a, at.b, at.live && on[u]}, x[u]);
+                turn.apply(y, row, chunk, a.rotary / 2);
+                y.to(x[u]);
             }
+            x[u].store(kind == 0 ? q + h * q_step : static_cast<T *>(kind == 1 ? a.k : a.v) + slot + h * kv_step, at, on);
         }
     }
 }
 
+// A persistent warp walks over items (a token, a part of its heads) and keeps its sums
+// of the weights' gradients.
 template <typename T, int kLanes, Pairing kPair>
-__global__ void __launch_bounds__(kThreads, 2) rope_grad_kernel(const RopeArgs a) {
-    constexpr int kPer = 32 / kLanes, kAhead = 4;
-    __shared__ float shared_rows[kWarps][256];
-    const int lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
+__global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a) {
+    constexpr int kAhead = 2;
+    __shared__ __align__(16) float tables[kWarps][Turn<kLanes, kPair, true>::kFloats];
+    __shared__ __align__(16) float weights[2][kTable];
+    __shared__ float shared_rows[kWarps][kPair == kGeneral ? 512 : kTable];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
     const Place at = lane_place<kPair>(chunk, a.dim, a.rotary);
     const Rounds<kLanes> rounds(a);
-    const int total_heads = a.heads + 2 * a.kv_heads;
-    float *row = shared_rows[threadIdx.x >> 5] + sub * (kLanes * 8);
-    float wq[8], wk[8], dwq[8] = {}, dwk[8] = {};
+    float *row = shared_rows[warp] + (kPair == kGeneral ? sub * (kLanes * 16) : 0);
+    const int q_step = a.seq * a.dim;
+    Turn<kLanes, kPair, true> turn(tables[warp]);
+    weight_tables<T>(a, weights);
+    __syncthreads();
+    Elements dwq, dwk;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) wq[i] = wk[i] = 1.0f;
-    if (a.norm) {
-        widen8(load_row<T, kPair>(static_cast<const T *>(a.q_weight), at), wq);
-        widen8(load_row<T, kPair>(static_cast<const T *>(a.k_weight), at), wk);
-    }
-    const long long items = (long long)a.batch * a.seq * a.parts;
-    for (long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * kWarps) {
-        const int token = (int)(item / a.parts), part = (int)(item - (long long)token * a.parts);
-        const int b = token / a.seq, t = token - b * a.seq;
-        const int r0 = (int)((long long)rounds.total * part / a.parts), r1 = (int)((long long)rounds.total * (part + 1) / a.parts);
+    for (int i = 0; i < 8; ++i) dwq.v[i] = dwk.v[i] = 0;
+    const int items = a.batch * a.seq * a.parts;
+    for (int item = blockIdx.x * kWarps + warp; item < items; item += gridDim.x * kWarps) {
+        const int token = item / a.parts, part = item - token * a.parts, b = token / a.seq, t = token - b * a.seq;
+        const int r0 = rounds.total * part / a.parts, r1 = rounds.total * (part + 1) / a.parts;
         const int position = __ldg(a.positions + token);
-        const size_t packed = (size_t)token * total_heads * a.dim;
-        Angles<kPair> angles;
+        const size_t packed = (size_t)token * (a.heads + 2 * a.kv_heads) * a.dim;
+        const T *in = static_cast<const T *>(a.qkv) + packed;
+        T *out = static_cast<T *>(a.dqkv) + packed;
+        const T *q = static_cast<const T *>(a.q) + ((size_t)b * a.heads * a.seq + t) * a.dim;
+        const size_t slot = ((size_t)b * a.kv_heads * a.seq + t) * a.dim;
         for (int r = r0; r < r1; r += kAhead) {
-            Row8<T> g[kAhead], x[kAhead];
-            size_t to[kAhead];
+            Row<T> g[kAhead], x[kAhead];
+            int to[kAhead];
             bool on[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int rr = min(r + u, r1 - 1), kind = rr < rounds.q ? 0 : rr < rounds.k ? 1 : 2;
-                const int h = (rr - (kind == 0 ? 0 : kind == 1 ? rounds.q : rounds.k)) * kPer + sub, heads = kind ? a.kv_heads : a.heads;
-                on[u] = h < heads && r + u < r1;
-                const Place here{at.a, at.b, at.live && on[u]};
-                const T *from = static_cast<const T *>(kind == 0 ? a.q : kind == 1 ? a.k : a.v);
-                to[u] = packed + (size_t)(h + (kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads)) * a.dim;
-                g[u] = load_row<T, kPair>(from + (((size_t)b * heads + h) * a.seq + t) * a.dim, here);
-                if (a.norm && kind < 2) x[u] = load_row<T, kPair>(static_cast<const T *>(a.qkv) + to[u], here);
+                int kind, h;
+                on[u] = rounds.at(a, r + u, sub, kind, h) && r + u < r1;
+                to[u] = ((kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads) + h) * a.dim;
+                g[u].load((kind == 0 ? q : static_cast<const T *>(kind == 1 ? a.k : a.v) + slot) + h * q_step, at, on[u]);
+                x[u].load(in + to[u], at, on[u] && a.norm && kind < 2);
             }
-            if (r == r0 && r < rounds.k) angles.set(a, chunk, position, -1.0f);
+            if (r == r0 && r < rounds.k) turn.form(a, position, lane);
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
                 if (r + u >= r1) break;
                 if (r + u < rounds.k) {
-                    const bool query = r + u < rounds.q;
-                    float d[8];
-                    widen8(g[u], d);
-                    angles.turn(d, row, chunk, a.rotary / 2);
+                    Elements d;
+                    d.from(g[u]);
+                    turn.apply(d, row, chunk, a.rotary / 2);
                     if (a.norm) {
-                        float y[8], ss = 0.0f, ux = 0.0f;
-                        widen8(x[u], y);
+                        const int kind = r + u < rounds.q ? 0 : 1;
+                        Elements y;
+                        y.from(x[u]);
+                        const float scale = rsqrtf(fmaf(row_sum<kLanes>(y.dot(y)), a.inv_dim, a.epsilon));
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
-                        const float scale = rsqrtf(row_sum<kLanes>(ss) / (float)a.dim + a.epsilon);
-                        if (query) {  // lanes without a row hold zeros
+                        for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], both(scale));
+                        // lanes without a row hold zeros
+                        if (kind == 0) {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) y[i] *= scale, dwq[i] = fmaf(d[i], y[i], dwq[i]), d[i] *= wq[i], ux = fmaf(d[i], y[i], ux);
+                            for (int i = 0; i < 8; ++i) dwq.v[i] = fma2(d.v[i], y.v[i], dwq.v[i]);
                         } else {
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) y[i] *= scale, dwk[i] = fmaf(d[i], y[i], dwk[i]), d[i] *= wk[i], ux = fmaf(d[i], y[i], ux);
+                            for (int i = 0; i < 8; ++i) dwk.v[i] = fma2(d.v[i], y.v[i], dwk.v[i]);
                         }
-                        const float mean = row_sum<kLanes>(ux) / (float)a.dim;
+                        Elements w;
+                        load_weights(w, weights[kind], at);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) d[i] = scale * (d[i] - y[i] * mean);
+                        for (int i = 0; i < 8; ++i) d.v[i] = mul2(d.v[i], w.v[i]);
+                        const float mean = -row_sum<kLanes>(d.dot(y)) * a.inv_dim;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) d.v[i] = mul2(both(scale), fma2(y.v[i], both(mean), d.v[i]));
                     }
-                    g[u] = narrow8<T>(d);
+                    d.to(g[u]);
                 }
-                store_row<T, kPair>(static_cast<T *>(a.dqkv) + to[u], Place{at.a, at.b, at.live && on[u]}, g[u]);
+                g[u].store(out + to[u], at, on[u]);
             }
         }
     }
+    grid_dependency_trigger();
     if (!a.norm) return;
     // the block's sums: rows of the warp first, then the warps, each in a fixed order
     for (int which = 0; which < 2; ++which) {
-        float(&dw)[8] = which ? dwk : dwq;
+        const Elements &sums = which ? dwk : dwq;
+        float dw[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) unpack2f(sums.v[i], dw[2 * i], dw[2 * i + 1]);
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
 #pragma unroll
             for (int o = kLanes; o < 32; o <<= 1) dw[i] += __shfl_xor_sync(0xffffffffu, dw[i], o);
-            if (sub == 0 && at.live) shared_rows[threadIdx.x >> 5][(i < 4 ? at.a : at.b) + (i & 3)] = dw[i];
+            if (sub == 0 && (i < 8 ? at.has_lo : at.has_hi)) shared_rows[warp][(i < 8 ? at.lo : at.hi) + (i & 7)] = dw[i];
         }
         __syncthreads();
         for (int e = threadIdx.x; e < a.dim; e += kThreads) {
             float s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) s += shared_rows[w][e];
+            for (int i = 0; i < kWarps; ++i) s += shared_rows[i][e];
             a.partial[((size_t)blockIdx.x * 2 + which) * a.dim + e] = s;
         }
     }
@@ -390,6 +473,8 @@ __global__ void __launch_bounds__(1024) rope_weight_grad_kernel(const float *par
         (col < dim ? dq : dk)[col < dim ? col : col - dim] = s;
     }
 }
+
+constexpr int kPartWaves = 2;
 
 // theta_i / 2 pi as 0.64 fixed-point fractions of a turn.
 std::vector<uint64_t> turn_fractions(const Spec &s) {
@@ -419,12 +504,18 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
     base.gain = s.scaling == "yarn" ? (float)(0.1 * std::log((double)s.factor) + 1.0) : 1.0f;
     base.err = ctx->err_dev;
     const bool grad = s.op == Op::QkNormRopeGrad, norm = s.norm, cached = s.capacity != 0;
-    // Resident warps get one token each where there are as many; fewer tokens share
-    // theirs among warps, down to one round of rows a warp.
-    const long long tokens = (long long)s.batch * s.seq, resident = (long long)ctx->sm_count * kWarps * (grad ? 2 : 4);
-    const int per = 32 / kLanes, rounds = (int)((s.heads + per - 1) / per + 2 * ((s.kv_heads + per - 1) / per));
-    base.parts = (int)std::max(1ll, std::min<long long>(rounds, resident / tokens));
-    const int blocks = (int)std::min((tokens * base.parts + kWarps - 1) / kWarps, grad ? resident / kWarps : 1ll << 30), dim = s.dim;
+    base.inv_dim = 1.0f / (float)s.dim;
+    // A warp's rounds: enough to spread the cost of its angles (about one round's) where
+    // there are tokens for many waves, down to one round a warp for few tokens.
+    const int per = 32 / kLanes, rounds = rounds_of((int)s.heads, per) + 2 * rounds_of((int)s.kv_heads, per), dim = s.dim;
+    int per_sm = 0;
+    const void *kernel = grad ? reinterpret_cast<const void *>(rope_grad_kernel<T, kLanes, kPair>) : reinterpret_cast<const void *>(rope_kernel<T, kLanes, kPair>);
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0) != cudaSuccess || per_sm < 1)
+        throw IrError("the rotation kernel does not fit on an SM");
+    const long long tokens = (long long)s.batch * s.seq, resident = (long long)per_sm * ctx->sm_count * kWarps;
+    base.parts = (int)std::max(1ll, std::min<long long>(rounds, kPartWaves * resident / tokens));
+    if (tokens * base.parts > INT_MAX / 2) throw IrError("too many tokens for one launch");
+    const int blocks = (int)std::min((tokens * base.parts + kWarps - 1) / kWarps, grad ? resident / kWarps : 1ll << 31);
     // the frequencies, and behind them the gradient's partial sums
     const std::vector<uint64_t> turns = turn_fractions(s);
     const size_t table = (turns.size() * 8 + 255) / 256 * 256;
@@ -456,13 +547,13 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
 
 template <typename T, Pairing kPair>
 LaunchFn rope_lanes(Context *ctx, const Spec &s) {
-    if (s.dim <= 64) return rope_launch<T, 8, kPair>(ctx, s);
-    return s.dim <= 128 ? rope_launch<T, 16, kPair>(ctx, s) : rope_launch<T, 32, kPair>(ctx, s);
+    if (s.dim <= 64) return rope_launch<T, 4, kPair>(ctx, s);
+    return s.dim <= 128 ? rope_launch<T, 8, kPair>(ctx, s) : rope_launch<T, 16, kPair>(ctx, s);
 }
 template <typename T>
 LaunchFn rope_pick(Context *ctx, const Spec &s) {
     if (s.interleaved) return rope_lanes<T, kNeighbours>(ctx, s);
-    return s.rotary % 8 == 0 ? rope_lanes<T, kHalves>(ctx, s) : rope_lanes<T, kGeneral>(ctx, s);
+    return s.rotary % 16 == 0 ? rope_lanes<T, kHalves>(ctx, s) : rope_lanes<T, kGeneral>(ctx, s);
 }
 
 }  // namespace
