@@ -39,86 +39,117 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 1024, kSelectEach = 8, kSelectTile = kSelectThreads * kSelectEach, kBins = 2048;
 
-// Exclusive prefix sum of one flag per thread over the block, in thread order, and the total.
-__device__ __forceinline__ int block_rank(bool flag, int *warp_sums, int &total) {
+// Exclusive prefix sum of v over the block, in thread order, and its total.
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *warp_sums, uint32_t &total) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t ballot = __ballot_sync(0xffffffffu, flag);
-    __syncthreads();
-    if (lane == 0) warp_sums[warp] = __popc(ballot);
-    __syncthreads();
-    int v = warp_sums[lane], sum = v;
+    uint32_t sum = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int n = __shfl_up_sync(0xffffffffu, sum, o);
+        const uint32_t n = __shfl_up_sync(0xffffffffu, sum, o);
         if (lane >= o) sum += n;
     }
-    total = __shfl_sync(0xffffffffu, sum, 31);
-    const int before = __shfl_sync(0xffffffffu, sum - v, warp);
-    return before + __popc(ballot & ((1u << lane) - 1));
+    __syncthreads();  // warp_sums may still be read
+    if (lane == 31) warp_sums[warp] = sum;
+    __syncthreads();
+    uint32_t w = warp_sums[lane], upto = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t n = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += n;
+    }
+    total = __shfl_sync(0xffffffffu, upto, 31);
+    return __shfl_sync(0xffffffffu, upto - w, warp) + sum - v;
 }
 
-// One block per (sequence, head): the need-th largest key among the entries that
-// may go, digit by digit (8 bits, from the top), then the kept slots in order.
+// One block per (sequence, head). The need-th largest key among the entries that may
+// go is found digit by digit from the top (11, 11, 10 bits: with 8-bit digits the
+// first holds little but the exponent, and its few bins serialise the counting), then
+// the kept slots are written in order: 8 neighbouring entries a thread, one prefix sum
+// over the block for entries above the threshold and entries equal to it together.
+// Weights come from memory once where a sequence has at most kSelectTile entries
+// (their keys stay in shared memory), else once per pass.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
-    __shared__ int hist[256], warp_sums[32], chosen[2];
-    const int bh = blockIdx.x, b = bh / a.kv_heads;
-    const int n = a.lengths[b];
-    int *kept = a.kept + (size_t)bh * a.keep;
-    float *w_out = a.weights_out + (size_t)bh * a.capacity;
+    __shared__ uint32_t keys[kSelectTile + kSelectTile / 32], hist[kBins], warp_sums[32], chosen[2];
+    const int bh = blockIdx.x, b = bh / a.kv_heads, n = a.lengths[b], thread = threadIdx.x;
+    grid_dependency_trigger();
     if (n < 0 || n > a.capacity) {
-        if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrCacheLength);
+        if (thread == 0) atomicCAS(a.err, 0, kErrCacheLength);
         return;
     }
+    int *kept = a.kept + (size_t)bh * a.keep;
     const float *w = a.weights + (size_t)bh * a.capacity;
+    float *w_out = a.weights_out + (size_t)bh * a.capacity;
     const int count = min(n, a.keep), last = max(0, n - a.recent);
-    int need = count - (n - last);  // of the first `last` entries
-    uint32_t prefix = 0;
-    const bool all = need >= last;
-    for (int shift = 24; shift >= 0 && !all && need > 0; shift -= 8) {
-        for (int i = threadIdx.x; i < 256; i += kSelectThreads) hist[i] = 0;
+    uint32_t need = count - (n - last);  // of the first `last` entries
+    const bool all = need >= (uint32_t)last, single = n <= kSelectTile;
+    auto at = [](int j) { return j + (j >> 5); };  // a thread's run of 8 without bank conflicts
+    auto load_tile = [&](int j0) {
+#pragma unroll
+        for (int u = 0; u < kSelectEach; ++u) {
+            const int j = u * kSelectThreads + thread;
+            if (j0 + j < n) keys[at(j)] = weight_key(w[j0 + j]);
+        }
+    };
+    uint32_t threshold = 0;
+    if (single) load_tile(0);
+    for (int pass = 0; pass < 3 && !all && need > 0; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, digit = pass < 2 ? 11 : 10;
+        for (int i = thread; i < kBins; i += kSelectThreads) hist[i] = 0;
         __syncthreads();
-        for (int j = threadIdx.x; j < last; j += kSelectThreads) {
-            const uint32_t key = weight_key(w[j]);
-            if (shift == 24 || key >> (shift + 8) == prefix) atomicAdd(&hist[key >> shift & 255], 1);
+        for (int j = thread; j < last; j += kSelectThreads) {
+            const uint32_t key = single ? keys[at(j)] : weight_key(w[j]);
+            if (pass == 0 || key >> (shift + digit) == threshold) atomicAdd(&hist[key >> shift & ((1u << digit) - 1)], 1u);
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            int above = 0, d = 255;
-            while (above + hist[d] < need) above += hist[d--];
-            chosen[0] = d, chosen[1] = need - above;
-        }
+        const int high = kBins - 1 - 2 * thread;  // two bins a thread, the largest first
+        const uint32_t c0 = hist[high], c1 = hist[high - 1];
+        uint32_t total;
+        const uint32_t above = block_prefix(c0 + c1, warp_sums, total);
+        if (above < need && need <= above + c0) chosen[0] = high, chosen[1] = need - above;
+        else if (above + c0 < need && need <= above + c0 + c1) chosen[0] = high - 1, chosen[1] = need - above - c0;
         __syncthreads();
-        prefix = prefix << 8 | (uint32_t)chosen[0];
+        threshold = threshold << digit | chosen[0];
         need = chosen[1];
     }
-    // prefix: the smallest kept key; need: how many entries with exactly it are kept
-    int ties = 0, written = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelectThreads) {
-        const int j = j0 + threadIdx.x;
-        bool take = j < n && (all || j >= last), tie = false;
-        if (!all && j < last && need > 0) {
-            const uint32_t key = weight_key(w[j]);
-            take = key > prefix;
-            tie = key == prefix;
+    // threshold: the smallest kept key; need: how many entries with exactly it are kept, the lowest slots
+    uint32_t takes = 0, ties = 0;
+    for (int j0 = 0; j0 < n; j0 += kSelectTile) {
+        __syncthreads();
+        if (!single) {
+            load_tile(j0);
+            __syncthreads();
         }
-        int total;
-        if (!all && need > 0) {
-            const int rank = block_rank(tie, warp_sums, total);
-            take = take || (tie && ties + rank < need);
-            ties += total;
+        uint32_t mask = 0, equal = 0;
+#pragma unroll
+        for (int i = 0; i < kSelectEach; ++i) {
+            const int j = j0 + thread * kSelectEach + i;
+            if (j >= n) break;
+            const uint32_t key = keys[at(thread * kSelectEach + i)];
+            if (all || j >= last || (need > 0 && key > threshold)) mask |= 1u << i;
+            else if (need > 0 && key == threshold) equal |= 1u << i;
         }
-        const int at = written + block_rank(take, warp_sums, total);
-        if (take) {
-            kept[at] = j;
-            w_out[at] = w[j];
+        uint32_t total;
+        const uint32_t before = block_prefix(__popc(mask) | __popc(equal) << 16, warp_sums, total);
+        uint32_t take = takes + (before & 0xffffu), tie = ties + (before >> 16);
+#pragma unroll
+        for (int i = 0; i < kSelectEach; ++i) {
+            const bool is_tie = equal >> i & 1, on = (mask >> i & 1) || (is_tie && tie < need);
+            if (on) {
+                const int j = j0 + thread * kSelectEach + i;
+                const uint32_t to = take + min(tie, need);
+                kept[to] = j;
+                w_out[to] = w[j];
+            }
+            take += mask >> i & 1;
+            tie += is_tie;
         }
-        written += total;
+        takes += total & 0xffffu, ties += total >> 16;
     }
-    for (int i = count + threadIdx.x; i < a.keep; i += kSelectThreads) kept[i] = -1;
-    for (int i = count + threadIdx.x; i < a.capacity; i += kSelectThreads) w_out[i] = 0.0f;
-    if (bh % a.kv_heads == 0 && threadIdx.x == 0) a.lengths_out[b] = count;
+    for (int i = count + thread; i < a.keep; i += kSelectThreads) kept[i] = -1;
+    for (int i = count + thread; i < a.capacity; i += kSelectThreads) w_out[i] = 0.0f;
+    if (bh % a.kv_heads == 0 && thread == 0) a.lengths_out[b] = count;
 }
 
 __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
@@ -126,6 +157,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
     const int *kept = a.kept + (size_t)bh * a.keep;
     const size_t base = (size_t)bh * a.capacity;
     const long long total = (long long)count * a.vecs;
+    grid_dependency_wait();  // kept; in every block: this grid's end stands for the one's before it
     if (n < 0 || n > a.capacity) return;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
         const int row = (int)(i / a.vecs), vec = (int)(i - (long long)row * a.vecs);
@@ -220,8 +252,8 @@ LaunchFn make_cache_op(Context *ctx, const Spec &s, std::string &impl) {
         a.lengths = static_cast<const int *>(b[3]), a.k_out = static_cast<uint4 *>(b[4]), a.v_out = static_cast<uint4 *>(b[5]);
         a.weights_out = static_cast<float *>(b[6]), a.kept = static_cast<int *>(b[7]), a.lengths_out = static_cast<int *>(b[8]);
         evict_select_kernel<<<heads, kSelectThreads, 0, st>>>(a);
-        evict_move_kernel<<<dim3(blocks, heads), 256, 0, st>>>(a);
-        return cudaGetLastError();
+        const cudaError_t e = launch_after(st, evict_move_kernel, dim3(blocks, heads), 256, 0, a);
+        return e == cudaSuccess ? cudaGetLastError() : e;
     };
 }
 

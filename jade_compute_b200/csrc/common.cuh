@@ -425,9 +425,9 @@ __device__ __forceinline__ float stable_sigmoid(float v) {
 // Launches `kernel` so that its blocks may start, up to grid_dependency_wait, while
 // the kernel before it on the stream still runs.
 template <typename... P, typename... A>
-cudaError_t launch_after(cudaStream_t st, void (*kernel)(P...), int grid, int block, size_t smem, A &&...args) {
+cudaError_t launch_after(cudaStream_t st, void (*kernel)(P...), dim3 grid, int block, size_t smem, A &&...args) {
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(grid), config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = st;
+    config.gridDim = grid, config.blockDim = dim3(block), config.dynamicSmemBytes = smem, config.stream = st;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
