@@ -91,6 +91,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, i
         if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrCacheLength);
         return;
     }
+    grid_dependency_trigger();
     const int n = length + a.seq, tiles = (n + kKeys - 1) / kKeys;
     const int t0 = (int)((long long)tiles * blockIdx.y / splits), t1 = (int)((long long)tiles * (blockIdx.y + 1) / splits);
     const size_t base = (size_t)bh * a.capacity * a.dim;
@@ -153,6 +154,8 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, i
 template <typename T>
 __global__ void __launch_bounds__(128) tree_join_kernel(const TreeArgs a, int splits, int total_rows) {
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    grid_dependency_trigger();
+    grid_dependency_wait();
     if (row >= total_rows) return;
     const int bh = row / a.rows, rr = row - bh * a.rows, b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
     if (a.lengths[b] < 0 || a.lengths[b] > a.capacity - a.seq) return;
@@ -186,6 +189,7 @@ __global__ void __launch_bounds__(kThreads) tree_weights_simt_kernel(const TreeA
     float *q = smem, *k = q + kRows * q_stride(a.dim), *sums = k + kKeys * q_stride(a.dim);
     const int bh = blockIdx.y, b = bh / a.kv_heads, r = threadIdx.x >> 3, c = threadIdx.x & 7;
     const int length = a.lengths[b], n = length + a.seq;
+    grid_dependency_wait();  // the rows' stats
     if (length < 0 || length > a.capacity - a.seq) return;
     for (int j0 = blockIdx.x * kKeys; j0 < n; j0 += gridDim.x * kKeys) {
         float acc[4] = {};
@@ -220,9 +224,9 @@ LaunchFn simt_launch(Context *ctx, const Spec &s) {
     TreeArgs base = tree_args(ctx, s);
     const int heads = (int)(s.batch * s.kv_heads), rows = base.rows, row_blocks = (rows + kRows - 1) / kRows, total_rows = heads * rows;
     if (heads > 65535) throw IrError("attention_tree: batch * kv_heads must be at most 65535");
-    // about four blocks per SM, each with at least four tiles of keys
+    // about four blocks per SM
     const long long items = (long long)heads * row_blocks;
-    const int splits = (int)std::max<long long>(1, std::min<long long>({(4ll * ctx->sm_count + items - 1) / items, ((long long)s.capacity + 4 * kKeys - 1) / (4 * kKeys), 64ll}));
+    const int splits = (int)std::max<long long>(1, std::min<long long>({(4ll * ctx->sm_count + items - 1) / items, ((long long)s.capacity + kKeys - 1) / kKeys, 64ll}));
     const size_t stats = (size_t)total_rows * sizeof(float2), ml = stats * splits;
     auto ws = kernel_workspace(stats + ml + (size_t)total_rows * splits * s.dim * 4, "attention_tree partial results");
     base.stats = static_cast<float2 *>(ws.get());
@@ -238,9 +242,9 @@ LaunchFn simt_launch(Context *ctx, const Spec &s) {
     return [=, keep = ws](cudaStream_t st, void **b) {
         const TreeArgs a = tree_bind(base, b, weights);
         tree_simt_kernel<T><<<dim3(row_blocks, splits, heads), kThreads, smem, st>>>(a, splits);
-        tree_join_kernel<T><<<(total_rows + 3) / 4, 128, 0, st>>>(a, splits, total_rows);
-        if (weights) tree_weights_simt_kernel<T><<<dim3(key_blocks, heads), kThreads, smem_w, st>>>(a);
-        return cudaGetLastError();
+        cudaError_t e = launch_after(st, tree_join_kernel<T>, dim3((total_rows + 3) / 4), 128, 0, a, splits, total_rows);
+        if (weights && e == cudaSuccess) e = launch_after(st, tree_weights_simt_kernel<T>, dim3(key_blocks, heads), kThreads, smem_w, a);
+        return e == cudaSuccess ? cudaGetLastError() : e;
     };
 }
 
