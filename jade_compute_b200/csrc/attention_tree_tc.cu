@@ -60,8 +60,16 @@ struct Layout {
     static constexpr uint32_t kSmem = kBytes + 1024 < 227 * 1024 ? kBytes + 1024 : 227 * 1024;
 };
 
-// Rows of stats per item: whole groups of 16 columns of the weights' MMA, the last ones zero.
-__host__ __device__ constexpr size_t stats_stride(int rows) { return ((size_t)rows + 15) / 16 * 16; }
+// Stats of an item: x of every row, p_j = 2^(s_j scale_log2 + x) (the row's sum folded
+// into the exponent: one constant per column for the weights' pass to read), -inf for
+// rows that see nothing and up to whole groups of 32 columns of that pass's MMA.
+__host__ __device__ constexpr size_t stats_stride(int rows) { return ((size_t)rows + 31) / 32 * 32; }
+__device__ __forceinline__ void store_stats(const TreeArgs &t, size_t item, int row, float m, float inv) {
+    float *x = t.row_exponents + item * stats_stride(t.rows) + row;
+    *x = log2f(inv) - (m == -INFINITY ? 0.0f : m);
+    if (row == t.rows - 1)
+        for (int r = t.rows; r < (int)stats_stride(t.rows); ++r) *++x = -INFINITY;
+}
 
 struct TcArgs {
     TreeArgs t;
@@ -598,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (both) mbar_arrive(&o_free[1]);
             if (valid && (kTwoTiles || t == 0)) {
                 if (!whole) ta.part_ml[slot * slot_rows + slot_row] = make_float2(m_used, l_run);
-                else if (ta.stats) ta.stats[(size_t)bh * stats_stride(ta.rows) + item_row] = make_float2(m_used == -INFINITY ? 0.0f : m_used, inv);
+                else if (ta.row_exponents) store_stats(ta, bh, item_row, m_used, inv);
             }
         }
     }
@@ -663,7 +671,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_tc(const TcArgs a, int
         o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
     }
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (col == 0 && t.stats) t.stats[((size_t)b * t.kv_heads + hk) * stats_stride(t.rows) + row] = make_float2(shift, inv);
+    if (col == 0 && t.row_exponents) store_stats(t, (size_t)b * t.kv_heads + hk, row, m, inv);
     if (col * 4 >= t.dim) return;
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const int g = row / t.seq, tok = row - g * t.seq;
@@ -672,15 +680,18 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_tc(const TcArgs a, int
 }
 
 // ------------------------------------------------------------------ weights
-// weights[j] += sum over the item's M rows of p_j = 2^(s_j c - x) y, (x, y) the
-// rows' stats from the pass before. Transposed, S^T = K Q^T with 128 keys in the TMEM
+// weights[j] += sum over the item's M rows of p_j = 2^(s_j c + x), x the rows' stats
+// from the pass before. Transposed, S^T = K Q^T with 128 keys in the TMEM
 // lanes and up to 256 rows of Q in the columns, so that a thread owns a key and adds
 // its row of p in order: no sums between threads, no atomics. Ranges of key tiles per
-// CTA as above; more than 256 rows take several passes over the segment's keys.
+// CTA as above; more than 256 rows take several passes over the segment's keys. Tiles
+// go last to first: the pass before has left a range's last ones in L2.
 // Bound by K's second read and by one exponential per (row, key).
 //   warp 0 TMA (Q rows and their stats per segment, K tiles through a ring),
-//   warp 1 MMA into two buffers, warps 2-5 and 6-9 take the tiles in turn.
-constexpr int kWeightRows = 256, kWeightsBoundary = 2;
+//   warp 1 MMA into two or four buffers (four where 128 columns do, so that S of a
+//   group's next tile is ready when it has finished one), warps 2-5 and 6-9 take the
+//   tiles in turn.
+constexpr int kWeightRows = 256, kWeightsBoundary = 2, kTreeBytes = 128 * 4 * 4;
 
 template <int DP>
 struct WeightsLayout {
@@ -689,7 +700,8 @@ struct WeightsLayout {
     static constexpr int kStages = DP == 128 ? 4 : 8;
     static constexpr uint32_t kRing = (DP / 64) * kRows64;
     static constexpr uint32_t kStats = kRing + kStages * kTile;
-    static constexpr uint32_t kBar = kStats + kWeightRows * 8;
+    static constexpr uint32_t kTree = kStats + kWeightRows * 4;  // per consumer warp: the sequence's tree words
+    static constexpr uint32_t kBar = kTree + 8 * kTreeBytes;
     static constexpr uint32_t kSmem = kBar + 512 + 1024;
 };
 
@@ -702,21 +714,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBar);
-    uint64_t *q_full = bars, *q_empty = bars + 1, *s_full = bars + 2, *s_empty = bars + 4, *mma_done = bars + 6;
-    uint64_t *full = bars + 8, *empty = bars + 8 + kStages;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
+    uint64_t *q_full = bars, *q_empty = bars + 2, *mma_done = bars + 4, *s_full = bars + 5, *s_empty = bars + 9;
+    uint64_t *full = bars + 13, *empty = bars + 13 + kStages;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 30);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     int *plan = reinterpret_cast<int *>(tmem_slot + 2);
     long long *scratch = reinterpret_cast<long long *>(tmem_slot + 6);
-    const float2 *stats = reinterpret_cast<const float2 *>(smem + L::kStats);
 
     const TreeArgs &ta = args.t;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *err = ta.err;
     int ring_loads = 0, q_loads = 0;
     if (threadIdx.x == 0) {
-        mbar_init(q_full, 1); mbar_init(q_empty, 1 + 256); mbar_init(mma_done, 1);
-        for (int t = 0; t < 2; ++t) mbar_init(&s_full[t], 1), mbar_init(&s_empty[t], 128);
+        mbar_init(mma_done, 1);
+        for (int t = 0; t < 2; ++t) mbar_init(&q_full[t], 1), mbar_init(&q_empty[t], 1 + 256);
+        for (int t = 0; t < 4; ++t) mbar_init(&s_full[t], 1), mbar_init(&s_empty[t], 128);
         for (int i = 0; i < kStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
         *abort_flag = 0;
         fence_barrier_init();
@@ -728,34 +740,50 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     Segments segments = open_range(args, plan, scratch);
     const uint32_t tmem = *tmem_slot;
+    // Up to 128 rows: four S buffers, and Q of the next segment loads beside this one's
+    // (128 rows each); else two buffers, one Q of up to 256 rows at a time.
+    const bool narrow = ta.rows <= 128;
+    const int buffers = narrow ? 4 : 2, buffer_columns = 512 / buffers;
+    auto q_buffer = [&](int use) { return narrow ? use & 1 : 0; };
+    auto q_phase = [&](int use) { return narrow ? use >> 1 & 1 : use & 1; };
     Segment s;
 
     if (warp == 0) {
         if (lane == 0) {
             tma_prefetch_desc(&tmQ);
             tma_prefetch_desc(&tmK);
-            bool ok = true;
-            grid_dependency_wait();  // the rows' stats
+            bool ok = true, waited = false;
             while (ok && segments.next(args, s)) {
-                const int bh = s.b * ta.kv_heads + s.hk;
+                const int bh = s.b * ta.kv_heads + s.hk, n = s.count();
+                const float *item = ta.row_exponents + (size_t)bh * stats_stride(ta.rows);
                 for (int r0 = 0; ok && r0 < ta.rows; r0 += kWeightRows) {
-                    if (!(ok = mbar_wait(q_empty, (q_loads & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) break;
-                    const int boxes = min(2, (ta.rows - r0 + 127) / 128), padded = min(kWeightRows, (ta.rows - r0 + 15) & ~15);
-                    mbar_arrive_expect_tx(q_full, boxes * L::kTile + padded * 8);
+                    const int qb = q_buffer(q_loads);
+                    if (!(ok = mbar_wait(&q_empty[qb], q_phase(q_loads) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) break;
+                    const int boxes = min(2, (ta.rows - r0 + 127) / 128), padded = min(kWeightRows, (ta.rows - r0 + 31) & ~31);
+                    mbar_arrive_expect_tx(&q_full[qb], boxes * L::kTile + padded * 4);
                     for (int t = 0; t < boxes; ++t)
                         for (int c = 0; c < kDChunks; ++c)
-                            tma_load_3d(smem + c * L::kRows64 + t * 128 * 128, &tmQ, q_full, c * 64, r0 + t * 128, bh);
-                    bulk_load(smem + L::kStats, ta.stats + (size_t)bh * stats_stride(ta.rows) + r0, padded * 8, q_full);
+                            tma_load_3d(smem + c * L::kRows64 + (qb + t) * 128 * 128, &tmQ, &q_full[qb], c * 64, r0 + t * 128, bh);
                     ++q_loads;
-                    for (int i = s.first; i < s.last; ++i, ++ring_loads) {
+                    auto load = [&](int i) {
                         const int st = ring_loads % kStages;
-                        if (!(ok = mbar_wait(&empty[st], (ring_loads / kStages & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) break;
+                        if (!(ok = mbar_wait(&empty[st], (ring_loads / kStages & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) return;
                         mbar_arrive_expect_tx(&full[st], L::kTile);
                         for (int c = 0; c < kDChunks; ++c)
-                            tma_load_3d(smem + L::kRing + st * L::kTile + c * 128 * 128, &tmK, &full[st], c * 64, i * kTileKeys, bh);
+                            tma_load_3d(smem + L::kRing + st * L::kTile + c * 128 * 128, &tmK, &full[st], c * 64, (s.last - 1 - i) * kTileKeys, bh);
+                        ++ring_loads;
+                    };
+                    int i = 0;
+                    if (!waited) {  // the first tiles are under way before the rows' stats are there
+                        for (; i < min(n, kStages); ++i) load(i);
+                        grid_dependency_wait();
+                        waited = true;
                     }
+                    bulk_load(smem + L::kStats + qb * 128 * 4, item + r0, padded * 4, &q_full[qb]);
+                    for (; ok && i < n; ++i) load(i);
                 }
             }
+            if (!waited) grid_dependency_wait();  // in every block: this grid's end stands for the one's before it
         }
     } else if (warp == 1) {
         auto wait = [&](uint64_t *bar, uint32_t parity, int code) {
@@ -766,65 +794,86 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         while (ok && segments.next(args, s))
             for (int r0 = 0; ok && r0 < ta.rows; r0 += kWeightRows) {
-                const uint32_t idesc = idesc_f32acc(kFmt, kFmt, false, false, kTileKeys, min(kWeightRows, (ta.rows - r0 + 15) & ~15));
-                ok = wait(q_full, qn++ & 1, kErrWaitTmaFull);
+                const uint32_t idesc = idesc_f32acc(kFmt, kFmt, false, false, kTileKeys, min(kWeightRows, (ta.rows - r0 + 31) & ~31));
+                const int qb = q_buffer(qn);
+                ok = wait(&q_full[qb], q_phase(qn++), kErrWaitTmaFull);
                 for (int i = s.first; ok && i < s.last; ++i, ++pos) {
-                    const int st = pos % kStages, t = pos & 1;
-                    ok = wait(&full[st], pos / kStages & 1, kErrWaitTmaFull) && wait(&s_empty[t], (pos >> 1 & 1) ^ 1, kErrWaitAccEmpty);
+                    const int st = pos % kStages, t = pos % buffers;
+                    ok = wait(&full[st], pos / kStages & 1, kErrWaitTmaFull) && wait(&s_empty[t], (pos / buffers & 1) ^ 1, kErrWaitAccEmpty);
                     if (!ok) break;
                     tc_fence_after();
                     uint64_t a[DP / 16], b[DP / 16];
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         a[k] = dk0 + ((st * L::kTile + (k >> 2) * 128 * 128 + (k & 3) * 32) >> 4);
-                        b[k] = dq0 + (((k >> 2) * L::kRows64 + (k & 3) * 32) >> 4);
+                        b[k] = dq0 + (((k >> 2) * L::kRows64 + qb * 128 * 128 + (k & 3) * 32) >> 4);
                     }
-                    umma_ss_group<DP / 16>(tmem + t * kWeightRows, a, b, idesc, 0);
+                    umma_ss_group<DP / 16>(tmem + t * buffer_columns, a, b, idesc, 0);
                     umma_commit(&s_full[t]);
                     umma_commit(&empty[st]);
                 }
-                umma_commit(q_empty);
+                umma_commit(&q_empty[qb]);
             }
         umma_commit(mma_done);
         mbar_wait_drain(mma_done, 0, err);
     } else {
-        const int t = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane;
-        const uint32_t ts = tmem + t * kWeightRows + ((uint32_t)(quarter * 32) << 16);
+        const int group = (warp - 2) >> 2, quarter = warp & 3, key = quarter * 32 + lane;
         const float c = ta.scale_log2;
+        const uint64_t c2 = pack2f(c, c);
+        uint32_t *tree = reinterpret_cast<uint32_t *>(smem + L::kTree + (warp - 2) * kTreeBytes);
         int pos = 0, qn = 0;
         bool ok = true;
         while (ok && segments.next(args, s)) {
             float *weights = ta.weights + ((size_t)s.b * ta.kv_heads + s.hk) * ta.capacity;
             for (int r0 = 0; ok && r0 < ta.rows; r0 += kWeightRows) {
-                ok = __all_sync(0xffffffffu, mbar_wait(q_full, qn++ & 1, abort_flag, err, kErrWaitTmaFull));
+                const int qb = q_buffer(qn);
+                if (s.last * kTileKeys > s.length && r0 == 0) {  // the segment reaches the drafts
+                    __syncwarp();
+                    for (int i = lane; i < ta.seq * ta.words; i += 32) tree[i] = __ldg(ta.tree + (size_t)s.b * ta.seq * ta.words + i);
+                    __syncwarp();
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&q_full[qb], q_phase(qn++), abort_flag, err, kErrWaitTmaFull));
+                const float *stats = reinterpret_cast<const float *>(smem + L::kStats) + qb * 128;
                 const int count = min(kWeightRows, ta.rows - r0);
-                for (int i = s.first; ok && i < s.last; ++i, ++pos) {
-                    if ((pos & 1) != t) continue;
-                    const int j = i * kTileKeys + key, draft = j - s.length;
+                for (int i = s.last - 1; ok && i >= s.first; --i, ++pos) {
+                    if ((pos & 1) != group) continue;
+                    const int t = pos % buffers, j = i * kTileKeys + key, draft = j - s.length;
+                    const uint32_t ts = tmem + t * buffer_columns + ((uint32_t)(quarter * 32) << 16);
                     const float old = draft < ta.seq ? weights[j] : 0.0f;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], pos >> 1 & 1, abort_flag, err, kErrWaitScore));
+                    ok = __all_sync(0xffffffffu, mbar_wait(&s_full[t], pos / buffers & 1, abort_flag, err, kErrWaitScore));
                     if (!ok) break;
                     tc_fence_after();
                     float sum = 0.0f;
                     if (i * kTileKeys + kTileKeys <= s.length) {
-                        float sums[4] = {};
+                        // columns beyond the rows are products with zeros, their exponent is -inf
+                        uint64_t sums[2] = {0, 0};
+                        float sv[32];
+                        tmem_ld32f(ts, sv);
 #pragma unroll 1
                         for (int n = 0; n < count; n += 32) {
-                            float sv[32];
-                            tmem_ld32f(ts + n, sv);
                             tmem_wait_ld();
+                            reg_fence(sv);
+                            float e[32];
 #pragma unroll
-                            for (int k = 0; k < 32; k += 2) {
-                                const float4 st = *reinterpret_cast<const float4 *>(stats + n + k);
-                                if (n + k < count) {
-                                    sums[k & 2] = fmaf(mufu_exp2(fmaf(sv[k], c, -st.x)), st.y, sums[k & 2]);
-                                    sums[(k & 2) + 1] = fmaf(mufu_exp2(fmaf(sv[k + 1], c, -st.z)), st.w, sums[(k & 2) + 1]);
-                                }
+                            for (int k = 0; k < 32; ++k) e[k] = sv[k];
+                            if (n + 32 < count) tmem_ld32f(ts + n + 32, sv);
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4) {
+                                const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(stats + n + k);
+                                float a0, a1, b0, b1;
+                                unpack2f(fma2(pack2f(e[k], e[k + 1]), c2, x.x), a0, a1);
+                                unpack2f(fma2(pack2f(e[k + 2], e[k + 3]), c2, x.y), b0, b1);
+                                sums[0] = add2(pack2f(mufu_exp2(a0), mufu_exp2(a1)), sums[0]);
+                                sums[1] = add2(pack2f(mufu_exp2(b0), mufu_exp2(b1)), sums[1]);
                             }
                         }
-                        sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                        float a0, a1;
+                        unpack2f(add2(sums[0], sums[1]), a0, a1);
+                        sum = a0 + a1;
                     } else {
-                        const uint32_t *tree = ta.tree + (size_t)s.b * ta.seq * ta.words + (max(draft, 0) >> 5);
+                        // selected without branches: lanes lie on both sides of the first draft
+                        const uint32_t *word = tree + (min(max(draft, 0), ta.seq - 1) >> 5);
+                        const uint32_t always = draft < 0, drafted = draft >= 0 && draft < ta.seq;
                         int tok = r0 % ta.seq;
 #pragma unroll 1
                         for (int n = 0; n < count; n += 16) {
@@ -833,10 +882,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tmem_wait_ld();
 #pragma unroll
                             for (int k = 0; k < 16; ++k) {
-                                const bool sees = n + k < count && (draft < 0 || (draft < ta.seq && __ldg(tree + (size_t)tok * ta.words) >> (draft & 31) & 1));
-                                const float2 st = stats[min(n + k, kWeightRows - 1)];
-                                if (sees) sum = fmaf(mufu_exp2(fmaf(__uint_as_float(raw[k]), c, -st.x)), st.y, sum);
-                                if (++tok == ta.seq) tok = 0;
+                                const uint32_t sees = always | (word[tok * ta.words] >> (draft & 31) & drafted);
+                                const float p = mufu_exp2(fmaf(__uint_as_float(raw[k]), c, stats[n + k]));
+                                sum += sees && n + k < count ? p : 0.0f;
+                                tok = tok + 1 == ta.seq ? 0 : tok + 1;
                             }
                         }
                     }
@@ -844,7 +893,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     mbar_arrive(&s_empty[t]);
                     if (draft < ta.seq) weights[j] = old + sum;
                 }
-                mbar_arrive(q_empty);
+                mbar_arrive(&q_empty[qb]);
             }
         }
     }
@@ -853,7 +902,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
         if (lane == 0 && *abort_flag) {
             for (int i = max(0, ring_loads - kStages); i < ring_loads; ++i) mbar_wait_drain(&full[i % kStages], i / kStages & 1, err);
-            if (q_loads) mbar_wait_drain(q_full, (q_loads - 1) & 1, err);
+            for (int i = max(0, q_loads - (narrow ? 2 : 1)); i < q_loads; ++i) mbar_wait_drain(&q_full[q_buffer(i)], q_phase(i), err);
         }
         __syncwarp();
         tc_fence_after();
@@ -903,9 +952,9 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
     const long long join_blocks = (long long)heads * base.row_blocks * item_blocks;
     if (join_blocks > INT_MAX) throw IrError("attention_tree too large for one launch");
     const bool weights = s.weights;
-    const size_t stats = (heads * stats_stride((int)rows) * sizeof(float2) + 255) / 256 * 256, slots = (size_t)base.ctas * 2 * base.slot_rows;
+    const size_t stats = (heads * stats_stride((int)rows) * sizeof(float) + 255) / 256 * 256, slots = (size_t)base.ctas * 2 * base.slot_rows;
     auto ws = kernel_workspace(stats + slots * (sizeof(float2) + DP * sizeof(float)), "attention_tree partial results");
-    base.t.stats = weights ? static_cast<float2 *>(ws.get()) : nullptr;
+    base.t.row_exponents = weights ? static_cast<float *>(ws.get()) : nullptr;
     base.t.part_o = reinterpret_cast<float *>(static_cast<char *>(ws.get()) + stats);
     base.t.part_ml = reinterpret_cast<float2 *>(base.t.part_o + slots * DP);
     const CUtensorMapDataType dt = std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
