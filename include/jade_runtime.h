@@ -119,6 +119,10 @@ typedef struct jr_dispatch {
  * each other (e.g. one repeat's result read-back with the next repeat's uploads).
  * No counterpart in the reference (its execute is strictly in order). */
 #define JR_EXEC_STREAMS 2u
+/* The batch's event time is not read back: *gpu_ms stays 0 and jr_batch_ms returns
+ * it on request (reading the events costs about 3 us of host time per batch on a
+ * B200 host, which callers of short batches need not pay). */
+#define JR_EXEC_DEFER_MS 4u
 
 /* Validates every job (context ownership, registered buffers, exact byte sizes,
  * output aliasing - corex.rs:557-569, ir.rs:340-367) before any work is
@@ -127,6 +131,9 @@ typedef struct jr_dispatch {
  * not with JR_EXEC_GRAPH): per-job event time summed over repeats. */
 JR_API int jr_execute2(void *ctx, const jr_dispatch *jobs, size_t job_count, uint32_t repeats, uint32_t flags,
                 double *gpu_ms, double *job_ms, char *err, size_t cap);
+
+/* Event time of the context's last batch that completed, until its next one starts. */
+JR_API int jr_batch_ms(void *ctx, double *gpu_ms, char *err, size_t cap);
 
 /* Registry queries and pinned host memory for transfer jobs (spec op "copy"). */
 JR_API int jr_buffer_bytes(void *ctx, const void *ptr, size_t *bytes);

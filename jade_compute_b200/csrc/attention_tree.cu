@@ -27,6 +27,7 @@ namespace jade {
 namespace {
 
 constexpr int kThreads = 128, kRows = 16, kKeys = 32;  // a block: 16 rows of q, tiles of 32 keys
+constexpr int kMaxSplits = 64;
 
 template <typename T>
 __device__ __forceinline__ float4 load4(const T *p);
@@ -47,15 +48,20 @@ __device__ __forceinline__ float4 load4<__half>(const __half *p) {
 
 __host__ __device__ constexpr int q_stride(int dim) { return dim + 4; }  // rows 4 banks apart
 
-// Rows of q or keys (zeros from `limit` on) as FP32 into shared memory.
-template <typename T>
-__device__ __forceinline__ void stage(float *dst, const T *src, int first, int count, int limit, int dim) {
-    const int vecs = dim / 4;
-    for (int i = threadIdx.x; i < count * vecs; i += kThreads) {
-        const int r = i / vecs, c = (i - r * vecs) * 4;
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (first + r < limit) x = load4(src + (size_t)(first + r) * dim + c);
-        *reinterpret_cast<float4 *>(dst + r * q_stride(dim) + c) = x;
+// Rows of q or keys (zeros from `limit` on) as FP32 into shared memory: 8 threads a
+// row, 16 rows at a time, the loads of all of a thread's rows under way together.
+template <typename T, int kCount>
+__device__ __forceinline__ void stage(float *dst, const T *src, int first, int limit, int dim) {
+    const int r = threadIdx.x >> 3;
+    for (int c = (threadIdx.x & 7) * 4; c < dim; c += 32) {
+        float4 x[kCount / 16];
+#pragma unroll
+        for (int i = 0; i < kCount / 16; ++i) {
+            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (first + r + 16 * i < limit) x[i] = load4(src + (size_t)(first + r + 16 * i) * dim + c);
+        }
+#pragma unroll
+        for (int i = 0; i < kCount / 16; ++i) *reinterpret_cast<float4 *>(dst + (r + 16 * i) * q_stride(dim) + c) = x[i];
     }
 }
 
@@ -80,8 +86,8 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, int b, int row, int j, i
     return a.tree[((size_t)b * a.seq + row % a.seq) * a.words + (i >> 5)] >> (i & 31) & 1;
 }
 
-// grid: (row blocks, splits, batch * kv_heads)
-template <typename T>
+// grid: (row blocks, splits, batch * kv_heads); kCols: 32-element columns of a head
+template <typename T, int kCols>
 __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, int splits) {
     extern __shared__ float smem[];
     float *q = smem, *k = q + kRows * q_stride(a.dim), *v = k + kKeys * q_stride(a.dim), *p = v + kKeys * q_stride(a.dim);
@@ -95,16 +101,16 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, i
     const int n = length + a.seq, tiles = (n + kKeys - 1) / kKeys;
     const int t0 = (int)((long long)tiles * blockIdx.y / splits), t1 = (int)((long long)tiles * (blockIdx.y + 1) / splits);
     const size_t base = (size_t)bh * a.capacity * a.dim;
-    stage(q, static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, blockIdx.x * kRows, kRows, a.rows, a.dim);
+    stage<T, kRows>(q, static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, blockIdx.x * kRows, a.rows, a.dim);
     float m = -INFINITY, l = 0.0f;
-    float4 o[8];
+    float4 o[kCols];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < kCols; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int t = t0; t < t1; ++t) {
         const int j0 = t * kKeys;
         __syncthreads();
-        stage(k, static_cast<const T *>(a.k) + base, j0, kKeys, n, a.dim);
-        stage(v, static_cast<const T *>(a.v) + base, j0, kKeys, n, a.dim);
+        stage<T, kKeys>(k, static_cast<const T *>(a.k) + base, j0, n, a.dim);
+        stage<T, kKeys>(v, static_cast<const T *>(a.v) + base, j0, n, a.dim);
         __syncthreads();
         float s[4], top = -INFINITY;
         tile_scores(q, k, r, c, a.dim, s);
@@ -128,16 +134,22 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, i
         l = l * alpha + sum;  // this thread's keys
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i].x *= alpha, o[i].y *= alpha, o[i].z *= alpha, o[i].w *= alpha;
-        for (int j = 0; j < kKeys; ++j) {
-            const float w = p[r * (kKeys + 1) + j];
-            if (w == 0.0f) continue;  // not seen, or below FP32: no product
+        for (int i = 0; i < kCols; ++i) o[i].x *= alpha, o[i].y *= alpha, o[i].z *= alpha, o[i].w *= alpha;
+        auto add = [&](int j, float w) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < kCols; ++i)
                 if ((c + 8 * i) * 4 < a.dim) {
                     const float4 x = *reinterpret_cast<const float4 *>(v + j * q_stride(a.dim) + (c + 8 * i) * 4);
                     o[i].x = fmaf(w, x.x, o[i].x), o[i].y = fmaf(w, x.y, o[i].y), o[i].z = fmaf(w, x.z, o[i].z), o[i].w = fmaf(w, x.w, o[i].w);
                 }
+        };
+        const float *mine = p + r * (kKeys + 1);
+        if (j0 + kKeys <= length) {
+#pragma unroll 4
+            for (int j = 0; j < kKeys; ++j) add(j, mine[j]);
+        } else {  // drafts: no product with one that the row does not see
+            for (int j = 0; j < kKeys; ++j)
+                if (mine[j] != 0.0f) add(j, mine[j]);
         }
     }
 #pragma unroll
@@ -146,66 +158,86 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, i
     const size_t at = ((size_t)bh * a.rows + row) * splits + blockIdx.y;
     if (c == 0) a.part_ml[at] = make_float2(m, l);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < kCols; ++i)
         if ((c + 8 * i) * 4 < a.dim) *reinterpret_cast<float4 *>(a.part_o + at * a.dim + (c + 8 * i) * 4) = o[i];
 }
 
 // Joins the splits of one row: one warp a row.
 template <typename T>
-__global__ void __launch_bounds__(128) tree_join_kernel(const TreeArgs a, int splits, int total_rows) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    grid_dependency_trigger();
-    grid_dependency_wait();
+__device__ __forceinline__ void join_rows(const TreeArgs &a, int splits, int total_rows, int block) {
+    const int row = block * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= total_rows) return;
     const int bh = row / a.rows, rr = row - bh * a.rows, b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
     if (a.lengths[b] < 0 || a.lengths[b] > a.capacity - a.seq) return;
+    // lane s holds splits s and s + 32 (at most kMaxSplits)
     const float2 *ml = a.part_ml + (size_t)row * splits;
-    float m = -INFINITY, l = 0.0f;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[s].x);
+    const float2 none = make_float2(-INFINITY, 0.0f);
+    const float2 u = lane < splits ? ml[lane] : none, v = lane + 32 < splits ? ml[lane + 32] : none;
+    float m = fmaxf(u.x, v.x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float shift = m == -INFINITY ? 0.0f : m;
-    for (int s = 0; s < splits; ++s) l += ml[s].y * exp2f((ml[s].x - shift) * a.scale_log2);
+    const float wu = exp2f((u.x - shift) * a.scale_log2), wv = exp2f((v.x - shift) * a.scale_log2);
+    float l = u.y * wu + v.y * wv;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    if (lane == 0 && a.stats) a.stats[row] = make_float2(shift * a.scale_log2, inv);
     const int g = rr / a.seq, t = rr - g * a.seq;
     T *out = static_cast<T *>(a.out) + (((size_t)b * a.seq + t) * a.kv_heads * a.group + hk * a.group + g) * a.dim;
-    for (int d = lane * 4; d < a.dim; d += 128) {
+    for (int d0 = 0; d0 < a.dim; d0 += 128) {
+        const int d = d0 + lane * 4;
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
         for (int s = 0; s < splits; ++s) {
-            const float w = exp2f((ml[s].x - shift) * a.scale_log2);
-            if (w == 0.0f) continue;
-            const float4 y = *reinterpret_cast<const float4 *>(a.part_o + ((size_t)row * splits + s) * a.dim + d);
-            x.x = fmaf(w, y.x, x.x), x.y = fmaf(w, y.y, x.y), x.z = fmaf(w, y.z, x.z), x.w = fmaf(w, y.w, x.w);
+            const float w = __shfl_sync(0xffffffffu, s < 32 ? wu : wv, s & 31);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (d < a.dim) y = *reinterpret_cast<const float4 *>(a.part_o + ((size_t)row * splits + s) * a.dim + d);
+            if (w != 0.0f) x.x = fmaf(w, y.x, x.x), x.y = fmaf(w, y.y, x.y), x.z = fmaf(w, y.z, x.z), x.w = fmaf(w, y.w, x.w);
         }
-        out[d] = from_f32<T>(x.x * inv), out[d + 1] = from_f32<T>(x.y * inv), out[d + 2] = from_f32<T>(x.z * inv), out[d + 3] = from_f32<T>(x.w * inv);
+        if (d < a.dim)
+            out[d] = from_f32<T>(x.x * inv), out[d + 1] = from_f32<T>(x.y * inv), out[d + 2] = from_f32<T>(x.z * inv), out[d + 3] = from_f32<T>(x.w * inv);
     }
 }
 
-// weights[j] += sum over all rows of p_j, p from the rows' final maximum and sum: a
-// block owns 32 keys of a (sequence, head), walks over the rows 16 at a time and
-// adds the 16 row slots in order. grid: (key tiles, batch * kv_heads)
+// weights[j] += sum over all rows of p_j, p from the rows' joined maximum and sum: a
+// block owns 32 keys of a (sequence, head), walks over the rows 16 at a time and adds
+// the 16 row slots in order.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) tree_weights_simt_kernel(const TreeArgs a) {
-    extern __shared__ float smem[];
+__device__ __forceinline__ void add_weights(const TreeArgs &a, int splits, int first_tile, int step, int bh, float *smem) {
     float *q = smem, *k = q + kRows * q_stride(a.dim), *sums = k + kKeys * q_stride(a.dim);
-    const int bh = blockIdx.y, b = bh / a.kv_heads, r = threadIdx.x >> 3, c = threadIdx.x & 7;
+    const int b = bh / a.kv_heads, r = threadIdx.x >> 3, c = threadIdx.x & 7;
     const int length = a.lengths[b], n = length + a.seq;
-    grid_dependency_wait();  // the rows' stats
     if (length < 0 || length > a.capacity - a.seq) return;
-    for (int j0 = blockIdx.x * kKeys; j0 < n; j0 += gridDim.x * kKeys) {
+    for (int j0 = first_tile * kKeys; j0 < n; j0 += step * kKeys) {
         float acc[4] = {};
         __syncthreads();
-        stage(k, static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, j0, kKeys, n, a.dim);
+        stage<T, kKeys>(k, static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, j0, n, a.dim);
         for (int r0 = 0; r0 < a.rows; r0 += kRows) {
             __syncthreads();
-            stage(q, static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, r0, kRows, a.rows, a.dim);
+            stage<T, kRows>(q, static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, r0, a.rows, a.dim);
+            // the row's maximum and sum over its splits, by its 8 threads
+            float m = -INFINITY, l = 0.0f;
+            if (r0 + r < a.rows) {
+                const float2 *ml = a.part_ml + ((size_t)bh * a.rows + r0 + r) * splits;
+                for (int s = c; s < splits; s += 8) m = fmaxf(m, ml[s].x);
+            }
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            const float shift = m == -INFINITY ? 0.0f : m;
+            if (r0 + r < a.rows) {
+                const float2 *ml = a.part_ml + ((size_t)bh * a.rows + r0 + r) * splits;
+                for (int s = c; s < splits; s += 8) l = fmaf(ml[s].y, exp2f((ml[s].x - shift) * a.scale_log2), l);
+            }
+#pragma unroll
+            for (int x = 1; x < 8; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
             __syncthreads();
             if (r0 + r >= a.rows) continue;
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
             float s[4];
             tile_scores(q, k, r, c, a.dim, s);
-            const float2 st = a.stats[(size_t)bh * a.rows + r0 + r];
 #pragma unroll
             for (int u = 0; u < 4; ++u)
-                if (sees(a, b, r0 + r, j0 + c + 8 * u, length)) acc[u] += exp2f(fmaf(s[u], a.scale_log2, -st.x)) * st.y;
+                if (sees(a, b, r0 + r, j0 + c + 8 * u, length)) acc[u] += exp2f((s[u] - shift) * a.scale_log2) * inv;
         }
         __syncthreads();
 #pragma unroll
@@ -219,6 +251,17 @@ __global__ void __launch_bounds__(kThreads) tree_weights_simt_kernel(const TreeA
     }
 }
 
+// Behind the splits: the first join_blocks blocks join rows, the others add weights
+// (which read the splits' maxima and sums themselves, so neither waits for the other).
+template <typename T>
+__global__ void __launch_bounds__(kThreads) tree_finish_kernel(const TreeArgs a, int splits, int total_rows, int join_blocks, int key_blocks) {
+    extern __shared__ float smem[];
+    grid_dependency_wait();
+    if ((int)blockIdx.x < join_blocks) return join_rows<T>(a, splits, total_rows, blockIdx.x);
+    const int i = blockIdx.x - join_blocks, bh = i / key_blocks;
+    add_weights<T>(a, splits, i - bh * key_blocks, key_blocks, bh, smem);
+}
+
 template <typename T>
 LaunchFn simt_launch(Context *ctx, const Spec &s) {
     TreeArgs base = tree_args(ctx, s);
@@ -226,24 +269,25 @@ LaunchFn simt_launch(Context *ctx, const Spec &s) {
     if (heads > 65535) throw IrError("attention_tree: batch * kv_heads must be at most 65535");
     // about four blocks per SM
     const long long items = (long long)heads * row_blocks;
-    const int splits = (int)std::max<long long>(1, std::min<long long>({(4ll * ctx->sm_count + items - 1) / items, ((long long)s.capacity + kKeys - 1) / kKeys, 64ll}));
-    const size_t stats = (size_t)total_rows * sizeof(float2), ml = stats * splits;
-    auto ws = kernel_workspace(stats + ml + (size_t)total_rows * splits * s.dim * 4, "attention_tree partial results");
-    base.stats = static_cast<float2 *>(ws.get());
-    base.part_ml = base.stats + total_rows;
-    base.part_o = reinterpret_cast<float *>(base.part_ml + (size_t)total_rows * splits);
+    const int splits = (int)std::max<long long>(1, std::min<long long>({(4ll * ctx->sm_count + items - 1) / items, ((long long)s.capacity + kKeys - 1) / kKeys, (long long)kMaxSplits}));
+    const size_t parts = (size_t)total_rows * splits;
+    auto ws = kernel_workspace(parts * (s.dim * sizeof(float) + sizeof(float2)), "attention_tree partial results");
+    base.part_o = static_cast<float *>(ws.get());  // rows of a multiple of 32 bytes: read as 16-byte vectors
+    base.part_ml = reinterpret_cast<float2 *>(base.part_o + parts * s.dim);
     const size_t row = (size_t)q_stride(s.dim) * 4;
-    const size_t smem = (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4, smem_w = (kRows + kKeys) * row + kRows * kKeys * 4;
-    if (cudaFuncSetAttribute(tree_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaFuncSetAttribute(tree_weights_simt_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_w) != cudaSuccess)
+    const size_t smem = (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4, smem_w = s.weights ? (kRows + kKeys) * row + kRows * kKeys * 4 : 0;
+    auto kernel = s.dim <= 64 ? tree_simt_kernel<T, 2> : s.dim <= 128 ? tree_simt_kernel<T, 4> : tree_simt_kernel<T, 8>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaFuncSetAttribute(tree_finish_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_w) != cudaSuccess)
         throw IrError("cannot reserve shared memory for attention_tree");
     const bool weights = s.weights;
     const int key_blocks = (int)std::min<long long>((s.capacity + kKeys - 1) / kKeys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
+    const int join_blocks = (total_rows + 3) / 4;
     return [=, keep = ws](cudaStream_t st, void **b) {
         const TreeArgs a = tree_bind(base, b, weights);
-        tree_simt_kernel<T><<<dim3(row_blocks, splits, heads), kThreads, smem, st>>>(a, splits);
-        cudaError_t e = launch_after(st, tree_join_kernel<T>, dim3((total_rows + 3) / 4), 128, 0, a, splits, total_rows);
-        if (weights && e == cudaSuccess) e = launch_after(st, tree_weights_simt_kernel<T>, dim3(key_blocks, heads), kThreads, smem_w, a);
+        kernel<<<dim3(row_blocks, splits, heads), kThreads, smem, st>>>(a, splits);
+        const cudaError_t e = launch_after(st, tree_finish_kernel<T>, dim3(join_blocks + (weights ? key_blocks * heads : 0)), kThreads, smem_w, a, splits,
+                                           total_rows, join_blocks, key_blocks);
         return e == cudaSuccess ? cudaGetLastError() : e;
     };
 }

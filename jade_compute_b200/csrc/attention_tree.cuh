@@ -14,7 +14,6 @@ struct TreeArgs {
     const uint32_t *tree;  // [batch, seq, words]
     void *out;
     float *weights;
-    float2 *stats;    // for the FFMA weights, per row of q: p_j = 2^(s_j scale_log2 - x) y
     float *row_exponents;  // for the tcgen05 weights (attention_tree_tc.cu)
     float2 *part_ml;  // per row and split: maximum and sum
     float *part_o;    // per row and split: dim unnormalised sums

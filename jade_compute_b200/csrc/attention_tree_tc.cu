@@ -41,10 +41,12 @@ namespace {
 
 constexpr int kThreads = 10 * 32, kTileKeys = 128, kTileRows = 128;
 constexpr float kRescaleThreshold = 8.0f;  // log2 units
-// An item's end in tiles (see "work ranges"): measured on B200 with 16 sequences of
-// 1,000 to 8,000 tokens, 128 items of 9 to 63 tiles: 73.8 us with 0, 67.3 with 2, 65.7
-// with 4, 64.6 with 6, 64.5 with 8
-constexpr int kBoundary = 6;
+// An item's end in tiles (see "work ranges"), more of them the more rows it writes.
+// Measured on B200, 4 rows, 128 items of 9 to 63 tiles: 73.8 us with 0, 67.3 with 2,
+// 65.7 with 4, 64.6 with 6, 64.5 with 8, 67.0 with 12; 128 rows, 32 items of 72 to 126
+// tiles: 60.3 us with 6, 56.8 with 10, 55.8 with 12, 55.4 with 16. Two row tiles
+// (twice the time per tile): 73.6 us with 6, 74.9 with 10.
+constexpr int boundary_tiles(int rows) { return rows > 128 ? 6 : 6 + rows / 20; }
 
 template <int DP, bool kTwoTiles>
 struct Layout {
@@ -946,7 +948,7 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
     // one CTA per SM, none for which even full caches have no tile
     const unsigned __int128 most = (unsigned __int128)heads * base.row_blocks * ((capacity + kTileKeys - 1) / kTileKeys);
     base.ctas = most < (unsigned __int128)ctx->sm_count ? (int)most : ctx->sm_count;
-    base.boundary = kBoundary;
+    base.boundary = boundary_tiles((int)rows);
     base.slot_rows = rows >= (uint64_t)kSlotRows ? kSlotRows : (int)((rows + 7) / 8 * 8);
     const int item_blocks = (base.slot_rows * (DP / 4) + kJoinThreads - 1) / kJoinThreads;
     const long long join_blocks = (long long)heads * base.row_blocks * item_blocks;

@@ -304,6 +304,7 @@ extern "C" int jr_execute(void *handle, const jr_job *jobs, size_t job_count, ui
                 raise(JR_EINVAL, "null buffer in job %zu", j);
         }
         Context &ctx = enter(handle);
+        ctx.timed = false;
         check_cuda(cudaEventRecord(ctx.start, ctx.stream), "record start event");
         for (uint64_t launch = 0, total = (uint64_t)repeats * job_count; launch < total; ++launch) {
             const jr_job &job = jobs[launch % job_count];
@@ -667,7 +668,7 @@ extern "C" int jr_execute2(void *handle, const jr_dispatch *jobs, size_t job_cou
     return jade::c_entry(err, cap, [&] {
         require(jobs && job_count && repeats && gpu_ms, "empty dispatch sequence or missing timing output");
         const bool graph = flags & JR_EXEC_GRAPH, lanes = flags & JR_EXEC_STREAMS;
-        if (flags & ~(JR_EXEC_GRAPH | JR_EXEC_STREAMS)) raise(JR_EINVAL, "unknown execution flags 0x%x", flags);
+        if (flags & ~(JR_EXEC_GRAPH | JR_EXEC_STREAMS | JR_EXEC_DEFER_MS)) raise(JR_EINVAL, "unknown execution flags 0x%x", flags);
         require(!(graph && job_ms), "per-job timing is not available with graph replay");
         require(!(graph && lanes), "graph replay and dependency-scheduled streams cannot be combined");
         auto *raw = static_cast<Context *>(handle);
@@ -688,6 +689,7 @@ extern "C" int jr_execute2(void *handle, const jr_dispatch *jobs, size_t job_cou
                 if (!*s) check_cuda(cudaStreamCreateWithFlags(s, cudaStreamNonBlocking), what);
             reserve_events(ctx.dep_events, launches, cudaEventDisableTiming, what);
         }
+        ctx.timed = false;
         CapturedPass pass;
         if (graph) pass.capture(ctx.stream, jobs, job_count);
         check_cuda(cudaEventRecord(ctx.start, ctx.stream), "record start event");
@@ -725,13 +727,24 @@ extern "C" int jr_execute2(void *handle, const jr_dispatch *jobs, size_t job_cou
         }
         await_event(ctx, ctx.stop, collective);
         raise_device_wait_error(ctx);
-        *gpu_ms = bracket_ms(ctx);
+        ctx.timed = true;
+        if (!(flags & JR_EXEC_DEFER_MS)) *gpu_ms = bracket_ms(ctx);
         if (job_ms)
             for (size_t launch = 0; launch < launches; ++launch) {
                 float t = 0;
                 cudaEventElapsedTime(&t, ctx.job_events[2 * launch], ctx.job_events[2 * launch + 1]);
                 job_ms[launch % job_count] += t;
             }
+    });
+}
+
+extern "C" int jr_batch_ms(void *handle, double *gpu_ms, char *err, size_t cap) {
+    if (gpu_ms) *gpu_ms = 0;
+    return jade::c_entry(err, cap, [&] {
+        require(gpu_ms != nullptr, "missing timing output");
+        Context &ctx = enter(handle);
+        require(ctx.timed, "no completed batch to time");
+        *gpu_ms = bracket_ms(ctx);
     });
 }
 

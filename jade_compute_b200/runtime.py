@@ -15,6 +15,7 @@ import ctypes
 import json
 import os
 import time
+import weakref
 from array import array
 from dataclasses import dataclass, field
 from typing import Iterable, Sequence
@@ -30,6 +31,7 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include", "jade_runtime.h")
 JR_OK, JR_EINVAL, JR_ECUDA, JR_ENOMEM, JR_ETIMEOUT = 0, 1, 2, 3, 4
 JR_EXEC_GRAPH = 1
 JR_EXEC_STREAMS = 2
+JR_EXEC_DEFER_MS = 4
 
 DTYPE_SIZE = {"fp32": 4, "tf32": 4, "bf16": 2, "fp16": 2, "u8": 1, "i32": 4}
 NP_DTYPE = {"fp32": np.float32, "tf32": np.float32, "bf16": np.uint16, "fp16": np.float16, "u8": np.uint8, "i32": np.int32}
@@ -85,6 +87,7 @@ def lib() -> ctypes.CDLL:
     L.jr_kernel_info.argtypes = [vp, c_char_p, sz, c_char_p, sz]
     L.jr_execute2.argtypes = [vp, vp, sz, u32, u32, ctypes.POINTER(ctypes.c_double),
                               ctypes.POINTER(ctypes.c_double), c_char_p, sz]
+    L.jr_batch_ms.argtypes = [vp, ctypes.POINTER(ctypes.c_double), c_char_p, sz]
     L.jr_buffer_bytes.argtypes = [vp, vp, ctypes.POINTER(sz)]
     L.jr_host_alloc.argtypes = [vp, sz, ctypes.POINTER(vp), c_char_p, sz]
     L.jr_host_free.argtypes = [vp, vp]
@@ -225,14 +228,21 @@ class Kernel:
             self.handle = 0
 
 
-@dataclass
 class Execution:
-    """src/runtime/mod.rs:23-30 plus per-job device times."""
-    host_ms: float
-    gpu_ms: float | None
-    dispatches: int
-    repeats: int
-    job_ms: list | None = None
+    """src/runtime/mod.rs:23-30 plus per-job device times. ``gpu_ms`` is read from the
+    device when it is asked for, or before the runtime's next batch at the latest."""
+    __slots__ = ("host_ms", "dispatches", "repeats", "job_ms", "_runtime", "_gpu_ms", "__weakref__")
+
+    def __init__(self, runtime: "Runtime", host_ms: float, dispatches: int, repeats: int, job_ms: list | None = None):
+        self.host_ms, self.dispatches, self.repeats, self.job_ms = host_ms, dispatches, repeats, job_ms
+        self._runtime, self._gpu_ms = runtime, None
+
+    @property
+    def gpu_ms(self) -> float | None:
+        if self._runtime is not None:
+            self._gpu_ms = self._runtime._batch_ms()
+            self._runtime = None
+        return self._gpu_ms
 
 
 class _Dispatch(ctypes.Structure):
@@ -257,10 +267,15 @@ class Runtime:
         self.device_info = out.value.decode()
         self._kernels: list[Kernel] = []
         self._message = _err()  # of execute (a context is used serially)
+        self._last = None  # weak reference to the last batch's Execution
 
     # -- lifetime
     def close(self) -> None:
         if self.ctx:
+            try:
+                self._settle()
+            except JadeError:
+                pass  # a context that has failed has no time to give
             for k in self._kernels:
                 k.release()
             lib().jr_destroy(self.ctx)
@@ -373,14 +388,28 @@ class Runtime:
         e = self._message
         gpu = ctypes.c_double(0)
         jm = (ctypes.c_double * len(jobs))() if per_job else None
-        flags = (JR_EXEC_GRAPH if graph else 0) | (JR_EXEC_STREAMS if streams else 0)
+        flags = (JR_EXEC_GRAPH if graph else 0) | (JR_EXEC_STREAMS if streams else 0) | JR_EXEC_DEFER_MS
+        self._settle()
         t0 = time.perf_counter()
         rc = lib().jr_execute2(self.ctx, words.buffer_info()[0], len(jobs), repeats, flags, ctypes.byref(gpu), jm, e, len(e))
         host_ms = (time.perf_counter() - t0) * 1e3
         if rc != JR_OK:
             _check(rc, e)
-        return Execution(host_ms, gpu.value if gpu.value > 0 else None, len(jobs) * repeats, repeats,
-                         list(jm) if per_job else None)
+        done = Execution(self, host_ms, len(jobs) * repeats, repeats, list(jm) if per_job else None)
+        self._last = weakref.ref(done)
+        return done
+
+    def _batch_ms(self) -> float | None:
+        e, ms = _err(), ctypes.c_double(0)
+        _check(lib().jr_batch_ms(self.ctx, ctypes.byref(ms), e, len(e)), e)
+        return ms.value if ms.value > 0 else None
+
+    def _settle(self) -> None:
+        """Reads the last batch's time if its Execution is still held."""
+        held = self._last and self._last()
+        self._last = None
+        if held:
+            held.gpu_ms
 
     # -- conveniences used by tests and benches
     def fill(self, buf: Buffer, dist: str, seed: int, stream: int = 0, lo: float = 0.0, hi: float = 1.0,

@@ -520,3 +520,19 @@ def test_commit_refuses_a_path_that_is_none(rt, path, count):
     with pytest.raises(JadeError, match="path must ascend") as e:
         R.run(rt, spec, x)
     assert e.value.code == 1
+
+
+# ------------------------------------------------------------------ batch times read on request
+def test_batch_times_outlive_the_next_batch_and_the_runtime():
+    r = jc.Runtime(0)
+    k = r.compile({"op": "l2_flush", "bytes": 1 << 28})
+    b = r.alloc_bytes(1 << 28)
+    try:
+        r.execute([(k, [b])])  # nobody holds this one
+        first = r.execute([(k, [b])], repeats=20)
+        second = r.execute([(k, [b])])
+        third = r.execute([(k, [b])], repeats=20)
+    finally:
+        r.close()
+    assert second.gpu_ms > 0 and first.gpu_ms > 5 * second.gpu_ms and third.gpu_ms > 5 * second.gpu_ms
+    assert first.gpu_ms == first.gpu_ms
