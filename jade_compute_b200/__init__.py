@@ -2,7 +2,8 @@
 KernelSpec -> compile -> ordered-batch execute hot path.
 
 The product is the C-ABI library ``lib/libjade_runtime.so`` (declared in
-``include/jade_runtime.h``); this package is its Python host mirror.
+``include/jade_runtime.h``); this package is its Python host mirror. ``mlp`` and
+``cached_attention`` are blocks built on it.
 """
 from .runtime import (Buffer, Execution, JadeError, Kernel, Runtime, bf16_to_f32, canonical, comm_init_all,
                       comm_unique_id, device_count, emit, f32_to_bf16, lib, library_path, spec_bindings, spec_launch,
