@@ -20,6 +20,7 @@
 // attention_tree_tc.cu: 16-bit types with dim up to 128, on tcgen05.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "attention_tree.cuh"
 
@@ -165,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, i
 // Joins the splits of one row: one warp a row.
 template <typename T>
 __device__ __forceinline__ void join_rows(const TreeArgs &a, int splits, int total_rows, int block) {
-    const int row = block * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int row = block * (int)(blockDim.x >> 5) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= total_rows) return;
     const int bh = row / a.rows, rr = row - bh * a.rows, b = bh / a.kv_heads, hk = bh - b * a.kv_heads;
     if (a.lengths[b] < 0 || a.lengths[b] > a.capacity - a.seq) return;
@@ -262,32 +263,269 @@ __global__ void __launch_bounds__(kThreads) tree_finish_kernel(const TreeArgs a,
     add_weights<T>(a, splits, i - bh * key_blocks, key_blocks, bh, smem);
 }
 
+// ------------------------------------------------------------------ many rows
+// From kWideRows rows on: 64 rows by 64 keys a block of 256 threads, 4 x 4 scores and 4
+// rows by kCols x 4 columns of the sums a thread, so that a 16-byte shared-memory read
+// feeds 8 to 11 FFMAs (the 16-row blocks: 3). K and V share a buffer; V is loaded into
+// registers while the scores are formed, the next K while the sums are. Bound by FFMA
+// issue beside shared-memory reads: 2 sequences, 512 rows of 128, 8 heads of 1,000 to
+// 4,000 keys in FP32: see the measured table of the launch rule below.
+constexpr int kWideThreads = 256, kWideTile = 64, kWideRows = 48;
+
+template <typename T, int kCols>  // kCols: 64-element columns of a head
+struct WideStage {  // a tile of rows on its way to shared memory: 8 threads a row, 32 rows at a time
+    float4 x[2][2 * kCols];
+    __device__ __forceinline__ void load(const T *src, int first, int limit, int dim) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = first + (threadIdx.x >> 3) + 32 * i;
+#pragma unroll
+            for (int u = 0; u < 2 * kCols; ++u) {
+                const int c = (threadIdx.x & 7) * 4 + 32 * u;
+                x[i][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (r < limit && c < dim) x[i][u] = load4(src + (size_t)r * dim + c);
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float *dst, int dim) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int u = 0; u < 2 * kCols; ++u) {
+                const int c = (threadIdx.x & 7) * 4 + 32 * u;
+                if (c < dim) *reinterpret_cast<float4 *>(dst + ((threadIdx.x >> 3) + 32 * i) * q_stride(dim) + c) = x[i][u];
+            }
+    }
+};
+
+// s[i][u]: row 4 ty + i with key tx + 16 u.
+__device__ __forceinline__ void wide_scores(const float *q, const float *k, int dim, float (&s)[4][4]) {
+    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) s[i][u] = 0.0f;
+#pragma unroll 2
+    for (int d = 0; d < dim; d += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(q + (4 * ty + i) * q_stride(dim) + d);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) y[u] = *reinterpret_cast<const float4 *>(k + (tx + 16 * u) * q_stride(dim) + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) s[i][u] = fmaf(x[i].x, y[u].x, fmaf(x[i].y, y[u].y, fmaf(x[i].z, y[u].z, fmaf(x[i].w, y[u].w, s[i][u]))));
+    }
+}
+
+constexpr int kWideP = kWideTile + 4;  // floats of a row of weights
+
+// grid: (row blocks, splits, batch * kv_heads)
+template <typename T, int kCols>
+__global__ void __launch_bounds__(kWideThreads, kCols == 4 ? 1 : 2) tree_wide_kernel(const TreeArgs a, int splits) {
+    extern __shared__ float smem[];
+    float *q = smem, *kv = q + kWideTile * q_stride(a.dim), *p = kv + kWideTile * q_stride(a.dim);
+    const int bh = blockIdx.z, b = bh / a.kv_heads, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, row0 = blockIdx.x * kWideTile + 4 * ty;
+    const int length = a.lengths[b];
+    if (length < 0 || length > a.capacity - a.seq) {
+        if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrCacheLength);
+        return;
+    }
+    grid_dependency_trigger();
+    const int n = length + a.seq, tiles = (n + kWideTile - 1) / kWideTile;
+    const int t0 = (int)((long long)tiles * blockIdx.y / splits), t1 = (int)((long long)tiles * (blockIdx.y + 1) / splits);
+    const T *k = static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, *v = static_cast<const T *>(a.v) + (size_t)bh * a.capacity * a.dim;
+    WideStage<T, kCols> stage;
+    stage.load(static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, blockIdx.x * kWideTile, a.rows, a.dim);
+    stage.store(q, a.dim);
+    if (t0 < t1) stage.load(k, t0 * kWideTile, n, a.dim);
+    float m[4], l[4];
+    float4 o[4][kCols];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        m[i] = -INFINITY, l[i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int j0 = t * kWideTile;
+        __syncthreads();
+        stage.store(kv, a.dim);
+        stage.load(v, j0, n, a.dim);
+        __syncthreads();
+        float s[4][4];
+        wide_scores(q, kv, a.dim, s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float top = -INFINITY;
+            if (j0 + kWideTile > length)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s[i][u] = sees(a, b, row0 + i, j0 + tx + 16 * u, length) ? s[i][u] : -INFINITY;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) top = fmaxf(top, s[i][u]);
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+            const float m_new = fmaxf(m[i], top), shift = m_new == -INFINITY ? 0.0f : m_new;
+            const float alpha = exp2f((m[i] - shift) * a.scale_log2);
+            m[i] = m_new;
+            float sum = 0.0f;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float e = exp2f((s[i][u] - shift) * a.scale_log2);
+                p[(4 * ty + i) * kWideP + tx + 16 * u] = e;
+                sum += e;
+            }
+            l[i] = l[i] * alpha + sum;  // this thread's keys
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) o[i][c].x *= alpha, o[i][c].y *= alpha, o[i][c].z *= alpha, o[i][c].w *= alpha;
+        }
+        __syncthreads();  // K has been read, P is written
+        stage.store(kv, a.dim);
+        if (t + 1 < t1) stage.load(k, j0 + kWideTile, n, a.dim);
+        __syncthreads();
+        auto add = [&](auto careful) {
+#pragma unroll 1
+            for (int j = 0; j < kWideTile; j += 4) {
+                float w[4][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) *reinterpret_cast<float4 *>(w[i]) = *reinterpret_cast<const float4 *>(p + (4 * ty + i) * kWideP + j);
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj)
+#pragma unroll
+                    for (int c = 0; c < kCols; ++c)
+                        if (tx * 4 + 64 * c < a.dim) {
+                            const float4 x = *reinterpret_cast<const float4 *>(kv + (j + jj) * q_stride(a.dim) + tx * 4 + 64 * c);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if (!careful || w[i][jj] != 0.0f) {
+                                    o[i][c].x = fmaf(w[i][jj], x.x, o[i][c].x), o[i][c].y = fmaf(w[i][jj], x.y, o[i][c].y);
+                                    o[i][c].z = fmaf(w[i][jj], x.z, o[i][c].z), o[i][c].w = fmaf(w[i][jj], x.w, o[i][c].w);
+                                }
+                        }
+            }
+        };
+        if (j0 + kWideTile <= length) add(std::false_type{});
+        else add(std::true_type{});  // drafts: no product with one that the row does not see
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
+        if (row0 + i >= a.rows) continue;
+        const size_t at = ((size_t)bh * a.rows + row0 + i) * splits + blockIdx.y;
+        if (tx == 0) a.part_ml[at] = make_float2(m[i], l[i]);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c)
+            if (tx * 4 + 64 * c < a.dim) *reinterpret_cast<float4 *>(a.part_o + at * a.dim + tx * 4 + 64 * c) = o[i][c];
+    }
+}
+
+// add_weights for many rows: 64 keys a block, 64 rows at a time.
+template <typename T, int kCols>
+__device__ __forceinline__ void add_weights_wide(const TreeArgs &a, int splits, int first_tile, int step, int bh, float *smem) {
+    float *q = smem, *k = q + kWideTile * q_stride(a.dim), *sums = k + kWideTile * q_stride(a.dim);
+    float2 *stats = reinterpret_cast<float2 *>(sums + 16 * kWideTile);
+    const int b = bh / a.kv_heads, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
+    const int length = a.lengths[b], n = length + a.seq;
+    if (length < 0 || length > a.capacity - a.seq) return;
+    for (int j0 = first_tile * kWideTile; j0 < n; j0 += step * kWideTile) {
+        float acc[4] = {};
+        WideStage<T, kCols> stage;
+        stage.load(static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, j0, n, a.dim);
+        __syncthreads();
+        stage.store(k, a.dim);
+        for (int r0 = 0; r0 < a.rows; r0 += kWideTile) {
+            stage.load(static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, r0, a.rows, a.dim);
+            __syncthreads();
+            stage.store(q, a.dim);
+            {  // a row's maximum and 1 / sum over its splits, by four threads
+                const int row = r0 + (threadIdx.x >> 2), part = threadIdx.x & 3;
+                const float2 *ml = a.part_ml + ((size_t)bh * a.rows + min(row, a.rows - 1)) * splits;
+                float m = -INFINITY, l = 0.0f;
+                for (int s = part; s < splits; s += 4) m = fmaxf(m, ml[s].x);
+#pragma unroll
+                for (int x = 1; x < 4; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+                const float shift = m == -INFINITY ? 0.0f : m;
+                for (int s = part; s < splits; s += 4) l = fmaf(ml[s].y, exp2f((ml[s].x - shift) * a.scale_log2), l);
+#pragma unroll
+                for (int x = 1; x < 4; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+                if (part == 0) stats[threadIdx.x >> 2] = make_float2(shift, row < a.rows && (l > 0.0f || l != l) ? 1.0f / l : 0.0f);
+            }
+            __syncthreads();
+            float s[4][4];
+            wide_scores(q, k, a.dim, s);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = r0 + 4 * ty + i;
+                const float2 st = stats[4 * ty + i];
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (row < a.rows && sees(a, b, row, j0 + tx + 16 * u, length)) acc[u] += exp2f((s[i][u] - st.x) * a.scale_log2) * st.y;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) sums[ty * kWideTile + tx + 16 * u] = acc[u];
+        __syncthreads();
+        if (threadIdx.x < kWideTile && j0 + threadIdx.x < n) {
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s += sums[i * kWideTile + threadIdx.x];
+            a.weights[(size_t)bh * a.capacity + j0 + threadIdx.x] += s;
+        }
+    }
+}
+
+template <typename T, int kCols>
+__global__ void __launch_bounds__(kWideThreads, kCols == 4 ? 1 : 2)
+    tree_finish_wide_kernel(const TreeArgs a, int splits, int total_rows, int join_blocks, int key_blocks) {
+    extern __shared__ float smem[];
+    grid_dependency_wait();
+    if ((int)blockIdx.x < join_blocks) return join_rows<T>(a, splits, total_rows, blockIdx.x);
+    const int i = blockIdx.x - join_blocks, bh = i / key_blocks;
+    add_weights_wide<T, kCols>(a, splits, i - bh * key_blocks, key_blocks, bh, smem);
+}
+
 template <typename T>
 LaunchFn simt_launch(Context *ctx, const Spec &s) {
     TreeArgs base = tree_args(ctx, s);
-    const int heads = (int)(s.batch * s.kv_heads), rows = base.rows, row_blocks = (rows + kRows - 1) / kRows, total_rows = heads * rows;
+    const int heads = (int)(s.batch * s.kv_heads), rows = base.rows, total_rows = heads * rows;
     if (heads > 65535) throw IrError("attention_tree: batch * kv_heads must be at most 65535");
+    const bool wide = rows >= kWideRows;
+    const int tile_rows = wide ? kWideTile : kRows, tile_keys = wide ? kWideTile : kKeys, threads = wide ? kWideThreads : kThreads;
+    const int row_blocks = (rows + tile_rows - 1) / tile_rows;
     // about four blocks per SM
     const long long items = (long long)heads * row_blocks;
-    const int splits = (int)std::max<long long>(1, std::min<long long>({(4ll * ctx->sm_count + items - 1) / items, ((long long)s.capacity + kKeys - 1) / kKeys, (long long)kMaxSplits}));
+    const int splits = (int)std::max<long long>(1, std::min<long long>({(4ll * ctx->sm_count + items - 1) / items, ((long long)s.capacity + tile_keys - 1) / tile_keys,
+                                                                        (long long)kMaxSplits}));
     const size_t parts = (size_t)total_rows * splits;
     auto ws = kernel_workspace(parts * (s.dim * sizeof(float) + sizeof(float2)), "attention_tree partial results");
     base.part_o = static_cast<float *>(ws.get());  // rows of a multiple of 32 bytes: read as 16-byte vectors
     base.part_ml = reinterpret_cast<float2 *>(base.part_o + parts * s.dim);
     const size_t row = (size_t)q_stride(s.dim) * 4;
-    const size_t smem = (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4, smem_w = s.weights ? (kRows + kKeys) * row + kRows * kKeys * 4 : 0;
-    auto kernel = s.dim <= 64 ? tree_simt_kernel<T, 2> : s.dim <= 128 ? tree_simt_kernel<T, 4> : tree_simt_kernel<T, 8>;
+    const size_t smem = wide ? 2 * kWideTile * row + kWideTile * kWideP * 4 : (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4;
+    const size_t smem_w = !s.weights ? 0 : wide ? 2 * kWideTile * row + 16 * kWideTile * 4 + kWideTile * 8 : (kRows + kKeys) * row + kRows * kKeys * 4;
+    void (*kernel)(TreeArgs, int);
+    void (*finish)(TreeArgs, int, int, int, int);
+    if (wide) {
+        kernel = s.dim <= 64 ? tree_wide_kernel<T, 1> : s.dim <= 128 ? tree_wide_kernel<T, 2> : tree_wide_kernel<T, 4>;
+        finish = s.dim <= 64 ? tree_finish_wide_kernel<T, 1> : s.dim <= 128 ? tree_finish_wide_kernel<T, 2> : tree_finish_wide_kernel<T, 4>;
+    } else {
+        kernel = s.dim <= 64 ? tree_simt_kernel<T, 2> : s.dim <= 128 ? tree_simt_kernel<T, 4> : tree_simt_kernel<T, 8>;
+        finish = tree_finish_kernel<T>;
+    }
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaFuncSetAttribute(tree_finish_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_w) != cudaSuccess)
+        cudaFuncSetAttribute(finish, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_w) != cudaSuccess)
         throw IrError("cannot reserve shared memory for attention_tree");
     const bool weights = s.weights;
-    const int key_blocks = (int)std::min<long long>((s.capacity + kKeys - 1) / kKeys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
-    const int join_blocks = (total_rows + 3) / 4;
+    const int key_blocks = (int)std::min<long long>((s.capacity + tile_keys - 1) / tile_keys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
+    const int join_blocks = (total_rows + threads / 32 - 1) / (threads / 32);
     return [=, keep = ws](cudaStream_t st, void **b) {
         const TreeArgs a = tree_bind(base, b, weights);
-        kernel<<<dim3(row_blocks, splits, heads), kThreads, smem, st>>>(a, splits);
-        const cudaError_t e = launch_after(st, tree_finish_kernel<T>, dim3(join_blocks + (weights ? key_blocks * heads : 0)), kThreads, smem_w, a, splits,
-                                           total_rows, join_blocks, key_blocks);
+        kernel<<<dim3(row_blocks, splits, heads), threads, smem, st>>>(a, splits);
+        const cudaError_t e = launch_after(st, finish, dim3(join_blocks + (weights ? key_blocks * heads : 0)), threads, smem_w, a, splits, total_rows,
+                                           join_blocks, key_blocks);
         return e == cudaSuccess ? cudaGetLastError() : e;
     };
 }
