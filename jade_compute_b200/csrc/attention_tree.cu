@@ -264,13 +264,14 @@ __global__ void __launch_bounds__(kThreads) tree_finish_kernel(const TreeArgs a,
 }
 
 // ------------------------------------------------------------------ many rows
-// From kWideRows rows on: 64 rows by 64 keys a block of 256 threads, 4 x 4 scores and 4
-// rows by kCols x 4 columns of the sums a thread, so that a 16-byte shared-memory read
-// feeds 8 to 11 FFMAs (the 16-row blocks: 3). K and V share a buffer; V is loaded into
-// registers while the scores are formed, the next K while the sums are. Bound by FFMA
-// issue beside shared-memory reads: 2 sequences, 512 rows of 128, 8 heads of 1,000 to
-// 4,000 keys in FP32: see the measured table of the launch rule below.
-constexpr int kWideThreads = 256, kWideTile = 64, kWideRows = 48;
+// From kWideRows rows on (FP32, 32 sequences and heads of 1,000 to 4,000 keys of 128: 144 us
+// here and 202 on 16-row blocks at 48 rows, 146 and 283 at 64, equal up to 32): 64 rows
+// by 64 keys a block of 256 threads, 4 x 4 scores and 4 rows by kCols x 4 columns of the
+// sums a thread, so that a 16-byte shared-memory read feeds 8 to 11 FFMAs (the 16-row
+// blocks: 3). K and V share a buffer; V is loaded into registers while the scores are
+// formed, the next K while the sums are. Bound by FFMA issue beside shared-memory reads:
+// 512 rows of 128 in FP32 run at about 20 TFLOP/s.
+constexpr int kWideThreads = 256, kWideTile = 64, kWideRows = 33;
 
 template <typename T, int kCols>  // kCols: 64-element columns of a head
 struct WideStage {  // a tile of rows on its way to shared memory: 8 threads a row, 32 rows at a time

@@ -11,6 +11,8 @@
 // cache_commit: after attention_tree over seq drafted tokens in slots length ..,
 // moves the accepted ones, path[0 .. count) ascending, to slots length + 0, 1, ...
 // in place; their accumulated weights too, the rest of the drafts' weights to 0.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <climits>
 
@@ -19,6 +21,8 @@
 
 namespace jade {
 namespace {
+
+namespace cg = cooperative_groups;
 
 // ------------------------------------------------------------------ cache_evict
 struct EvictArgs {
@@ -63,74 +67,110 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *warp_sums
     return __shfl_sync(0xffffffffu, upto - w, warp) + sum - v;
 }
 
-// One block per (sequence, head). The need-th largest key among the entries that may
-// go is found digit by digit from the top (11, 11, 10 bits: with 8-bit digits the
-// first holds little but the exponent, and its few bins serialise the counting), then
-// the kept slots are written in order: 8 neighbouring entries a thread, one prefix sum
-// over the block for entries above the threshold and entries equal to it together.
-// Weights come from memory once where a sequence has at most kSelectTile entries
+// A cluster of blocks per (sequence, head), each with a run of its entries. The
+// need-th largest key among the entries that may go is found digit by digit from the
+// top (11, 11, 10 bits: with 8-bit digits the first holds little but the exponent, and
+// its few bins serialise the counting): every block counts its run in shared memory and
+// adds up the counts of all blocks, two bins a thread. Then the kept slots are written
+// in order: 8 neighbouring entries a thread, one prefix sum over the block for entries
+// above the threshold and entries equal to it together, behind the earlier blocks'
+// totals. Weights come from memory once where a run has at most kSelectTile entries
 // (their keys stay in shared memory), else once per pass.
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
-    __shared__ uint32_t keys[kSelectTile + kSelectTile / 32], hist[kBins], warp_sums[32], chosen[2];
-    const int bh = blockIdx.x, b = bh / a.kv_heads, n = a.lengths[b], thread = threadIdx.x;
+    __shared__ uint32_t keys[kSelectTile + kSelectTile / 32], hist[kBins], warp_sums[32], chosen[2], totals[2];
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int bh = blockIdx.x / blocks, b = bh / a.kv_heads, n = a.lengths[b], thread = threadIdx.x;
     grid_dependency_trigger();
-    if (n < 0 || n > a.capacity) {
+    if (n < 0 || n > a.capacity) {  // the same for the whole cluster
         if (thread == 0) atomicCAS(a.err, 0, kErrCacheLength);
         return;
     }
+    auto sync = [&] {  // all blocks of the cluster
+        if (blocks > 1) cluster.sync();
+        else __syncthreads();
+    };
     int *kept = a.kept + (size_t)bh * a.keep;
     const float *w = a.weights + (size_t)bh * a.capacity;
     float *w_out = a.weights_out + (size_t)bh * a.capacity;
     const int count = min(n, a.keep), last = max(0, n - a.recent);
+    const int run = (n + blocks - 1) / blocks, lo = min(n, rank * run), hi = min(n, lo + run);
     uint32_t need = count - (n - last);  // of the first `last` entries
-    const bool all = need >= (uint32_t)last, single = n <= kSelectTile;
+    const bool all = need >= (uint32_t)last, single = run <= kSelectTile;
     auto at = [](int j) { return j + (j >> 5); };  // a thread's run of 8 without bank conflicts
     auto load_tile = [&](int j0) {
 #pragma unroll
         for (int u = 0; u < kSelectEach; ++u) {
             const int j = u * kSelectThreads + thread;
-            if (j0 + j < n) keys[at(j)] = weight_key(w[j0 + j]);
+            if (j0 + j < hi) keys[at(j)] = weight_key(w[j0 + j]);
         }
     };
     uint32_t threshold = 0;
-    if (single) load_tile(0);
+    if (single) load_tile(lo);
     for (int pass = 0; pass < 3 && !all && need > 0; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, digit = pass < 2 ? 11 : 10;
         for (int i = thread; i < kBins; i += kSelectThreads) hist[i] = 0;
         __syncthreads();
-        for (int j = thread; j < last; j += kSelectThreads) {
-            const uint32_t key = single ? keys[at(j)] : weight_key(w[j]);
+        for (int j = lo + thread; j < min(hi, last); j += kSelectThreads) {
+            const uint32_t key = single ? keys[at(j - lo)] : weight_key(w[j]);
             if (pass == 0 || key >> (shift + digit) == threshold) atomicAdd(&hist[key >> shift & ((1u << digit) - 1)], 1u);
         }
-        __syncthreads();
+        sync();
         const int high = kBins - 1 - 2 * thread;  // two bins a thread, the largest first
-        const uint32_t c0 = hist[high], c1 = hist[high - 1];
+        uint32_t c0 = 0, c1 = 0;
+#pragma unroll 8
+        for (int r = 0; r < blocks; ++r) {
+            const uint2 c = *reinterpret_cast<const uint2 *>((blocks > 1 ? cluster.map_shared_rank(hist, r) : hist) + high - 1);
+            c0 += c.y, c1 += c.x;
+        }
         uint32_t total;
         const uint32_t above = block_prefix(c0 + c1, warp_sums, total);
         if (above < need && need <= above + c0) chosen[0] = high, chosen[1] = need - above;
         else if (above + c0 < need && need <= above + c0 + c1) chosen[0] = high - 1, chosen[1] = need - above - c0;
-        __syncthreads();
+        sync();  // and no block clears counts that another still reads
         threshold = threshold << digit | chosen[0];
         need = chosen[1];
     }
     // threshold: the smallest kept key; need: how many entries with exactly it are kept, the lowest slots
-    uint32_t takes = 0, ties = 0;
-    for (int j0 = 0; j0 < n; j0 += kSelectTile) {
-        __syncthreads();
-        if (!single) {
-            load_tile(j0);
-            __syncthreads();
-        }
-        uint32_t mask = 0, equal = 0;
+    auto sort_out = [&](int j0, uint32_t &mask, uint32_t &equal) {  // of the thread's 8 entries of the tile
+        mask = equal = 0;
 #pragma unroll
         for (int i = 0; i < kSelectEach; ++i) {
             const int j = j0 + thread * kSelectEach + i;
-            if (j >= n) break;
+            if (j >= hi) break;
             const uint32_t key = keys[at(thread * kSelectEach + i)];
             if (all || j >= last || (need > 0 && key > threshold)) mask |= 1u << i;
             else if (need > 0 && key == threshold) equal |= 1u << i;
         }
-        uint32_t total;
+    };
+    uint32_t takes = 0, ties = 0, mask, equal, total;
+    if (blocks > 1) {
+        for (int j0 = lo; j0 < hi; j0 += kSelectTile) {
+            if (!single) {
+                __syncthreads();
+                load_tile(j0);
+            }
+            __syncthreads();
+            sort_out(j0, mask, equal);
+            block_prefix(__popc(mask) | __popc(equal) << 16, warp_sums, total);
+            takes += total & 0xffffu, ties += total >> 16;
+        }
+        if (thread == 0) totals[0] = takes, totals[1] = ties;
+        sync();
+        takes = ties = 0;
+        for (int r = 0; r < rank; ++r) {
+            const uint32_t *t = cluster.map_shared_rank(totals, r);
+            takes += t[0], ties += t[1];
+        }
+        sync();  // no block leaves while another reads its totals
+    }
+    for (int j0 = lo; j0 < hi; j0 += kSelectTile) {
+        if (!single) {
+            __syncthreads();
+            load_tile(j0);
+        }
+        __syncthreads();
+        sort_out(j0, mask, equal);
         const uint32_t before = block_prefix(__popc(mask) | __popc(equal) << 16, warp_sums, total);
         uint32_t take = takes + (before & 0xffffu), tie = ties + (before >> 16);
 #pragma unroll
@@ -147,9 +187,10 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         }
         takes += total & 0xffffu, ties += total >> 16;
     }
-    for (int i = count + thread; i < a.keep; i += kSelectThreads) kept[i] = -1;
-    for (int i = count + thread; i < a.capacity; i += kSelectThreads) w_out[i] = 0.0f;
-    if (bh % a.kv_heads == 0 && thread == 0) a.lengths_out[b] = count;
+    const int first = rank * kSelectThreads + thread, step = blocks * kSelectThreads;
+    for (int i = count + first; i < a.keep; i += step) kept[i] = -1;
+    for (int i = count + first; i < a.capacity; i += step) w_out[i] = 0.0f;
+    if (bh % a.kv_heads == 0 && first == 0) a.lengths_out[b] = count;
 }
 
 __global__ void __launch_bounds__(256) evict_move_kernel(const EvictArgs a) {
@@ -246,13 +287,24 @@ LaunchFn make_cache_op(Context *ctx, const Spec &s, std::string &impl) {
     base.kv_heads = s.kv_heads, base.capacity = s.capacity, base.keep = s.keep, base.recent = s.recent, base.vecs = vecs;
     base.err = ctx->err_dev;
     const int blocks = (int)std::min<long long>(((long long)s.keep * vecs + 1023) / 1024, std::max(1, 16 * ctx->sm_count / heads));
+    // Blocks per (sequence, head), up to 8: more while a block would have more than one
+    // tile and there are SMs. A cluster's barriers and counts from the other blocks cost
+    // about what a second tile does: 64 heads of 8192 entries take 37 us with one block
+    // each and 39 with two; 8 of 60,000 took 171 us with one, 89 with eight.
+    int cluster = 1;
+    while (cluster < 8 && heads * cluster * 2 <= ctx->sm_count && s.capacity > (uint32_t)(kSelectTile * cluster)) cluster *= 2;
     return [=](cudaStream_t st, void **b) {
         EvictArgs a = base;
         a.k = static_cast<const uint4 *>(b[0]), a.v = static_cast<const uint4 *>(b[1]), a.weights = static_cast<const float *>(b[2]);
         a.lengths = static_cast<const int *>(b[3]), a.k_out = static_cast<uint4 *>(b[4]), a.v_out = static_cast<uint4 *>(b[5]);
         a.weights_out = static_cast<float *>(b[6]), a.kept = static_cast<int *>(b[7]), a.lengths_out = static_cast<int *>(b[8]);
-        evict_select_kernel<<<heads, kSelectThreads, 0, st>>>(a);
-        const cudaError_t e = launch_after(st, evict_move_kernel, dim3(blocks, heads), 256, 0, a);
+        cudaLaunchAttribute shape{};
+        shape.id = cudaLaunchAttributeClusterDimension;
+        shape.val.clusterDim.x = cluster, shape.val.clusterDim.y = shape.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(heads * cluster), config.blockDim = dim3(kSelectThreads), config.stream = st, config.attrs = &shape, config.numAttrs = cluster > 1;
+        cudaError_t e = cudaLaunchKernelEx(&config, evict_select_kernel, a);
+        if (e == cudaSuccess) e = launch_after(st, evict_move_kernel, dim3(blocks, heads), 256, 0, a);
         return e == cudaSuccess ? cudaGetLastError() : e;
     };
 }
