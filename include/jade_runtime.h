@@ -120,8 +120,8 @@ typedef struct jr_dispatch {
  * No counterpart in the reference (its execute is strictly in order). */
 #define JR_EXEC_STREAMS 2u
 /* The batch's event time is not read back: *gpu_ms stays 0 and jr_batch_ms returns
- * it on request (reading the events costs about 3 us of host time per batch on a
- * B200 host, which callers of short batches need not pay). */
+ * it on request (waiting for a timed event and reading it costs about 7 us per batch
+ * on a B200 host, which callers of short batches need not pay). */
 #define JR_EXEC_DEFER_MS 4u
 
 /* Validates every job (context ownership, registered buffers, exact byte sizes,

@@ -26,7 +26,8 @@ struct Context {
     int sm_count = 148;
     cudaStream_t stream = nullptr;
     cudaEvent_t start = nullptr, stop = nullptr;
-    bool timed = false;  // start and stop bracket a completed batch
+    cudaEvent_t done = nullptr;  // end of a batch whose time is read later (untimed)
+    bool timed = false;          // start and stop bracket a batch that has ended
     std::map<uintptr_t, Allocation> allocations;
     int *err_host = nullptr;  // mapped, written by kernels (first error wins)
     int *err_dev = nullptr;

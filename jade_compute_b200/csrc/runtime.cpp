@@ -95,7 +95,7 @@ void teardown(Context *ctx) {
     ctx->allocations.clear();
     for (cudaEvent_t e : ctx->job_events) cudaEventDestroy(e);
     for (cudaEvent_t e : ctx->dep_events) cudaEventDestroy(e);
-    for (cudaEvent_t e : {ctx->start, ctx->stop})
+    for (cudaEvent_t e : {ctx->start, ctx->stop, ctx->done})
         if (e) cudaEventDestroy(e);
     for (cudaStream_t s : {ctx->copy_in, ctx->copy_out, ctx->collective, ctx->stream})
         if (s) cudaStreamDestroy(s);
@@ -113,6 +113,7 @@ Context *build_context(int device) {
     cudaError_t st = cudaStreamCreateWithFlags(&ctx->stream, cudaStreamNonBlocking);
     for (cudaEvent_t *e : {&ctx->start, &ctx->stop})
         if (st == cudaSuccess) st = cudaEventCreate(e);
+    if (st == cudaSuccess) st = cudaEventCreateWithFlags(&ctx->done, cudaEventDisableTiming);
     if (st == cudaSuccess) st = cudaHostAlloc(reinterpret_cast<void **>(&ctx->err_host), 64, cudaHostAllocMapped);
     if (st == cudaSuccess) st = cudaHostGetDevicePointer(reinterpret_cast<void **>(&ctx->err_dev), ctx->err_host, 0);
     if (st == cudaSuccess) st = cudaDeviceGetAttribute(&ctx->sm_count, cudaDevAttrMultiProcessorCount, device);
@@ -197,9 +198,10 @@ void await_event(Context &ctx, cudaEvent_t ev, bool collective) {
     }
 }
 
-// Milliseconds between the context's start and stop events, already completed.
+// Milliseconds between the context's start and stop events, the batch having ended.
 double bracket_ms(Context &ctx) {
     float ms = 0;
+    check_cuda(cudaEventSynchronize(ctx.stop), "event synchronization");
     check_cuda(cudaEventElapsedTime(&ms, ctx.start, ctx.stop), "event elapsed time");
     if (!std::isfinite(ms) || ms < 0) raise(JR_ECUDA, "invalid GPU-event duration");
     return ms;
@@ -720,12 +722,16 @@ extern "C" int jr_execute2(void *handle, const jr_dispatch *jobs, size_t job_cou
             cudaStreamSynchronize(ctx.stream);
             throw;
         }
-        const cudaError_t stop = cudaEventRecord(ctx.stop, ctx.stream);
+        // A timed event completes about 4 us after the work before it: a batch whose
+        // time is read later waits for an untimed one ahead of it.
+        const bool defer = flags & JR_EXEC_DEFER_MS && !job_ms;
+        cudaError_t stop = defer ? cudaEventRecord(ctx.done, ctx.stream) : cudaSuccess;
+        if (stop == cudaSuccess) stop = cudaEventRecord(ctx.stop, ctx.stream);
         if (stop != cudaSuccess) {
             cudaStreamSynchronize(ctx.stream);
             check_cuda(stop, "record stop event");
         }
-        await_event(ctx, ctx.stop, collective);
+        await_event(ctx, defer ? ctx.done : ctx.stop, collective);
         raise_device_wait_error(ctx);
         ctx.timed = true;
         if (!(flags & JR_EXEC_DEFER_MS)) *gpu_ms = bracket_ms(ctx);
