@@ -76,10 +76,11 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t *warp_sums
 // above the threshold and entries equal to it together, behind the earlier blocks'
 // totals. Weights come from memory once where a run has at most kSelectTile entries
 // (their keys stay in shared memory), else once per pass.
+template <bool kCluster>
 __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const EvictArgs a) {
     __shared__ uint32_t keys[kSelectTile + kSelectTile / 32], hist[kBins], warp_sums[32], chosen[2], totals[2];
     const cg::cluster_group cluster = cg::this_cluster();
-    const int blocks = cluster.num_blocks(), rank = cluster.block_rank();
+    const int blocks = kCluster ? cluster.num_blocks() : 1, rank = kCluster ? cluster.block_rank() : 0;
     const int bh = blockIdx.x / blocks, b = bh / a.kv_heads, n = a.lengths[b], thread = threadIdx.x;
     grid_dependency_trigger();
     if (n < 0 || n > a.capacity) {  // the same for the whole cluster
@@ -87,7 +88,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         return;
     }
     auto sync = [&] {  // all blocks of the cluster
-        if (blocks > 1) cluster.sync();
+        if constexpr (kCluster) cluster.sync();
         else __syncthreads();
     };
     int *kept = a.kept + (size_t)bh * a.keep;
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         uint32_t c0 = 0, c1 = 0;
 #pragma unroll 8
         for (int r = 0; r < blocks; ++r) {
-            const uint2 c = *reinterpret_cast<const uint2 *>((blocks > 1 ? cluster.map_shared_rank(hist, r) : hist) + high - 1);
+            const uint2 c = *reinterpret_cast<const uint2 *>((kCluster ? cluster.map_shared_rank(hist, r) : hist) + high - 1);
             c0 += c.y, c1 += c.x;
         }
         uint32_t total;
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kSelectThreads) evict_select_kernel(const Evic
         }
     };
     uint32_t takes = 0, ties = 0, mask, equal, total;
-    if (blocks > 1) {
+    if constexpr (kCluster) {
         for (int j0 = lo; j0 < hi; j0 += kSelectTile) {
             if (!single) {
                 __syncthreads();
@@ -303,7 +304,7 @@ LaunchFn make_cache_op(Context *ctx, const Spec &s, std::string &impl) {
         shape.val.clusterDim.x = cluster, shape.val.clusterDim.y = shape.val.clusterDim.z = 1;
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(heads * cluster), config.blockDim = dim3(kSelectThreads), config.stream = st, config.attrs = &shape, config.numAttrs = cluster > 1;
-        cudaError_t e = cudaLaunchKernelEx(&config, evict_select_kernel, a);
+        cudaError_t e = cudaLaunchKernelEx(&config, cluster > 1 ? evict_select_kernel<true> : evict_select_kernel<false>, a);
         if (e == cudaSuccess) e = launch_after(st, evict_move_kernel, dim3(blocks, heads), 256, 0, a);
         return e == cudaSuccess ? cudaGetLastError() : e;
     };
