@@ -23,7 +23,11 @@
 //              weights), O rescaled only when a maximum grows by more than 2^8
 // M <= 128: the chains take alternate key tiles of the same rows and are joined at
 // the segment's end, both sums being in the same TMEM lanes. M > 128: the chains are
-// two row tiles that share each K and V tile.
+// two row tiles that share each K and V tile. M <= 64: the tile holds two copies of the
+// rows, M <= 32: four, and each copy takes a half or a quarter of a key tile's columns
+// (its P is zero in the others), so that all four warps of a chain work and none forms
+// more than 128 / copies weights per row and tile; the copies' sums are joined with the
+// chains'.
 //
 // A tile that reaches beyond the committed slots is masked per row by the drafts'
 // bits. Its V rows from lengths + seq on are zeroed in shared memory before the
@@ -48,13 +52,16 @@ constexpr float kRescaleThreshold = 8.0f;  // log2 units
 // (twice the time per tile): 73.6 us with 6, 74.9 with 10.
 constexpr int boundary_tiles(int rows) { return rows > 128 ? 6 : 6 + rows / 20; }
 
-template <int DP, bool kTwoTiles>
+template <int DP, bool kTwoTiles, int kCopies>
 struct Layout {
     static constexpr uint32_t kChunk = 128 * 128;  // 128 rows x 64 elements, 128-byte swizzle
     static constexpr uint32_t kTile = (DP / 64) * kChunk;
-    static constexpr uint32_t kRing = 2 * kTile;                         // behind Q: two row tiles, or this segment's and the next one's
-    static constexpr int kStages = (224 * 1024 - kRing) / kTile;         // 160 KB of K and V in flight per SM (192 KB for DP = 64)
-    static constexpr uint32_t kExchange = kRing + kStages * kTile;               // (maximum, sum) of every row and chain
+    static constexpr uint32_t kRing = 2 * kTile;  // behind Q: two row tiles, or this segment's and the next one's
+    static constexpr uint32_t kMergeChain = 16384;  // joining the copies: 32 columns of the rows of all copies but one
+    static constexpr uint32_t kMergeBytes = kCopies > 1 ? 2 * kMergeChain : 0;
+    static constexpr int kStages = (224 * 1024 - kRing - kMergeBytes) / kTile;  // 128 KB or more of K and V in flight per SM
+    static constexpr uint32_t kMerge = kRing + kStages * kTile;
+    static constexpr uint32_t kExchange = kMerge + kMergeBytes;  // (maximum, sum) of every lane and chain
     static constexpr uint32_t kBar = kExchange + 2 * 128 * 8;
     static constexpr uint32_t kBytes = kBar + 512;
     // dynamic shared memory starts on a 1024-byte boundary in practice (checked in
@@ -238,11 +245,12 @@ __device__ __forceinline__ void clean_v(uint8_t *v, int thread, int j0, int leng
 }
 
 // ------------------------------------------------------------------ kernel
-template <int DP, typename T, bool kTwoTiles>
+template <int DP, typename T, bool kTwoTiles, int kCopies>
 __global__ void __launch_bounds__(kThreads, 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const TcArgs args) {
-    using L = Layout<DP, kTwoTiles>;
+    using L = Layout<DP, kTwoTiles, kCopies>;
+    constexpr int kCopyRows = 128 / kCopies, kCopyKeys = 128 / kCopies;  // rows of a copy, columns of a tile that it takes
     constexpr uint32_t kFmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     constexpr uint32_t kIdescS = idesc_f32acc(kFmt, kFmt, false, false, kTileRows, kTileKeys);
     constexpr uint32_t kIdescO = idesc_f32acc(kFmt, kFmt, false, true, kTileRows, DP);
@@ -258,7 +266,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *q_full = bars, *q_empty = bars + 2, *s_full = bars + 4, *p_full = bars + 6, *o_full = bars + 8, *o_free = bars + 10;
     uint64_t *x_full = bars + 12, *x_empty = bars + 13, *mma_done = bars + 14;
     uint64_t *full = bars + 16, *empty = bars + 16 + kStages;  // ring stages
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 44);
+    uint64_t *g_full = bars + 44, *g_empty = bars + 46;  // joining the copies [chain]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 48);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     uint32_t *bad = tmem_slot + 4;  // [3][4]: drafts with non-finite V, by segment number modulo 3
     int *plan = reinterpret_cast<int *>(tmem_slot + 16);  // the range's first b, sub, tile and (64 bits) length
@@ -276,6 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&s_full[t], 1); mbar_init(&p_full[t], 128);
             mbar_init(&o_full[t], 1); mbar_init(&o_free[t], kTwoTiles ? 128 : 256);
         }
+        for (int t = 0; t < 2; ++t) mbar_init(&g_full[t], 128 - kCopyRows + (kCopies == 1)), mbar_init(&g_empty[t], kCopyRows);
         mbar_init(x_full, 256); mbar_init(x_empty, 256); mbar_init(mma_done, 1);
         for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
         *abort_flag = 0;
@@ -314,7 +324,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (!(ok = ok && mbar_wait(&q_empty[buffer], (use & 1) ^ 1, abort_flag, err, kErrWaitSmemEmpty))) return;
                     mbar_arrive_expect_tx(&q_full[buffer], L::kTile);
                     for (int c = 0; c < kDChunks; ++c)
-                        tma_load_3d(smem + buffer * L::kTile + c * L::kChunk, &tmQ, &q_full[buffer], c * 64, tile * kTileRows, bh);
+                        for (int copy = 0; copy < kCopies; ++copy)
+                            tma_load_3d(smem + buffer * L::kTile + c * L::kChunk + copy * kCopyRows * 128, &tmQ, &q_full[buffer], c * 64,
+                                        tile * kTileRows, bh);
                 };
                 if constexpr (kTwoTiles) {  // row tiles 2 rb and 2 rb + 1 (which may lie beyond the rows: zeros)
                     load_q(0, 2 * s.rb, q_loads);
@@ -435,16 +447,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_wait_drain(mma_done, 0, err);
     } else {
         // ----------------------------------------------------- softmax (warps 2-5: chain 0, 6-9: chain 1)
-        const int t = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+        const int t = (warp - 2) >> 2, quarter = warp & 3, row = quarter * 32 + lane, copy = row / kCopyRows, copy_row = row % kCopyRows;
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t ts = tmem_s[t] + lane_off, to = tmem_o[t] + lane_off;
         const float c = ta.scale_log2;
-        // cs: S tiles consumed; on: segments with O_t; xn: exchanges; ring: loads before the segment; sn: segments
-        int cs = 0, on[2] = {0, 0}, xn = 0, ring = 0, sn = 0;
+        // cs: S tiles consumed; on: segments with O_t; xn: exchanges; gn: columns joined; ring: loads before the segment; sn: segments
+        int cs = 0, on[2] = {0, 0}, xn = 0, gn = 0, ring = 0, sn = 0;
         bool ok = true;
         for (; ok && segments.next(args, s); ++sn) {
             const int n = s.count(), bh = s.b * ta.kv_heads + s.hk;
-            const int item_row = kTwoTiles ? s.rb * 256 + t * 128 + row : row;  // row of the item's M
+            const int item_row = kTwoTiles ? s.rb * 256 + t * 128 + row : copy_row;  // row of the item's M
             const bool live = __any_sync(0xffffffffu, item_row < ta.rows);      // some row of this warp is one
             uint32_t bits[4] = {0, 0, 0, 0};
             uint32_t *bad_now = bad + (sn % 3) * 4;
@@ -470,29 +482,27 @@ __global__ void __launch_bounds__(kThreads, 1)
                     fence_proxy_async();
                 }
                 if (live) {
-                    float sv[128];
-                    tmem_ld32f(ts, sv);
-                    tmem_ld32f(ts + 32, sv + 32);
-                    tmem_ld32f(ts + 64, sv + 64);
-                    tmem_ld32f(ts + 96, sv + 96);
+                    float sv[kCopyKeys];
+#pragma unroll
+                    for (int k = 0; k < kCopyKeys; k += 32) tmem_ld32f(ts + copy * kCopyKeys + k, sv + k);
                     tmem_wait_ld();
                     if (masked) {
                         uint32_t seen[4], mask[4];
 #pragma unroll
                         for (int w = 0; w < 4; ++w) seen[w] = bits[w] & draft_bits(w, ta.seq);
-                        column_mask(seen, s.length - j0, mask);
+                        column_mask(seen, s.length - j0 - copy * kCopyKeys, mask);
 #pragma unroll
-                        for (int k = 0; k < 128; ++k) sv[k] = mask[k >> 5] >> (k & 31) & 1 ? sv[k] : -INFINITY;
+                        for (int k = 0; k < kCopyKeys; ++k) sv[k] = mask[k >> 5] >> (k & 31) & 1 ? sv[k] : -INFINITY;
                     }
                     float mx[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) mx[e] = max3(sv[e], sv[e + 8], sv[e + 16]);
 #pragma unroll
-                    for (int k = 24; k < 120; k += 16)
+                    for (int k = 24; k < kCopyKeys - 8; k += 16)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], sv[k + e], sv[k + 8 + e]);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], sv[120 + e]);
+                    for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], sv[kCopyKeys - 8 + e]);
                     const float m_tile = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
                     float m_new = m_used, alpha = 1.0f;
                     if (first) m_new = m_tile;
@@ -502,8 +512,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     m_used = m_new;
                     // a row that has seen nothing yet has maximum -inf: its weights are e^-inf = 0
-                    const float psum = masked ? store_p<kFmt, false, 128>(sv, c, m_used == -INFINITY ? 0.0f : m_used, ts)
-                                              : store_p<kFmt, kTwoTiles, 128, 2>(sv, c, m_used, ts);
+                    const uint32_t tp = ts + copy * (kCopyKeys / 2);
+                    const float psum = masked ? store_p<kFmt, false, kCopyKeys>(sv, c, m_used == -INFINITY ? 0.0f : m_used, tp)
+                                              : store_p<kFmt, kTwoTiles, kCopyKeys, 2>(sv, c, m_used, tp);
+                    if constexpr (kCopies > 1) {
+                        const uint32_t zeros[8] = {};
+#pragma unroll
+                        for (int k = 0; k < 64; k += 8)
+                            if (k / (kCopyKeys / 2) != copy) tmem_st8(ts + k, zeros);
+                    }
                     if (!first && __any_sync(0xffffffffu, alpha != 1.0f)) {
 #pragma unroll 1
                         for (int oc = 0; oc < DP; oc += 32) {
@@ -533,19 +550,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 mbar_arrive(x_full);
                 ok = __all_sync(0xffffffffu, mbar_wait(x_full, xn++ & 1, abort_flag, err, kErrWaitPv));
                 if (!ok) break;
-                const float2 e0 = exchange[row], e1 = exchange[128 + row];
+                float2 e[2][kCopies];
+                m_used = -INFINITY;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int y = 0; y < kCopies; ++y) e[x][y] = exchange[x * 128 + y * kCopyRows + copy_row], m_used = fmaxf(m_used, e[x][y].x);
                 mbar_arrive(x_empty);
-                m_used = fmaxf(e0.x, e1.x);
                 const float shift = m_used == -INFINITY ? 0.0f : m_used;
-                f0 = mufu_exp2(e0.x - shift), f1 = mufu_exp2(e1.x - shift);
-                l_run = e0.y * f0 + e1.y * f1;
+                l_run = 0.0f;
+#pragma unroll
+                for (int y = 0; y < kCopies; ++y) {
+                    const float g0 = mufu_exp2(e[0][y].x - shift), g1 = mufu_exp2(e[1][y].x - shift);
+                    l_run += e[0][y].y * g0 + e[1][y].y * g1;
+                    if (y == copy) f0 = g0, f1 = g1;
+                }
             }
             const int o0 = kTwoTiles ? t : 0;
             ok = __all_sync(0xffffffffu, mbar_wait(&o_full[o0], on[o0]++ & 1, abort_flag, err, kErrWaitPv));
             if (ok && both) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[1], on[1]++ & 1, abort_flag, err, kErrWaitPv));
             if (!ok) break;
             tc_fence_after();
-            const bool whole = s.first == 0 && s.last == s.tiles, valid = item_row < ta.rows;
+            const bool whole = s.first == 0 && s.last == s.tiles, valid = item_row < ta.rows && copy == 0;
             const float inv = l_run > 0.0f || l_run != l_run ? 1.0f / l_run : 0.0f;
             if (whole) f0 *= inv, f1 *= inv;
             uint32_t extra[4];
@@ -573,6 +599,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                     } else {
 #pragma unroll
                         for (int k = 0; k < 32; ++k) r[k] *= f0;
+                    }
+                    if constexpr (kCopies > 1) {  // the first copy's threads add up the others' rows, 32 columns at a time
+                        float *merge = reinterpret_cast<float *>(smem + L::kMerge + t * L::kMergeChain);
+                        if (copy > 0) {
+                            ok = ok && __all_sync(0xffffffffu, mbar_wait(&g_empty[t], (gn & 1) ^ 1, abort_flag, err, kErrWaitAccEmpty));
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) merge[((copy - 1) * 32 + k) * kCopyRows + copy_row] = r[k];
+                            mbar_arrive(&g_full[t]);
+                        } else {
+                            ok = ok && __all_sync(0xffffffffu, mbar_wait(&g_full[t], gn & 1, abort_flag, err, kErrWaitPv));
+#pragma unroll
+                            for (int y = 0; y < kCopies - 1; ++y)
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) r[k] += merge[(y * 32 + k) * kCopyRows + copy_row];
+                            mbar_arrive(&g_empty[t]);
+                        }
+                        ++gn;
                     }
                     if (extra[0] | extra[1] | extra[2] | extra[3]) {  // non-finite values that this row sees
 #pragma unroll
@@ -603,6 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     __syncwarp();
                 }
             }
+            if (!ok) break;
             tc_fence_before();
             mbar_arrive(&o_free[o0]);
             if (both) mbar_arrive(&o_free[1]);
@@ -924,20 +968,20 @@ EncodeFn encoder() {
     return fn;
 }
 
-// [heads, rows, dim] tensor, box {64, 128, 1}, 128-byte swizzle; elements beyond dim or rows read as 0.
-bool row_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, uint64_t heads, uint64_t rows, uint64_t dim) {
+// [heads, rows, dim] tensor, box {64, box_rows, 1}, 128-byte swizzle; elements beyond dim or rows read as 0.
+bool row_map(CUtensorMap *map, CUtensorMapDataType dt, const void *ptr, uint64_t heads, uint64_t rows, uint64_t dim, uint32_t box_rows = 128) {
     const cuuint64_t dims[3] = {dim, rows, heads};
     const cuuint64_t strides[2] = {dim * 2, rows * dim * 2};
-    const cuuint32_t box[3] = {64, 128, 1};
+    const cuuint32_t box[3] = {64, box_rows, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     return encoder()(map, dt, 3, const_cast<void *>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DP, typename T, bool kTwoTiles>
+template <int DP, typename T, bool kTwoTiles, int kCopies>
 LaunchFn tc_launch(Context *ctx, const Spec &s) {
-    using L = Layout<DP, kTwoTiles>;
-    auto kernel = tree_tc_kernel<DP, T, kTwoTiles>;
+    using L = Layout<DP, kTwoTiles, kCopies>;
+    auto kernel = tree_tc_kernel<DP, T, kTwoTiles, kCopies>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::kSmem) != cudaSuccess)
         throw IrError("cannot reserve shared memory for the tcgen05 attention_tree");
     constexpr int kSlotRows = kTwoTiles ? 256 : 128;
@@ -967,15 +1011,15 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
     return [=, keep = ws](cudaStream_t st, void **b) {
         TcArgs a = base;
         a.t = tree_bind(base.t, b, weights);
-        CUtensorMap mq, mk, mv;
-        if (!row_map(&mq, dt, b[0], heads, rows, dim) || !row_map(&mk, dt, b[1], heads, capacity, dim) || !row_map(&mv, dt, b[2], heads, capacity, dim))
+        CUtensorMap mq, mqw, mk, mv;  // mqw: Q for the weights' pass
+        if (!row_map(&mq, dt, b[0], heads, rows, dim, 128 / kCopies) || !row_map(&mqw, dt, b[0], heads, rows, dim) || !row_map(&mk, dt, b[1], heads, capacity, dim) || !row_map(&mv, dt, b[2], heads, capacity, dim))
             return cudaErrorInvalidValue;
         kernel<<<a.ctas, kThreads, L::kSmem, st>>>(mq, mk, mv, a);
         cudaError_t e = launch_after(st, tree_join_tc<DP, T>, (int)join_blocks, kJoinThreads, 0, a, item_blocks);
         if (weights && e == cudaSuccess) {
             TcArgs w = a;
             w.row_blocks = 1, w.boundary = kWeightsBoundary;
-            e = launch_after(st, weights_kernel, a.ctas, kThreads, W::kSmem, mq, mk, w);
+            e = launch_after(st, weights_kernel, a.ctas, kThreads, W::kSmem, mqw, mk, w);
         }
         return e == cudaSuccess ? cudaGetLastError() : e;
     };
@@ -985,11 +1029,15 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
 
 LaunchFn make_attention_tree_tc(Context *ctx, const Spec &s) {
     if (!encoder()) throw IrError("cuTensorMapEncodeTiled unavailable");
-    const bool two = (uint64_t)s.heads / s.kv_heads * s.seq > kTileRows, wide = s.dim > 64;
-    auto pick = [&](auto type) {
+    const uint64_t rows = (uint64_t)s.heads / s.kv_heads * s.seq;
+    auto shape = [&](auto type, auto width) -> LaunchFn {
         using T = decltype(type);
-        if (wide) return two ? tc_launch<128, T, true>(ctx, s) : tc_launch<128, T, false>(ctx, s);
-        return two ? tc_launch<64, T, true>(ctx, s) : tc_launch<64, T, false>(ctx, s);
+        constexpr int DP = decltype(width)::value;
+        if (rows > kTileRows) return tc_launch<DP, T, true, 1>(ctx, s);
+        return rows > 64 ? tc_launch<DP, T, false, 1>(ctx, s) : rows > 32 ? tc_launch<DP, T, false, 2>(ctx, s) : tc_launch<DP, T, false, 4>(ctx, s);
+    };
+    auto pick = [&](auto type) {
+        return s.dim > 64 ? shape(type, std::integral_constant<int, 128>{}) : shape(type, std::integral_constant<int, 64>{});
     };
     return s.dtype == DType::BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
 }
