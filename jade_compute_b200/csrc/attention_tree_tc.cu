@@ -674,11 +674,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // Joins the parts of items that several CTAs share, in range order. A thread takes
 // one row and four columns: consecutive threads, consecutive memory of every part.
+// kWays > 1: the parts are dealt to kWays threads each, whose sums are added in order:
+// few items have many parts, and one thread would wait for them one after the other.
 constexpr int kJoinThreads = 256;
 
-template <int DP, typename T>
+template <int DP, typename T, int kWays>
 __global__ void __launch_bounds__(kJoinThreads) tree_join_tc(const TcArgs a, int blocks) {
+    constexpr int kEach = kJoinThreads / kWays;  // rows x columns / 4 of a block
     __shared__ long long counts[2];
+    __shared__ float maxima[kWays][kEach];
+    __shared__ float4 sums[kWays][kEach];
+    __shared__ float totals[kWays][kEach];
     const TreeArgs &t = a.t;
     const int subs = t.kv_heads * a.row_blocks;
     const int item = blockIdx.x / blocks, b = item / subs, sub = item - b * subs, hk = sub / a.row_blocks, rb = sub - hk * a.row_blocks;
@@ -695,27 +701,50 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_tc(const TcArgs a, int
         if (threadIdx.x == 0) counts[0] = all, counts[1] = before;
     }
     __syncthreads();
-    const int at = (blockIdx.x - item * blocks) * kJoinThreads + threadIdx.x, col = at / a.slot_rows, slot_row = at - col * a.slot_rows;
+    const int way = threadIdx.x / kEach, lane = threadIdx.x % kEach;
+    const int at = (blockIdx.x - item * blocks) * kEach + lane, col = at / a.slot_rows, slot_row = at - col * a.slot_rows;
     const int row = rb * a.slot_rows + slot_row;
     const int tiles = tiles_of(t, length_of(t, b));
     grid_dependency_wait();  // in every block: this grid's end stands for the one's before it
     const long long per = range_units(a, counts[0] * subs), begin = counts[1] * subs + (long long)sub * (tiles + a.boundary);
     const int c0 = (int)(begin / per), c1 = (int)((begin + tiles - 1) / per);
-    if (tiles == 0 || c0 == c1 || row >= t.rows || col * 4 >= DP) return;  // c0 == c1: written whole
+    if (tiles == 0 || c0 == c1) return;  // c0 == c1: written whole
+    const bool on = row < t.rows && col * 4 < DP;
     auto slot = [&](int c) { return (size_t)c * 2 + (c == c0); };
     float m = -INFINITY, l = 0.0f;
-    for (int c = c0; c <= c1; ++c) m = fmaxf(m, t.part_ml[slot(c) * a.slot_rows + slot_row].x);
-    const float shift = m == -INFINITY ? 0.0f : m;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    const float4 *part = reinterpret_cast<const float4 *>(t.part_o) + at;
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-        const float2 ml = t.part_ml[slot(c) * a.slot_rows + slot_row];
-        const float4 x = part[slot(c) * (DP / 4) * a.slot_rows];
-        const float w = exp2f(ml.x - shift);
-        l = fmaf(ml.y, w, l);
-        o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+    if (on)
+        for (int c = c0 + way; c <= c1; c += kWays) m = fmaxf(m, t.part_ml[slot(c) * a.slot_rows + slot_row].x);
+    if constexpr (kWays > 1) {
+        maxima[way][lane] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWays; ++w) m = fmaxf(m, maxima[w][lane]);
     }
+    const float shift = m == -INFINITY ? 0.0f : m;
+    if (on) {
+        const float4 *part = reinterpret_cast<const float4 *>(t.part_o) + at;
+#pragma unroll 4
+        for (int c = c0 + way; c <= c1; c += kWays) {
+            const float2 ml = t.part_ml[slot(c) * a.slot_rows + slot_row];
+            const float4 x = part[slot(c) * (DP / 4) * a.slot_rows];
+            const float w = exp2f(ml.x - shift);
+            l = fmaf(ml.y, w, l);
+            o.x = fmaf(w, x.x, o.x), o.y = fmaf(w, x.y, o.y), o.z = fmaf(w, x.z, o.z), o.w = fmaf(w, x.w, o.w);
+        }
+    }
+    if constexpr (kWays > 1) {
+        sums[way][lane] = o, totals[way][lane] = l;
+        __syncthreads();
+        if (way > 0) return;
+#pragma unroll
+        for (int w = 1; w < kWays; ++w) {
+            const float4 x = sums[w][lane];
+            o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+            l += totals[w][lane];
+        }
+    }
+    if (!on) return;
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     if (col == 0 && t.row_exponents) store_stats(t, (size_t)b * t.kv_heads + hk, row, m, inv);
     if (col * 4 >= t.dim) return;
@@ -994,7 +1023,10 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
     base.ctas = most < (unsigned __int128)ctx->sm_count ? (int)most : ctx->sm_count;
     base.boundary = boundary_tiles((int)rows);
     base.slot_rows = rows >= (uint64_t)kSlotRows ? kSlotRows : (int)((rows + 7) / 8 * 8);
-    const int item_blocks = (base.slot_rows * (DP / 4) + kJoinThreads - 1) / kJoinThreads;
+    // an item's parts: the CTAs over the items; from about 8 on a thread's are too many
+    const bool spread = heads * base.row_blocks * 8 <= (uint64_t)base.ctas;
+    constexpr int kWays = 8;
+    const int each = spread ? kJoinThreads / kWays : kJoinThreads, item_blocks = (base.slot_rows * (DP / 4) + each - 1) / each;
     const long long join_blocks = (long long)heads * base.row_blocks * item_blocks;
     if (join_blocks > INT_MAX) throw IrError("attention_tree too large for one launch");
     const bool weights = s.weights;
@@ -1015,7 +1047,7 @@ LaunchFn tc_launch(Context *ctx, const Spec &s) {
         if (!row_map(&mq, dt, b[0], heads, rows, dim, 128 / kCopies) || !row_map(&mqw, dt, b[0], heads, rows, dim) || !row_map(&mk, dt, b[1], heads, capacity, dim) || !row_map(&mv, dt, b[2], heads, capacity, dim))
             return cudaErrorInvalidValue;
         kernel<<<a.ctas, kThreads, L::kSmem, st>>>(mq, mk, mv, a);
-        cudaError_t e = launch_after(st, tree_join_tc<DP, T>, (int)join_blocks, kJoinThreads, 0, a, item_blocks);
+        cudaError_t e = launch_after(st, spread ? tree_join_tc<DP, T, kWays> : tree_join_tc<DP, T, 1>, (int)join_blocks, kJoinThreads, 0, a, item_blocks);
         if (weights && e == cudaSuccess) {
             TcArgs w = a;
             w.row_blocks = 1, w.boundary = kWeightsBoundary;
