@@ -202,6 +202,11 @@ TREES = [
     dict(batch=5, seq=2, heads=4, kv_heads=4, dim=128, capacity=2100, lengths=[2098, 1000, 3, 0, 2047]),
     dict(batch=1, seq=1, heads=64, kv_heads=1, dim=128, capacity=9000, lengths=[8999]),
     dict(batch=1, seq=16, heads=8, kv_heads=8, dim=120, capacity=1500, lengths=[1400]),
+    # more sequences than a warp has lanes, lengths around the tiles' ends, most items short
+    dict(batch=77, seq=3, heads=4, kv_heads=2, dim=64, capacity=400, lengths=[(37 * b) % 398 if b % 5 else (0, 125, 126, 253, 397)[b // 5 % 5] for b in range(77)]),
+    dict(batch=4, seq=10, heads=12, kv_heads=3, dim=72, capacity=1100, lengths=[1090, 118, 119, 500]),  # 40 rows
+    dict(batch=2, seq=17, heads=6, kv_heads=2, dim=104, capacity=1300, lengths=[1283, 640]),  # 51 rows
+    dict(batch=2, seq=100, heads=3, kv_heads=1, dim=64, capacity=5000, lengths=[4900, 20]),  # 300 rows: a second row block
 ]
 
 
@@ -536,3 +541,61 @@ def test_batch_times_outlive_the_next_batch_and_the_runtime():
         r.close()
     assert second.gpu_ms > 0 and first.gpu_ms > 5 * second.gpu_ms and third.gpu_ms > 5 * second.gpu_ms
     assert first.gpu_ms == first.gpu_ms
+
+
+# ------------------------------------------------------------------ the runtime's ways to run a batch
+def tensors(rt, spec, arrays):
+    kernel, bufs = rt.compile(spec), {}
+    for b in kernel.info["bindings"]:
+        bufs[b["name"]] = rt.alloc(b["elements"], b["dtype"])
+        if b["name"] in arrays:
+            x = np.asarray(arrays[b["name"]]).ravel()
+            rt.upload(bufs[b["name"]], x if b["dtype"] == "i32" else jc.f32_to_bf16(x.astype(np.float32)) if b["dtype"] == "bf16" else x)
+    return kernel, bufs
+
+
+@pytest.mark.parametrize("way", [{"graph": True}, {"streams": True}, {"per_job": True}])
+def test_batches_of_several_operators_run_every_way(rt, way):
+    # two attention kernels with their own workspaces in turn, an eviction and a gradient: each
+    # is several launches, some started early; a graph, transfer streams and per-job events
+    # give what single batches gave
+    cases = [(tree_spec(TREES[i], "bf16"), tree_inputs(TREES[i], "bf16", i)[0]) for i in (1, 4)]
+    ev = {"op": "cache_evict", "batch": 1, "kv_heads": 2, "dim": 64, "capacity": 900, "keep": 100, "recent": 5, "dtype": "bf16"}
+    rng = np.random.default_rng(60)
+    cases.append((ev, {"k": R.rounded(rng.standard_normal((1, 2, 900, 64)), "bf16"), "v": R.rounded(rng.standard_normal((1, 2, 900, 64)), "bf16"),
+                       "weights": rng.random((1, 2, 900)).astype(np.float32), "lengths": np.array([850], np.int32)}))
+    grad = rope_spec(ROPES[1], "bf16", "qk_norm_rope_grad")
+    cases.append((grad, grad_inputs(grad, 1)))
+    jobs = [tensors(rt, spec, x) for spec, x in cases]
+    try:
+        expected = [R.run(rt, spec, x) for spec, x in cases]
+        batch = [(k, [bufs[b["name"]] for b in k.info["bindings"]]) for k, bufs in jobs]
+        done = rt.execute(batch, **way)
+        assert not way.get("per_job") or min(done.job_ms) > 0
+        for (k, bufs), want in zip(jobs, expected):
+            for name, values in want.items():
+                got = rt.download(bufs[name]) if bufs[name].dtype == "i32" else rt.download_f32(bufs[name])
+                np.testing.assert_array_equal(got.astype(values.dtype), values, err_msg=name)
+        if "graph" in way:  # replays: the attention weights accumulate, everything else stays
+            rt.execute(batch, repeats=3, graph=True)
+            for (k, bufs), want in zip(jobs, expected):
+                for name, values in want.items():
+                    if name != "weights":
+                        got = rt.download(bufs[name]) if bufs[name].dtype == "i32" else rt.download_f32(bufs[name])
+                        np.testing.assert_array_equal(got.astype(values.dtype), values, err_msg=name)
+    finally:
+        for k, bufs in jobs:
+            for b in bufs.values():
+                b.free()
+
+
+def test_weight_gradients_repeat_bit_for_bit(rt):
+    spec = rope_spec(dict(batch=3, seq=700, heads=8, kv_heads=2, dim=96, rotary=32), "bf16", "qk_norm_rope_grad")
+    x = grad_inputs(spec, 61)
+    a, b = (R.run(rt, spec, x, repeats=n) for n in (1, 3))
+    for name in a:
+        np.testing.assert_array_equal(a[name], b[name])
+    ref, m, dw = rope_gradient(spec, x)
+    close(a["dqkv"].reshape(ref.shape), ref, m, R.ROUNDOFF["bf16"], 2e-5)
+    for name, (s, ms) in dw.items():
+        close(a[f"d{name}_weight"], s, ms, 0.0, 2e-5)
