@@ -27,7 +27,9 @@
 // a few a lane, in shared memory; the rows of the next rounds load meanwhile. Angles
 // and norm weights are read from shared memory for every round: registers hold rows
 // only, so that enough warps are resident. No block barrier per token, so that warps
-// drift apart and memory stays busy.
+// drift apart and memory stays busy. Measured on B200, BF16, 4 x 2048 tokens of 16 + 2 x 16
+// heads of 128 (201 MB moved; a plain copy of them takes 36 us): 42 us = 4.7 TB/s with
+// halves, 52 with neighbours; the gradient (268 MB) 64 us = 4.2 TB/s. One token: 4.2 us.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -453,7 +455,8 @@ __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a
     }
 }
 
-// Sums the blocks' partial weight gradients: 32 columns of [blocks][2 dim] a block,
+// Sums the blocks' partial weight gradients (592 blocks of 2 x 128: about 3 us behind the
+// rows, bound by the latency of a few dependent loads): 32 columns of [blocks][2 dim] a block,
 // its 32 warps striding over the blocks, then over the warps' sums in order.
 __global__ void __launch_bounds__(1024) rope_weight_grad_kernel(const float *partial, int blocks, int dim, float *dq, float *dk) {
     __shared__ float sums[32][33];
@@ -474,6 +477,8 @@ __global__ void __launch_bounds__(1024) rope_weight_grad_kernel(const float *par
     }
 }
 
+// A token's heads are dealt to several warps while that leaves the GPU's warps (as many
+// as are resident) at most this many items each.
 constexpr int kPartWaves = 2;
 
 // theta_i / 2 pi as 0.64 fixed-point fractions of a turn.
