@@ -22,63 +22,14 @@
 #include <climits>
 #include <type_traits>
 
+#include "attention_softmax.cuh"
 #include "attention_tree.cuh"
 
 namespace jade {
 namespace {
 
-constexpr int kThreads = 128, kRows = 16, kKeys = 32;  // a block: 16 rows of q, tiles of 32 keys
 constexpr int kMaxSplits = 64;
-
-template <typename T>
-__device__ __forceinline__ float4 load4(const T *p);
-template <>
-__device__ __forceinline__ float4 load4<float>(const float *p) { return __ldg(reinterpret_cast<const float4 *>(p)); }
-template <>
-__device__ __forceinline__ float4 load4<__nv_bfloat16>(const __nv_bfloat16 *p) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
-    const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.x)), b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162 *>(&u.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-template <>
-__device__ __forceinline__ float4 load4<__half>(const __half *p) {
-    const uint2 u = __ldg(reinterpret_cast<const uint2 *>(p));
-    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-
-__host__ __device__ constexpr int q_stride(int dim) { return dim + 4; }  // rows 4 banks apart
-
-// Rows of q or keys (zeros from `limit` on) as FP32 into shared memory: 8 threads a
-// row, 16 rows at a time, the loads of all of a thread's rows under way together.
-template <typename T, int kCount>
-__device__ __forceinline__ void stage(float *dst, const T *src, int first, int limit, int dim) {
-    const int r = threadIdx.x >> 3;
-    for (int c = (threadIdx.x & 7) * 4; c < dim; c += 32) {
-        float4 x[kCount / 16];
-#pragma unroll
-        for (int i = 0; i < kCount / 16; ++i) {
-            x[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (first + r + 16 * i < limit) x[i] = load4(src + (size_t)(first + r + 16 * i) * dim + c);
-        }
-#pragma unroll
-        for (int i = 0; i < kCount / 16; ++i) *reinterpret_cast<float4 *>(dst + (r + 16 * i) * q_stride(dim) + c) = x[i];
-    }
-}
-
-// Scores of row r with keys c, c + 8, c + 16, c + 24 of the tile.
-__device__ __forceinline__ void tile_scores(const float *q, const float *k, int r, int c, int dim, float (&s)[4]) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) s[u] = 0.0f;
-    for (int d = 0; d < dim; d += 4) {
-        const float4 a = *reinterpret_cast<const float4 *>(q + r * q_stride(dim) + d);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float4 b = *reinterpret_cast<const float4 *>(k + (c + 8 * u) * q_stride(dim) + d);
-            s[u] = fmaf(a.x, b.x, fmaf(a.y, b.y, fmaf(a.z, b.z, fmaf(a.w, b.w, s[u]))));
-        }
-    }
-}
+constexpr float kRescaleThreshold = 8.0f;  // log2 units
 
 __device__ __forceinline__ bool sees(const TreeArgs &a, int b, int row, int j, int length) {
     if (j < length) return true;
@@ -87,80 +38,241 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, int b, int row, int j, i
     return a.tree[((size_t)b * a.seq + row % a.seq) * a.words + (i >> 5)] >> (i & 31) & 1;
 }
 
-// grid: (row blocks, splits, batch * kv_heads); kCols: 32-element columns of a head
-template <typename T, int kCols>
-__global__ void __launch_bounds__(kThreads) tree_simt_kernel(const TreeArgs a, int splits) {
-    extern __shared__ float smem[];
-    float *q = smem, *k = q + kRows * q_stride(a.dim), *v = k + kKeys * q_stride(a.dim), *p = v + kKeys * q_stride(a.dim);
-    const int bh = blockIdx.z, b = bh / a.kv_heads, r = threadIdx.x >> 3, c = threadIdx.x & 7, row = blockIdx.x * kRows + r;
+// A block of four warps: K and V tiles of a split's keys, each a contiguous run of the
+// cache, come by bulk copies through a ring. Warps take row groups
+// of four rows, in registers with their sums, and a group's warps share the tile's keys.
+// kLanes lanes hold a key's elements (four at 4 lane + 4 kLanes i), so a warp works on
+// 32 / kLanes keys at once and twice as many an iteration: 4 rows x 2 keys of scores per
+// lane are summed by halving exchanges (7 shuffles, not 24) that leave each lane one
+// score, whose exponential it forms alone and hands back to the others. Maxima and sums
+// are per lane group and joined at the end; sums are rescaled only when a maximum grows
+// by more than 2^8. K and V cross shared memory once per row group.
+// Bound by HBM for a few rows, else by FFMA issue beside shuffles and shared-memory reads.
+// Measured on B200, FP32, dim 128: 64 heads of 1,000 to 8,000 keys, 4 rows (295 MB), 62 us
+// with the join = 4.8 TB/s; 32 heads of 1,000 to 4,000, 4 / 16 / 64 rows: 26 / 47 / 153 us;
+// 16 heads of up to 4,000, 512 rows, 442 us = 23 TFLOP/s. No fifth warp for the copies: it
+// would cap the others at 168 registers, and the spills cost more (62 us for 47).
+constexpr int kStreamWarps = 4, kStreamThreads = 32 * kStreamWarps, kStreamStages = 3, kGroupRows = 4;
+constexpr int kStreamPad = 1024;  // behind the ring: the last V row is read up to the lanes' width
+
+struct Four {  // four elements as packed FP32 pairs
+    uint64_t lo, hi;
+};
+__device__ __forceinline__ Four four_of(const float *p) {
+    const ulonglong2 u = *reinterpret_cast<const ulonglong2 *>(p);
+    return {u.x, u.y};
+}
+__device__ __forceinline__ Four four_of(const __nv_bfloat16 *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    return {pack2f(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u)), pack2f(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u))};
+}
+__device__ __forceinline__ Four four_of(const __half *p) {
+    const uint2 u = *reinterpret_cast<const uint2 *>(p);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&u.x)), y = __half22float2(*reinterpret_cast<const __half2 *>(&u.y));
+    return {pack2f(x.x, x.y), pack2f(y.x, y.y)};
+}
+
+// The pieces of a head that a lane holds, four elements each. kAll: as they lie there,
+// else zeros beyond the head.
+template <bool kAll, int kLanes, int kPieces, typename T>
+__device__ __forceinline__ void load_pieces(uint64_t (&x)[2 * kPieces], const T *p, int c, int dim) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        Four f{0, 0};
+        if (kAll || 4 * (c + kLanes * i) < dim) f = four_of(p + 4 * (c + kLanes * i));
+        x[2 * i] = f.lo, x[2 * i + 1] = f.hi;
+    }
+}
+template <int kPairs>
+__device__ __forceinline__ float dot(const uint64_t (&x)[kPairs], const uint64_t (&y)[kPairs]) {
+    uint64_t s = mul2(x[0], y[0]);
+#pragma unroll
+    for (int i = 1; i < kPairs; ++i) s = fma2(x[i], y[i], s);
+    float lo, hi;
+    unpack2f(s, lo, hi);
+    return lo + hi;
+}
+// Sums eight values over kLanes lanes; lane c gets the total of value c * 8 / kLanes.
+template <int kLanes>
+__device__ __forceinline__ float scattered_sum(float (&v)[8], int c) {
+    int o = kLanes / 2;
+#pragma unroll
+    for (int n = 4; n > 0; n >>= 1, o >>= 1) {
+        const bool up = c & o;
+#pragma unroll
+        for (int i = 0; i < n; ++i) v[i] = (up ? v[i + n] : v[i]) + __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + n], o);
+    }
+#pragma unroll
+    for (; o > 0; o >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    return v[0];
+}
+
+// grid: (row blocks of `groups` row groups, splits, batch * kv_heads)
+template <typename T, int kLanes, int kPieces, bool kWhole>
+__global__ void __launch_bounds__(kStreamThreads, 2) tree_stream_kernel(const TreeArgs a, int splits, int groups, int tile_keys) {
+    constexpr int kKeys = 32 / kLanes, kSame = kLanes / 8;  // keys at once; lanes that get the same score
+    extern __shared__ __align__(128) uint8_t ring_smem[];
+    __shared__ uint64_t full[kStreamStages], empty[kStreamStages];
+    __shared__ int aborted;
+    volatile int *abort_flag = &aborted;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bh = blockIdx.z, b = bh / a.kv_heads;
     const int length = a.lengths[b];
     if (length < 0 || length > a.capacity - a.seq) {
         if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrCacheLength);
         return;
     }
     grid_dependency_trigger();
-    const int n = length + a.seq, tiles = (n + kKeys - 1) / kKeys;
+    const int key_warps = kStreamWarps / groups, active = key_warps * groups;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStreamStages; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], active);
+        aborted = 0;
+        fence_barrier_init();
+        fence_proxy_async();
+    }
+    __syncthreads();
+    const int n = length + a.seq, tiles = (n + tile_keys - 1) / tile_keys;
     const int t0 = (int)((long long)tiles * blockIdx.y / splits), t1 = (int)((long long)tiles * (blockIdx.y + 1) / splits);
     const size_t base = (size_t)bh * a.capacity * a.dim;
-    stage<T, kRows>(q, static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, blockIdx.x * kRows, a.rows, a.dim);
+    const uint32_t tile = (uint32_t)tile_keys * a.dim;  // elements
+    T *ring = reinterpret_cast<T *>(ring_smem);
+    int loads = 0;
+
+    const int g = lane / kLanes, c = lane % kLanes, group = warp % groups, kw = warp / groups;
+    const int row0 = (blockIdx.x * groups + group) * kGroupRows;
+    const int mine = c / kSame, my_row = row0 + (mine >> 1), my_key = (mine & 1) * kKeys + g;  // of this lane's score
+    uint64_t o[kGroupRows][2 * kPieces];
     float m = -INFINITY, l = 0.0f;
-    float4 o[kCols];
+    // Thread 0 issues the copies; a stage is refilled one tile after it was read, when the
+    // other warps have read it too.
+    auto load = [&] {
+        const int st = loads % kStreamStages, j0 = (t0 + loads) * tile_keys;
+        if (!mbar_wait(&empty[st], (loads / kStreamStages & 1) ^ 1, abort_flag, a.err, kErrWaitSmemEmpty)) return;
+        const uint32_t bytes = (uint32_t)min(tile_keys, n - j0) * a.dim * sizeof(T);
+        mbar_arrive_expect_tx(&full[st], 2 * bytes);
+        bulk_load(ring + 2 * st * tile, static_cast<const T *>(a.k) + base + (size_t)j0 * a.dim, bytes, &full[st]);
+        bulk_load(ring + (2 * st + 1) * tile, static_cast<const T *>(a.v) + base + (size_t)j0 * a.dim, bytes, &full[st]);
+        ++loads;
+    };
+    if (threadIdx.x == 0)
+        while (loads < min(kStreamStages, t1 - t0)) load();
+    if (warp < active) {
+        uint64_t q[kGroupRows][2 * kPieces];
 #pragma unroll
-    for (int i = 0; i < kCols; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int t = t0; t < t1; ++t) {
-        const int j0 = t * kKeys;
-        __syncthreads();
-        stage<T, kKeys>(k, static_cast<const T *>(a.k) + base, j0, n, a.dim);
-        stage<T, kKeys>(v, static_cast<const T *>(a.v) + base, j0, n, a.dim);
-        __syncthreads();
-        float s[4], top = -INFINITY;
-        tile_scores(q, k, r, c, a.dim, s);
+        for (int r = 0; r < kGroupRows; ++r) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            s[u] = sees(a, b, row, j0 + c + 8 * u, length) ? s[u] : -INFINITY;
-            top = fmaxf(top, s[u]);
+            for (int i = 0; i < 2 * kPieces; ++i) q[r][i] = o[r][i] = 0;
+            if (row0 + r < a.rows) load_pieces<kWhole, kLanes, kPieces>(q[r], static_cast<const T *>(a.q) + ((size_t)bh * a.rows + row0 + r) * a.dim, c, a.dim);
         }
+        const float threshold = kRescaleThreshold / a.scale_log2;
+        auto pass = [&](const T *k, const T *v, int j0, int count, auto careful) {
+#pragma unroll 1
+            for (int k0 = kw * 2 * kKeys; k0 < count; k0 += key_warps * 2 * kKeys) {
+                float s8[8];
 #pragma unroll
-        for (int x = 1; x < 8; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        const float m_new = fmaxf(m, top), shift = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = exp2f((m - shift) * a.scale_log2);
-        m = m_new;
-        float sum = 0.0f;
+                for (int u = 0; u < 2; ++u) {
+                    uint64_t x[2 * kPieces];
+                    load_pieces<kWhole, kLanes, kPieces>(x, k + (k0 + u * kKeys + g) * a.dim, c, a.dim);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const float e = exp2f((s[u] - shift) * a.scale_log2);
-            p[r * (kKeys + 1) + c + 8 * u] = e;
-            sum += e;
-        }
-        l = l * alpha + sum;  // this thread's keys
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kCols; ++i) o[i].x *= alpha, o[i].y *= alpha, o[i].z *= alpha, o[i].w *= alpha;
-        auto add = [&](int j, float w) {
-#pragma unroll
-            for (int i = 0; i < kCols; ++i)
-                if ((c + 8 * i) * 4 < a.dim) {
-                    const float4 x = *reinterpret_cast<const float4 *>(v + j * q_stride(a.dim) + (c + 8 * i) * 4);
-                    o[i].x = fmaf(w, x.x, o[i].x), o[i].y = fmaf(w, x.y, o[i].y), o[i].z = fmaf(w, x.z, o[i].z), o[i].w = fmaf(w, x.w, o[i].w);
+                    for (int r = 0; r < kGroupRows; ++r) s8[2 * r + u] = dot(q[r], x);
                 }
+                float s = scattered_sum<kLanes>(s8, c);
+                if (careful) s = k0 + my_key < count && sees(a, b, my_row, j0 + k0 + my_key, length) ? s : -INFINITY;
+                const float top = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, kSame));
+                if (__any_sync(0xffffffffu, top > m + threshold)) {
+                    const float m_new = fmaxf(m, top), alpha = exp2f((m - (m_new == -INFINITY ? 0.0f : m_new)) * a.scale_log2);
+                    m = m_new;
+                    l *= alpha;
+#pragma unroll
+                    for (int r = 0; r < kGroupRows; ++r) {
+                        const float f = __shfl_sync(0xffffffffu, alpha, g * kLanes + 2 * r * kSame);
+#pragma unroll
+                        for (int i = 0; i < 2 * kPieces; ++i) o[r][i] = mul2(o[r][i], pack2f(f, f));
+                    }
+                }
+                const float p = exp2f((s - (m == -INFINITY ? 0.0f : m)) * a.scale_log2);
+                l += p;
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    uint64_t x[2 * kPieces];
+                    load_pieces<true, kLanes, kPieces>(x, v + (k0 + u * kKeys + g) * a.dim, c, a.dim);  // columns beyond the head are not written
+#pragma unroll
+                    for (int r = 0; r < kGroupRows; ++r) {
+                        const float w = __shfl_sync(0xffffffffu, p, g * kLanes + (2 * r + u) * kSame);
+                        if (!careful || w != 0.0f)  // drafts: no product with one that the row does not see
+#pragma unroll
+                            for (int i = 0; i < 2 * kPieces; ++i) o[r][i] = fma2(pack2f(w, w), x[i], o[r][i]);
+                    }
+                }
+            }
         };
-        const float *mine = p + r * (kKeys + 1);
-        if (j0 + kKeys <= length) {
-#pragma unroll 4
-            for (int j = 0; j < kKeys; ++j) add(j, mine[j]);
-        } else {  // drafts: no product with one that the row does not see
-            for (int j = 0; j < kKeys; ++j)
-                if (mine[j] != 0.0f) add(j, mine[j]);
+        for (int t = t0; t < t1; ++t) {
+            const int i = t - t0, st = i % kStreamStages, j0 = t * tile_keys, count = min(tile_keys, n - j0);
+            if (threadIdx.x == 0 && i > 0 && t0 + loads < t1) load();
+            if (!mbar_wait_warp(&full[st], i / kStreamStages & 1, abort_flag, a.err, kErrWaitTmaFull)) break;
+            const T *k = ring + 2 * st * tile, *v = k + tile;
+            if (j0 + tile_keys <= length) pass(k, v, j0, count, std::false_type{});
+            else pass(k, v, j0, count, std::true_type{});
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[st]);
         }
+        // the lane groups' maxima and sums, then the scores' of the two keys
+#pragma unroll
+        for (int x = kLanes; x < 32; x <<= 1) {
+            const float m_new = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x)), alpha = exp2f((m - (m_new == -INFINITY ? 0.0f : m_new)) * a.scale_log2);
+            m = m_new;
+            l *= alpha;
+            l += __shfl_xor_sync(0xffffffffu, l, x);
+#pragma unroll
+            for (int r = 0; r < kGroupRows; ++r) {
+                const float f = __shfl_sync(0xffffffffu, alpha, g * kLanes + 2 * r * kSame);
+#pragma unroll
+                for (int i = 0; i < 2 * kPieces; ++i) {
+                    o[r][i] = mul2(o[r][i], pack2f(f, f));
+                    o[r][i] = add2(o[r][i], __shfl_xor_sync(0xffffffffu, o[r][i], x));
+                }
+            }
+        }
+        l += __shfl_xor_sync(0xffffffffu, l, kSame);
     }
+    __syncthreads();  // the ring has been read
+    if (aborted) {
+        if (threadIdx.x == 0)  // copies still in flight land before the block exits
+            for (int i = max(0, loads - kStreamStages); i < loads; ++i) mbar_wait_drain(&full[i % kStreamStages], i / kStreamStages & 1, a.err);
+        return;
+    }
+    // the key warps of a row group, in order: [warp][row][width] sums, [warp][row] maxima and sums
+    constexpr int kWidth = 4 * kLanes * kPieces;
+    float *sums = reinterpret_cast<float *>(ring_smem);
+    float2 *stats = reinterpret_cast<float2 *>(sums + kStreamWarps * kGroupRows * kWidth);
+    if (warp < active) {
 #pragma unroll
-    for (int x = 1; x < 8; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-    if (row >= a.rows) return;
-    const size_t at = ((size_t)bh * a.rows + row) * splits + blockIdx.y;
-    if (c == 0) a.part_ml[at] = make_float2(m, l);
+        for (int r = 0; r < kGroupRows; ++r)
+            if (g == r % kKeys) {
+                if (c == 2 * r * kSame) stats[warp * kGroupRows + r] = make_float2(m, l);
 #pragma unroll
-    for (int i = 0; i < kCols; ++i)
-        if ((c + 8 * i) * 4 < a.dim) *reinterpret_cast<float4 *>(a.part_o + at * a.dim + (c + 8 * i) * 4) = o[i];
+                for (int i = 0; i < kPieces; ++i)
+                    *reinterpret_cast<ulonglong2 *>(sums + (warp * kGroupRows + r) * kWidth + 4 * (c + kLanes * i)) = make_ulonglong2(o[r][2 * i], o[r][2 * i + 1]);
+            }
+    }
+    __syncthreads();
+    const int quads = a.dim / 4, block_rows = min(groups * kGroupRows, a.rows - (int)blockIdx.x * groups * kGroupRows);
+    for (int i = threadIdx.x; i < block_rows * quads; i += kStreamThreads) {
+        const int r = i / quads, d = 4 * (i - r * quads);
+        float top = -INFINITY, sum = 0.0f;
+        for (int w = 0; w < key_warps; ++w) top = fmaxf(top, stats[w * groups * kGroupRows + r].x);
+        const float shift = top == -INFINITY ? 0.0f : top;
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 0; w < key_warps; ++w) {
+            const float2 st = stats[w * groups * kGroupRows + r];
+            const float f = exp2f((st.x - shift) * a.scale_log2);
+            const float4 y = *reinterpret_cast<const float4 *>(sums + (w * groups * kGroupRows + r) * kWidth + d);
+            sum += st.y * f;
+            x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
+        }
+        const size_t out = ((size_t)bh * a.rows + blockIdx.x * groups * kGroupRows + r) * splits + blockIdx.y;
+        if (d == 0) a.part_ml[out] = make_float2(top, sum);
+        *reinterpret_cast<float4 *>(a.part_o + out * a.dim + d) = x;
+    }
 }
 
 // Joins the splits of one row: one warp a row.
@@ -200,292 +312,106 @@ __device__ __forceinline__ void join_rows(const TreeArgs &a, int splits, int tot
     }
 }
 
-// weights[j] += sum over all rows of p_j, p from the rows' joined maximum and sum: a
-// block owns 32 keys of a (sequence, head), walks over the rows 16 at a time and adds
-// the 16 row slots in order.
-template <typename T>
-__device__ __forceinline__ void add_weights(const TreeArgs &a, int splits, int first_tile, int step, int bh, float *smem) {
-    float *q = smem, *k = q + kRows * q_stride(a.dim), *sums = k + kKeys * q_stride(a.dim);
-    const int b = bh / a.kv_heads, r = threadIdx.x >> 3, c = threadIdx.x & 7;
+// weights[j] += sum over all rows of p_j, p from the rows' joined maximum and sum. A block
+// takes the rows 32 at a time from shared memory; a warp holds four keys a lane group in
+// registers and adds their sums in row order.
+constexpr int kWeightRows = 32;
+
+template <typename T, int kLanes, int kPieces>
+__device__ __forceinline__ void add_weights(const TreeArgs &a, int splits, int first, int step, int bh) {
+    constexpr int kKeys = 32 / kLanes, kSame = kLanes / 8, kWidth = 4 * kLanes * kPieces, kUnit = 4 * kKeys;
+    __shared__ __align__(16) float q[kWeightRows * kWidth];
+    __shared__ float2 stats[kWeightRows];  // maximum (0 if the row sees nothing), 1 / sum
+    const int b = bh / a.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / kLanes, c = lane % kLanes, mine = c / kSame;
     const int length = a.lengths[b], n = length + a.seq;
     if (length < 0 || length > a.capacity - a.seq) return;
-    for (int j0 = first_tile * kKeys; j0 < n; j0 += step * kKeys) {
-        float acc[4] = {};
+    const T *k = static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, *queries = static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim;
+    auto stage = [&](int r0) {
         __syncthreads();
-        stage<T, kKeys>(k, static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, j0, n, a.dim);
-        for (int r0 = 0; r0 < a.rows; r0 += kRows) {
-            __syncthreads();
-            stage<T, kRows>(q, static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, r0, a.rows, a.dim);
-            // the row's maximum and sum over its splits, by its 8 threads
-            float m = -INFINITY, l = 0.0f;
-            if (r0 + r < a.rows) {
-                const float2 *ml = a.part_ml + ((size_t)bh * a.rows + r0 + r) * splits;
-                for (int s = c; s < splits; s += 8) m = fmaxf(m, ml[s].x);
-            }
-#pragma unroll
-            for (int x = 1; x < 8; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            const float shift = m == -INFINITY ? 0.0f : m;
-            if (r0 + r < a.rows) {
-                const float2 *ml = a.part_ml + ((size_t)bh * a.rows + r0 + r) * splits;
-                for (int s = c; s < splits; s += 8) l = fmaf(ml[s].y, exp2f((ml[s].x - shift) * a.scale_log2), l);
-            }
-#pragma unroll
-            for (int x = 1; x < 8; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-            __syncthreads();
-            if (r0 + r >= a.rows) continue;
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-            float s[4];
-            tile_scores(q, k, r, c, a.dim, s);
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (sees(a, b, r0 + r, j0 + c + 8 * u, length)) acc[u] += exp2f((s[u] - shift) * a.scale_log2) * inv;
+        for (int i = threadIdx.x; i < kWeightRows * kWidth / 4; i += kStreamThreads) {
+            const int r = i / (kWidth / 4), d = 4 * (i % (kWidth / 4));
+            Four f{0, 0};
+            if (r0 + r < a.rows && d < a.dim) f = four_of(queries + (size_t)(r0 + r) * a.dim + d);
+            *reinterpret_cast<ulonglong2 *>(q + 4 * i) = make_ulonglong2(f.lo, f.hi);
         }
-        __syncthreads();
+        // four threads a row
+        const int row = min(r0 + (int)(threadIdx.x >> 2), a.rows - 1), part = threadIdx.x & 3;
+        const float2 *ml = a.part_ml + ((size_t)bh * a.rows + row) * splits;
+        float m = -INFINITY, l = 0.0f;
+        for (int s = part; s < splits; s += 4) m = fmaxf(m, ml[s].x);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) sums[r * kKeys + c + 8 * u] = acc[u];
+        for (int x = 1; x < 4; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        const float shift = m == -INFINITY ? 0.0f : m;
+        for (int s = part; s < splits; s += 4) l = fmaf(ml[s].y, exp2f((ml[s].x - shift) * a.scale_log2), l);
+#pragma unroll
+        for (int x = 1; x < 4; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
+        if (part == 0) stats[threadIdx.x >> 2] = make_float2(shift, l > 0.0f || l != l ? 1.0f / l : 0.0f);
         __syncthreads();
-        if (threadIdx.x < kKeys && j0 + threadIdx.x < n) {
-            float s = 0.0f;
-            for (int i = 0; i < kRows; ++i) s += sums[i * kKeys + threadIdx.x];
-            a.weights[(size_t)bh * a.capacity + j0 + threadIdx.x] += s;
+    };
+    for (int block = first; block * kStreamWarps * kUnit < n; block += step) {
+        const int key0 = (block * kStreamWarps + warp) * kUnit + (mine & 1) * kKeys + g;  // of this lane's first score, the second 2 kKeys on
+        uint64_t x[4][2 * kPieces];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            load_pieces<false, kLanes, kPieces>(x[u], k + (size_t)min((block * kStreamWarps + warp) * kUnit + u * kKeys + g, n - 1) * a.dim, c, a.dim);
+        float acc[2] = {};
+        for (int r0 = 0; r0 < a.rows; r0 += kWeightRows) {
+            if (block == first || a.rows > kWeightRows) stage(r0);
+            const int rows = min(kWeightRows, a.rows - r0);
+#pragma unroll 1
+            for (int r = 0; r < rows; r += kGroupRows) {
+                float s8[2][8];
+#pragma unroll
+                for (int i = 0; i < kGroupRows; ++i) {
+                    uint64_t y[2 * kPieces];
+                    load_pieces<true, kLanes, kPieces>(y, q + (r + i) * kWidth, c, kWidth);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) s8[u >> 1][2 * i + (u & 1)] = dot(y, x[u]);
+                }
+                const int row = r + (mine >> 1);
+                const float2 st = stats[row];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float s = scattered_sum<kLanes>(s8[h], c);
+                    const int key = key0 + 2 * h * kKeys;
+                    if (row < rows && key < n && sees(a, b, r0 + row, key, length)) acc[h] += exp2f((s - st.x) * a.scale_log2) * st.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 2 * kSame);
+            acc[h] += __shfl_xor_sync(0xffffffffu, acc[h], 4 * kSame);
+            const int key = key0 + 2 * h * kKeys;
+            if (mine < 2 && c % kSame == 0 && key < n) a.weights[(size_t)bh * a.capacity + key] += acc[h];
         }
     }
 }
 
 // Behind the splits: the first join_blocks blocks join rows, the others add weights
 // (which read the splits' maxima and sums themselves, so neither waits for the other).
+template <typename T, int kLanes, int kPieces>
+__global__ void __launch_bounds__(kStreamThreads) tree_finish_kernel(const TreeArgs a, int splits, int total_rows, int join_blocks, int key_blocks) {
+    grid_dependency_wait();
+    if ((int)blockIdx.x < join_blocks) return join_rows<T>(a, splits, total_rows, blockIdx.x);
+    const int i = blockIdx.x - join_blocks, bh = i / key_blocks;
+    add_weights<T, kLanes, kPieces>(a, splits, i - bh * key_blocks, key_blocks, bh);
+}
+
+// The kernels of a head dimension (16-bit types come here above 128 only).
 template <typename T>
-__global__ void __launch_bounds__(kThreads) tree_finish_kernel(const TreeArgs a, int splits, int total_rows, int join_blocks, int key_blocks) {
-    extern __shared__ float smem[];
-    grid_dependency_wait();
-    if ((int)blockIdx.x < join_blocks) return join_rows<T>(a, splits, total_rows, blockIdx.x);
-    const int i = blockIdx.x - join_blocks, bh = i / key_blocks;
-    add_weights<T>(a, splits, i - bh * key_blocks, key_blocks, bh, smem);
+auto kernel_of(int dim) -> void (*)(TreeArgs, int, int, int) {
+    if constexpr (std::is_same<T, float>::value) {
+        if (dim <= 64) return dim == 64 ? tree_stream_kernel<T, 8, 2, true> : tree_stream_kernel<T, 8, 2, false>;
+        if (dim <= 128) return dim == 128 ? tree_stream_kernel<T, 8, 4, true> : tree_stream_kernel<T, 8, 4, false>;
+    }
+    return dim == 256 ? tree_stream_kernel<T, 16, 4, true> : tree_stream_kernel<T, 16, 4, false>;
 }
-
-// ------------------------------------------------------------------ many rows
-// From kWideRows rows on (FP32, 32 sequences and heads of 1,000 to 4,000 keys of 128: 144 us
-// here and 202 on 16-row blocks at 48 rows, 146 and 283 at 64, equal up to 32): 64 rows
-// by 64 keys a block of 256 threads, 4 x 4 scores and 4 rows by kCols x 4 columns of the
-// sums a thread, so that a 16-byte shared-memory read feeds 8 to 11 FFMAs (the 16-row
-// blocks: 3). K and V share a buffer; V is loaded into registers while the scores are
-// formed, the next K while the sums are. Bound by FFMA issue beside shared-memory reads:
-// 512 rows of 128 in FP32 run at about 20 TFLOP/s.
-constexpr int kWideThreads = 256, kWideTile = 64, kWideRows = 33;
-
-template <typename T, int kCols>  // kCols: 64-element columns of a head
-struct WideStage {  // a tile of rows on its way to shared memory: 8 threads a row, 32 rows at a time
-    float4 x[2][2 * kCols];
-    __device__ __forceinline__ void load(const T *src, int first, int limit, int dim) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = first + (threadIdx.x >> 3) + 32 * i;
-#pragma unroll
-            for (int u = 0; u < 2 * kCols; ++u) {
-                const int c = (threadIdx.x & 7) * 4 + 32 * u;
-                x[i][u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (r < limit && c < dim) x[i][u] = load4(src + (size_t)r * dim + c);
-            }
-        }
-    }
-    __device__ __forceinline__ void store(float *dst, int dim) const {
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-            for (int u = 0; u < 2 * kCols; ++u) {
-                const int c = (threadIdx.x & 7) * 4 + 32 * u;
-                if (c < dim) *reinterpret_cast<float4 *>(dst + ((threadIdx.x >> 3) + 32 * i) * q_stride(dim) + c) = x[i][u];
-            }
-    }
-};
-
-// s[i][u]: row 4 ty + i with key tx + 16 u.
-__device__ __forceinline__ void wide_scores(const float *q, const float *k, int dim, float (&s)[4][4]) {
-    const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) s[i][u] = 0.0f;
-#pragma unroll 2
-    for (int d = 0; d < dim; d += 4) {
-        float4 x[4], y[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(q + (4 * ty + i) * q_stride(dim) + d);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) y[u] = *reinterpret_cast<const float4 *>(k + (tx + 16 * u) * q_stride(dim) + d);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) s[i][u] = fmaf(x[i].x, y[u].x, fmaf(x[i].y, y[u].y, fmaf(x[i].z, y[u].z, fmaf(x[i].w, y[u].w, s[i][u]))));
-    }
-}
-
-constexpr int kWideP = kWideTile + 4;  // floats of a row of weights
-
-// grid: (row blocks, splits, batch * kv_heads)
-template <typename T, int kCols>
-__global__ void __launch_bounds__(kWideThreads, kCols == 4 ? 1 : 2) tree_wide_kernel(const TreeArgs a, int splits) {
-    extern __shared__ float smem[];
-    float *q = smem, *kv = q + kWideTile * q_stride(a.dim), *p = kv + kWideTile * q_stride(a.dim);
-    const int bh = blockIdx.z, b = bh / a.kv_heads, ty = threadIdx.x >> 4, tx = threadIdx.x & 15, row0 = blockIdx.x * kWideTile + 4 * ty;
-    const int length = a.lengths[b];
-    if (length < 0 || length > a.capacity - a.seq) {
-        if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrCacheLength);
-        return;
-    }
-    grid_dependency_trigger();
-    const int n = length + a.seq, tiles = (n + kWideTile - 1) / kWideTile;
-    const int t0 = (int)((long long)tiles * blockIdx.y / splits), t1 = (int)((long long)tiles * (blockIdx.y + 1) / splits);
-    const T *k = static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, *v = static_cast<const T *>(a.v) + (size_t)bh * a.capacity * a.dim;
-    WideStage<T, kCols> stage;
-    stage.load(static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, blockIdx.x * kWideTile, a.rows, a.dim);
-    stage.store(q, a.dim);
-    if (t0 < t1) stage.load(k, t0 * kWideTile, n, a.dim);
-    float m[4], l[4];
-    float4 o[4][kCols];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        m[i] = -INFINITY, l[i] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) o[i][c] = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    for (int t = t0; t < t1; ++t) {
-        const int j0 = t * kWideTile;
-        __syncthreads();
-        stage.store(kv, a.dim);
-        stage.load(v, j0, n, a.dim);
-        __syncthreads();
-        float s[4][4];
-        wide_scores(q, kv, a.dim, s);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float top = -INFINITY;
-            if (j0 + kWideTile > length)
-#pragma unroll
-                for (int u = 0; u < 4; ++u) s[i][u] = sees(a, b, row0 + i, j0 + tx + 16 * u, length) ? s[i][u] : -INFINITY;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) top = fmaxf(top, s[i][u]);
-#pragma unroll
-            for (int x = 1; x < 16; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-            const float m_new = fmaxf(m[i], top), shift = m_new == -INFINITY ? 0.0f : m_new;
-            const float alpha = exp2f((m[i] - shift) * a.scale_log2);
-            m[i] = m_new;
-            float sum = 0.0f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const float e = exp2f((s[i][u] - shift) * a.scale_log2);
-                p[(4 * ty + i) * kWideP + tx + 16 * u] = e;
-                sum += e;
-            }
-            l[i] = l[i] * alpha + sum;  // this thread's keys
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) o[i][c].x *= alpha, o[i][c].y *= alpha, o[i][c].z *= alpha, o[i][c].w *= alpha;
-        }
-        __syncthreads();  // K has been read, P is written
-        stage.store(kv, a.dim);
-        if (t + 1 < t1) stage.load(k, j0 + kWideTile, n, a.dim);
-        __syncthreads();
-        auto add = [&](auto careful) {
-#pragma unroll 1
-            for (int j = 0; j < kWideTile; j += 4) {
-                float w[4][4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) *reinterpret_cast<float4 *>(w[i]) = *reinterpret_cast<const float4 *>(p + (4 * ty + i) * kWideP + j);
-#pragma unroll
-                for (int jj = 0; jj < 4; ++jj)
-#pragma unroll
-                    for (int c = 0; c < kCols; ++c)
-                        if (tx * 4 + 64 * c < a.dim) {
-                            const float4 x = *reinterpret_cast<const float4 *>(kv + (j + jj) * q_stride(a.dim) + tx * 4 + 64 * c);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (!careful || w[i][jj] != 0.0f) {
-                                    o[i][c].x = fmaf(w[i][jj], x.x, o[i][c].x), o[i][c].y = fmaf(w[i][jj], x.y, o[i][c].y);
-                                    o[i][c].z = fmaf(w[i][jj], x.z, o[i][c].z), o[i][c].w = fmaf(w[i][jj], x.w, o[i][c].w);
-                                }
-                        }
-            }
-        };
-        if (j0 + kWideTile <= length) add(std::false_type{});
-        else add(std::true_type{});  // drafts: no product with one that the row does not see
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int x = 1; x < 16; x <<= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], x);
-        if (row0 + i >= a.rows) continue;
-        const size_t at = ((size_t)bh * a.rows + row0 + i) * splits + blockIdx.y;
-        if (tx == 0) a.part_ml[at] = make_float2(m[i], l[i]);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c)
-            if (tx * 4 + 64 * c < a.dim) *reinterpret_cast<float4 *>(a.part_o + at * a.dim + tx * 4 + 64 * c) = o[i][c];
-    }
-}
-
-// add_weights for many rows: 64 keys a block, 64 rows at a time.
-template <typename T, int kCols>
-__device__ __forceinline__ void add_weights_wide(const TreeArgs &a, int splits, int first_tile, int step, int bh, float *smem) {
-    float *q = smem, *k = q + kWideTile * q_stride(a.dim), *sums = k + kWideTile * q_stride(a.dim);
-    float2 *stats = reinterpret_cast<float2 *>(sums + 16 * kWideTile);
-    const int b = bh / a.kv_heads, ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-    const int length = a.lengths[b], n = length + a.seq;
-    if (length < 0 || length > a.capacity - a.seq) return;
-    for (int j0 = first_tile * kWideTile; j0 < n; j0 += step * kWideTile) {
-        float acc[4] = {};
-        WideStage<T, kCols> stage;
-        stage.load(static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, j0, n, a.dim);
-        __syncthreads();
-        stage.store(k, a.dim);
-        for (int r0 = 0; r0 < a.rows; r0 += kWideTile) {
-            stage.load(static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim, r0, a.rows, a.dim);
-            __syncthreads();
-            stage.store(q, a.dim);
-            {  // a row's maximum and 1 / sum over its splits, by four threads
-                const int row = r0 + (threadIdx.x >> 2), part = threadIdx.x & 3;
-                const float2 *ml = a.part_ml + ((size_t)bh * a.rows + min(row, a.rows - 1)) * splits;
-                float m = -INFINITY, l = 0.0f;
-                for (int s = part; s < splits; s += 4) m = fmaxf(m, ml[s].x);
-#pragma unroll
-                for (int x = 1; x < 4; x <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-                const float shift = m == -INFINITY ? 0.0f : m;
-                for (int s = part; s < splits; s += 4) l = fmaf(ml[s].y, exp2f((ml[s].x - shift) * a.scale_log2), l);
-#pragma unroll
-                for (int x = 1; x < 4; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-                if (part == 0) stats[threadIdx.x >> 2] = make_float2(shift, row < a.rows && (l > 0.0f || l != l) ? 1.0f / l : 0.0f);
-            }
-            __syncthreads();
-            float s[4][4];
-            wide_scores(q, k, a.dim, s);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int row = r0 + 4 * ty + i;
-                const float2 st = stats[4 * ty + i];
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    if (row < a.rows && sees(a, b, row, j0 + tx + 16 * u, length)) acc[u] += exp2f((s[i][u] - st.x) * a.scale_log2) * st.y;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < 4; ++u) sums[ty * kWideTile + tx + 16 * u] = acc[u];
-        __syncthreads();
-        if (threadIdx.x < kWideTile && j0 + threadIdx.x < n) {
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) s += sums[i * kWideTile + threadIdx.x];
-            a.weights[(size_t)bh * a.capacity + j0 + threadIdx.x] += s;
-        }
-    }
-}
-
-template <typename T, int kCols>
-__global__ void __launch_bounds__(kWideThreads, kCols == 4 ? 1 : 2)
-    tree_finish_wide_kernel(const TreeArgs a, int splits, int total_rows, int join_blocks, int key_blocks) {
-    extern __shared__ float smem[];
-    grid_dependency_wait();
-    if ((int)blockIdx.x < join_blocks) return join_rows<T>(a, splits, total_rows, blockIdx.x);
-    const int i = blockIdx.x - join_blocks, bh = i / key_blocks;
-    add_weights_wide<T, kCols>(a, splits, i - bh * key_blocks, key_blocks, bh, smem);
+template <typename T>
+auto finish_of(int dim) -> void (*)(TreeArgs, int, int, int, int) {
+    if constexpr (std::is_same<T, float>::value)
+        if (dim <= 128) return dim <= 64 ? tree_finish_kernel<T, 8, 2> : tree_finish_kernel<T, 8, 4>;
+    return tree_finish_kernel<T, 16, 4>;
 }
 
 template <typename T>
@@ -493,39 +419,33 @@ LaunchFn simt_launch(Context *ctx, const Spec &s) {
     TreeArgs base = tree_args(ctx, s);
     const int heads = (int)(s.batch * s.kv_heads), rows = base.rows, total_rows = heads * rows;
     if (heads > 65535) throw IrError("attention_tree: batch * kv_heads must be at most 65535");
-    const bool wide = rows >= kWideRows;
-    const int tile_rows = wide ? kWideTile : kRows, tile_keys = wide ? kWideTile : kKeys, threads = wide ? kWideThreads : kThreads;
-    const int row_blocks = (rows + tile_rows - 1) / tile_rows;
-    // about four blocks per SM
+    // blocks of up to four row groups, dealt evenly; tiles of 32 KB of K and V
+    const int row_groups = (rows + kGroupRows - 1) / kGroupRows, row_blocks = (row_groups + kStreamWarps - 1) / kStreamWarps;
+    const int groups = (row_groups + row_blocks - 1) / row_blocks, tile_keys = s.dim * sizeof(T) <= 512 ? 32 : 16;
+    // four blocks per SM at most, two whole waves. Fewer and longer ones leave mixed lengths
+    // unbalanced (64 heads of 1,000 to 8,000 keys: 62 us with four per SM, 74 with two, 69
+    // with six), more cost partial results.
     const long long items = (long long)heads * row_blocks;
-    const int splits = (int)std::max<long long>(1, std::min<long long>({(4ll * ctx->sm_count + items - 1) / items, ((long long)s.capacity + tile_keys - 1) / tile_keys,
-                                                                        (long long)kMaxSplits}));
+    const int splits = (int)std::max<long long>(1, std::min<long long>({4ll * ctx->sm_count / items, ((long long)s.capacity + tile_keys - 1) / tile_keys, (long long)kMaxSplits}));
     const size_t parts = (size_t)total_rows * splits;
     auto ws = kernel_workspace(parts * (s.dim * sizeof(float) + sizeof(float2)), "attention_tree partial results");
     base.part_o = static_cast<float *>(ws.get());  // rows of a multiple of 32 bytes: read as 16-byte vectors
     base.part_ml = reinterpret_cast<float2 *>(base.part_o + parts * s.dim);
-    const size_t row = (size_t)q_stride(s.dim) * 4;
-    const size_t smem = wide ? 2 * kWideTile * row + kWideTile * kWideP * 4 : (kRows + 2 * kKeys) * row + kRows * (kKeys + 1) * 4;
-    const size_t smem_w = !s.weights ? 0 : wide ? 2 * kWideTile * row + 16 * kWideTile * 4 + kWideTile * 8 : (kRows + kKeys) * row + kRows * kKeys * 4;
-    void (*kernel)(TreeArgs, int);
-    void (*finish)(TreeArgs, int, int, int, int);
-    if (wide) {
-        kernel = s.dim <= 64 ? tree_wide_kernel<T, 1> : s.dim <= 128 ? tree_wide_kernel<T, 2> : tree_wide_kernel<T, 4>;
-        finish = s.dim <= 64 ? tree_finish_wide_kernel<T, 1> : s.dim <= 128 ? tree_finish_wide_kernel<T, 2> : tree_finish_wide_kernel<T, 4>;
-    } else {
-        kernel = s.dim <= 64 ? tree_simt_kernel<T, 2> : s.dim <= 128 ? tree_simt_kernel<T, 4> : tree_simt_kernel<T, 8>;
-        finish = tree_finish_kernel<T>;
-    }
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
-        cudaFuncSetAttribute(finish, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_w) != cudaSuccess)
+    const int width = s.dim <= 64 ? 64 : s.dim <= 128 ? 128 : 256;
+    const size_t joined = kStreamWarps * kGroupRows * (width * sizeof(float) + sizeof(float2));
+    const size_t smem = std::max(2 * kStreamStages * tile_keys * s.dim * sizeof(T) + kStreamPad, joined);
+    const auto kernel = kernel_of<T>(s.dim);
+    const auto finish = finish_of<T>(s.dim);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         throw IrError("cannot reserve shared memory for attention_tree");
     const bool weights = s.weights;
-    const int key_blocks = (int)std::min<long long>((s.capacity + tile_keys - 1) / tile_keys, std::max<long long>(1, 8ll * ctx->sm_count / heads));
-    const int join_blocks = (total_rows + threads / 32 - 1) / (threads / 32);
+    const int unit = width > 128 ? 32 : 64;  // keys of a block of the weights' pass
+    const int key_blocks = (int)std::min<long long>((s.capacity + unit - 1) / unit, std::max<long long>(1, 8ll * ctx->sm_count / heads));
+    const int join_blocks = (total_rows + kStreamWarps - 1) / kStreamWarps;
     return [=, keep = ws](cudaStream_t st, void **b) {
         const TreeArgs a = tree_bind(base, b, weights);
-        kernel<<<dim3(row_blocks, splits, heads), threads, smem, st>>>(a, splits);
-        const cudaError_t e = launch_after(st, finish, dim3(join_blocks + (weights ? key_blocks * heads : 0)), threads, smem_w, a, splits, total_rows,
+        kernel<<<dim3(row_blocks, splits, heads), kStreamThreads, smem, st>>>(a, splits, groups, tile_keys);
+        const cudaError_t e = launch_after(st, finish, dim3(join_blocks + (weights ? key_blocks * heads : 0)), kStreamThreads, 0, a, splits, total_rows,
                                            join_blocks, key_blocks);
         return e == cudaSuccess ? cudaGetLastError() : e;
     };

@@ -143,11 +143,6 @@ struct Row {  // a lane's share of a head
     }
 };
 
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
 __device__ __forceinline__ uint64_t both(float x) { return pack2f(x, x); }
 
 // FP32 tables in shared memory, read 8 in a row by a lane (two 16-byte loads) without
