@@ -29,7 +29,8 @@
 // only, so that enough warps are resident. No block barrier per token, so that warps
 // drift apart and memory stays busy. Measured on B200, BF16, 4 x 2048 tokens of 16 + 2 x 16
 // heads of 128 (201 MB moved; a plain copy of them takes 36 us): 42 us = 4.7 TB/s with
-// halves, 52 with neighbours; the gradient (268 MB) 64 us = 4.2 TB/s. One token: 4.2 us.
+// halves, 52 with neighbours, 62 with halves whose length is no multiple of 8; the gradient
+// (268 MB) 64 us = 4.2 TB/s. One token: 4.2 us.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -154,6 +155,12 @@ __device__ __forceinline__ void table8(const float *table, int first, uint64_t *
     v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
 }
 
+// A row's elements in shared memory (kGeneral): lanes write and read 16 in a row each,
+// 17 words apart, so that no two meet in a bank (all rows of 16 words apart would: a
+// forward pass of 201 MB took 88 us so).
+__device__ __forceinline__ int row_at(int e) { return e + (e >> 4); }
+constexpr int kZeroAt = 16;  // between two lanes' elements: 0
+
 struct Elements {
     uint64_t v[8];
     template <typename T>
@@ -173,13 +180,13 @@ struct Elements {
 
 // The token's cosines and sines, formed by the warp in its shared memory as the
 // pairing multiplies them; kBack turns back.
-//   kNeighbours  x' = x a + (x with its pairs swapped) b: a = c c .., b = -s s ..
-//   else         a = c, b = s, n = -s of each pair
+//   kHalves  a = c, b = s, n = -s of each pair
+//   else     x' = x a + (x with its pairs swapped) b, of each element: a = c, b = -s or s
 template <int kLanes, Pairing kPair, bool kBack>
 struct Turn {
     float *a, *b, *n;
     __device__ __forceinline__ explicit Turn(float *tables) : a(tables), b(tables + kTable), n(tables + 2 * kTable) {}
-    static constexpr int kFloats = (kPair == kNeighbours ? 2 : 3) * kTable;
+    static constexpr int kFloats = (kPair == kHalves ? 3 : 2) * kTable;
     __device__ __forceinline__ void form(const RopeArgs &args, int position, int lane) {
         __syncwarp();  // the last token's have been read
         for (int i = lane; i < 8 * kLanes; i += 32) {
@@ -192,15 +199,21 @@ struct Turn {
             if constexpr (kPair == kNeighbours) {
                 *reinterpret_cast<float2 *>(a + table_at(2 * i)) = make_float2(c, c);
                 *reinterpret_cast<float2 *>(b + table_at(2 * i)) = make_float2(-s, s);
-            } else {
+            } else if constexpr (kPair == kHalves) {
                 a[table_at(i)] = c, b[table_at(i)] = s, n[table_at(i)] = -s;
+            } else {  // i beyond the pairs: two of the elements that pass
+                const int half = args.rotary / 2, e = i < half ? i : 2 * i, pair = i < half ? i + half : 2 * i + 1;
+                a[table_at(e)] = c, b[table_at(e)] = -s, a[table_at(pair)] = c, b[table_at(pair)] = s;
             }
         }
         __syncwarp();
     }
-    // row: the row's elements in shared memory (kGeneral)
-    __device__ __forceinline__ void apply(Elements &x, float *row, int chunk, int half) const {
+    // row, partners (kGeneral): the row's elements in shared memory, and where each
+    // element's partner lies there. Elements that pass are not touched: a partner's
+    // infinity times 0 would reach them.
+    __device__ __forceinline__ void apply(Elements &x, float *row, const int *partners, int chunk, int rotary) const {
         if constexpr (kPair == kHalves) {
+            if (16 * chunk >= rotary) return;
             uint64_t c[4], s[4], m[4];
             table8(a, 8 * chunk, c), table8(b, 8 * chunk, s), table8(n, 8 * chunk, m);
 #pragma unroll
@@ -216,7 +229,7 @@ struct Turn {
             for (int i = 0; i < 8; ++i) {
                 float p, q;
                 unpack2f(x.v[i], p, q);
-                x.v[i] = fma2(x.v[i], c[i], mul2(pack2f(q, p), s[i]));
+                if (16 * chunk + 2 * i < rotary) x.v[i] = fma2(x.v[i], c[i], mul2(pack2f(q, p), s[i]));
             }
         } else {
             float y[16];
@@ -224,20 +237,28 @@ struct Turn {
             for (int i = 0; i < 8; ++i) unpack2f(x.v[i], y[2 * i], y[2 * i + 1]);
             __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) row[16 * chunk + i] = y[i];
+            for (int i = 0; i < 16; ++i) row[row_at(16 * chunk) + i] = y[i];
             __syncwarp();
+            uint64_t c[8], s[8];
+            table8(a, 16 * chunk, c), table8(a, 16 * chunk + 8, c + 4), table8(b, 16 * chunk, s), table8(b, 16 * chunk + 8, s + 4);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int e = 16 * chunk + i;
-                if (e >= 2 * half) continue;
-                const int pair = table_at(e < half ? e : e - half);
-                y[i] = y[i] * a[pair] + (e < half ? n : b)[pair] * row[e < half ? e + half : e - half];
+            for (int i = 0; i < 4; ++i) {
+                const int4 at = *reinterpret_cast<const int4 *>(partners + table_at(16 * chunk + 4 * i));
+                x.v[2 * i] = fma2(x.v[2 * i], c[2 * i], mul2(pack2f(row[at.x], row[at.y]), s[2 * i]));
+                x.v[2 * i + 1] = fma2(x.v[2 * i + 1], c[2 * i + 1], mul2(pack2f(row[at.z], row[at.w]), s[2 * i + 1]));
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x.v[i] = pack2f(y[2 * i], y[2 * i + 1]);
         }
     }
 };
+
+// Where each element's partner lies in a row; a zero for those that pass (whole block; a
+// barrier is due before its use).
+__device__ __forceinline__ void partner_table(const RopeArgs &a, int *partners) {
+    for (int e = threadIdx.x; e < kTable; e += kThreads) {
+        const int half = a.rotary / 2;
+        partners[table_at(e)] = e < 2 * half ? row_at(e < half ? e + half : e - half) : kZeroAt;
+    }
+}
 
 // The norm weights of queries and keys as tables (whole block; a barrier is due before their use).
 template <typename T>
@@ -285,13 +306,18 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
     constexpr int kAhead = 2;  // rounds worked on, and as many loading
     __shared__ __align__(16) float tables[kWarps][Turn<kLanes, kPair, false>::kFloats];
     __shared__ __align__(16) float weights[2][kTable];
-    __shared__ float shared_rows[kPair == kGeneral ? kWarps : 1][512];
+    __shared__ float shared_rows[kPair == kGeneral ? kWarps : 1][32 * 17];
+    __shared__ __align__(16) int partners[kPair == kGeneral ? kTable : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
     const Place at = lane_place<kPair>(chunk, a.dim, a.rotary);
     const Rounds<kLanes> rounds(a);
-    float *row = shared_rows[kPair == kGeneral ? warp : 0] + sub * (kLanes * 16);
+    float *row = shared_rows[kPair == kGeneral ? warp : 0] + sub * (kLanes * 17);
     Turn<kLanes, kPair, false> turn(tables[warp]);
     weight_tables<T>(a, weights);
+    if constexpr (kPair == kGeneral) {
+        partner_table(a, partners);
+        if (chunk == 0) row[kZeroAt] = 0.0f;
+    }
     __syncthreads();
     const int item = blockIdx.x * kWarps + warp;
     if (item >= a.batch * a.seq * a.parts) return;
@@ -339,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
 #pragma unroll
                     for (int i = 0; i < 8; ++i) y.v[i] = mul2(mul2(y.v[i], scale), w.v[i]);
                 }
-                turn.apply(y, row, chunk, a.rotary / 2);
+                turn.apply(y, row, partners, chunk, a.rotary);
                 y.to(x[u]);
             }
             x[u].store(kind == 0 ? q + h * q_step : static_cast<T *>(kind == 1 ? a.k : a.v) + slot + h * kv_step, at, on);
@@ -354,14 +380,19 @@ __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a
     constexpr int kAhead = 2;
     __shared__ __align__(16) float tables[kWarps][Turn<kLanes, kPair, true>::kFloats];
     __shared__ __align__(16) float weights[2][kTable];
-    __shared__ float shared_rows[kWarps][kPair == kGeneral ? 512 : kTable];
+    __shared__ float shared_rows[kWarps][kPair == kGeneral ? 32 * 17 : kTable];
+    __shared__ __align__(16) int partners[kPair == kGeneral ? kTable : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, sub = lane / kLanes, chunk = lane % kLanes;
     const Place at = lane_place<kPair>(chunk, a.dim, a.rotary);
     const Rounds<kLanes> rounds(a);
-    float *row = shared_rows[warp] + (kPair == kGeneral ? sub * (kLanes * 16) : 0);
+    float *row = shared_rows[warp] + (kPair == kGeneral ? sub * (kLanes * 17) : 0);
     const int q_step = a.seq * a.dim;
     Turn<kLanes, kPair, true> turn(tables[warp]);
     weight_tables<T>(a, weights);
+    if constexpr (kPair == kGeneral) {
+        partner_table(a, partners);
+        if (chunk == 0) row[kZeroAt] = 0.0f;
+    }
     __syncthreads();
     Elements dwq, dwk;
 #pragma unroll
@@ -395,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a
                 if (r + u < rounds.k) {
                     Elements d;
                     d.from(g[u]);
-                    turn.apply(d, row, chunk, a.rotary / 2);
+                    turn.apply(d, row, partners, chunk, a.rotary);
                     if (a.norm) {
                         const int kind = r + u < rounds.q ? 0 : 1;
                         Elements y;

@@ -128,6 +128,27 @@ def test_rope_carries_nan_and_infinity_in_their_own_rows_only(rt):
         np.testing.assert_array_equal(a, b)
 
 
+@pytest.mark.parametrize("op", ["qk_norm_rope", "qk_norm_rope_grad"])
+@pytest.mark.parametrize("rotary, interleaved", [(32, False), (20, False), (20, True), (32, True), (2, False), (2, True), (0, False)])
+def test_rope_passes_infinities_beside_what_turns(rt, op, rotary, interleaved):
+    # without norms an element that does not turn is copied, whatever it is, and reaches no other
+    spec = rope_spec(dict(batch=1, seq=3, heads=2, kv_heads=1, dim=56, rotary=rotary, interleaved=interleaved, norm=False), "fp32", op)
+    x = rope_inputs(spec, 7) if op == "qk_norm_rope" else grad_inputs(spec, 7)
+    name, out = ("qkv", "q") if op == "qk_norm_rope" else ("dq", "dqkv")
+    clean = R.run(rt, spec, x)[out].copy()
+    bad = [rotary, rotary + 5, 55]
+    x[name] = x[name].copy()
+    rows = x[name][:, :, :2] if op == "qk_norm_rope" else x[name]  # of queries
+    rows[..., bad] = [np.inf, np.nan, -np.inf]
+    got = R.run(rt, spec, x)[out].copy()
+    heads = (2, 3, 56) if op == "qk_norm_rope" else (3, 4, 56)
+    got, clean = got.reshape(heads), clean.reshape(heads)
+    queries = got if op == "qk_norm_rope" else got[:, :2]
+    np.testing.assert_array_equal(queries[..., bad], np.broadcast_to(np.float32([np.inf, np.nan, -np.inf]), queries[..., bad].shape))
+    queries[..., bad] = (clean if op == "qk_norm_rope" else clean[:, :2])[..., bad]
+    np.testing.assert_array_equal(got, clean)
+
+
 def rope_gradient(spec, x):
     """The formula's gradients and their magnitudes: dqkv, and dq_weight, dk_weight."""
     H, Hk = spec["heads"], spec["kv_heads"]
