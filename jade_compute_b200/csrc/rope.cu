@@ -29,8 +29,9 @@
 // only, so that enough warps are resident. No block barrier per token, so that warps
 // drift apart and memory stays busy. Measured on B200, BF16, 4 x 2048 tokens of 16 + 2 x 16
 // heads of 128 (201 MB moved; a plain copy of them takes 36 us): 42 us = 4.7 TB/s with
-// halves, 52 with neighbours, 62 with halves whose length is no multiple of 8; the gradient
-// (268 MB) 64 us = 4.2 TB/s. One token: 4.2 us.
+// halves, 44 with neighbours, 51 with a rotary that is no multiple of 16; the gradient (268
+// MB) 58, 58 and 66 us = 4.7 TB/s (64 with each step's rows loaded to registers and waited
+// for). One token: 4.2 us.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -60,8 +61,8 @@ struct RopeArgs {
 
 // How a lane's 16 elements, two pieces of 8, lie in the head and find their partners.
 //   kHalves      rotated lanes hold 8 of the first half and their 8 partners of the
-//                second, rotary / 2 apart (rotary a multiple of 16); the others 16 in
-//                a row
+//                second, rotary / 2 apart (rotary a multiple of 16); the others the
+//                same of the rest
 //   kNeighbours  16 in a row, partners beside each other
 //   kGeneral     16 in a row, partners through the warp's rows in shared memory
 //                (halves of any length)
@@ -74,7 +75,12 @@ struct Place {
 template <Pairing kPair>
 __device__ __forceinline__ Place lane_place(int chunk, int dim, int rotary) {
     Place at{16 * chunk, 16 * chunk + 8, 16 * chunk < dim, 16 * chunk + 8 < dim};
-    if (kPair == kHalves && 16 * chunk < rotary) at.lo = 8 * chunk, at.hi = 8 * chunk + rotary / 2, at.has_hi = true;
+    if (kPair == kHalves) {
+        const bool turns = 16 * chunk < rotary;
+        const int i = turns ? chunk : chunk - rotary / 16, lanes = turns ? rotary / 16 : ((dim - rotary) / 8 + 1) / 2;
+        at.lo = (turns ? 0 : rotary) + 8 * i, at.hi = at.lo + 8 * lanes;
+        at.has_lo = i < lanes, at.has_hi = at.has_lo && at.hi < dim;
+    }
     return at;
 }
 
@@ -144,14 +150,50 @@ struct Row {  // a lane's share of a head
     }
 };
 
+// A round's rows on their way through shared memory, in units of 16 bytes that leave
+// memory in whole sectors. kHalves: every lane copies its own pieces (its neighbours'
+// lie beside them). Else the lanes of a row copy its units in turn, and lane c takes
+// units kUnits c ..; unit n is kept at n ^ (n / 8 mod kUnits), clear of bank conflicts.
+template <typename T, int kLanes, Pairing kPair>
+struct Staged {
+    static constexpr int kUnits = 2 * sizeof(Piece<T>) / 16, kEach = 16 / sizeof(T);
+    static __device__ __forceinline__ int place(int lane, int i) {
+        if (kPair == kHalves) return 32 * i + lane;
+        const int n = kUnits * (lane % kLanes) + i;
+        return lane / kLanes * (kLanes * kUnits) + (n ^ (n >> 3 & (kUnits - 1)));
+    }
+    static __device__ __forceinline__ void copy(uint4 *to, const T *p, const Place &at, bool on, int lane, int dim) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+            const int n = lane % kLanes + kLanes * i, hi = i >= kUnits / 2;
+            const bool has = on && (kPair == kHalves ? (hi ? at.has_hi : at.has_lo) : n * kEach < dim);
+            const int from = kPair == kHalves ? (hi ? at.hi : at.lo) + i % (kUnits / 2) * kEach : n * kEach;
+            const int slot = kPair == kHalves ? 32 * i + lane : lane / kLanes * (kLanes * kUnits) + (n ^ (n >> 3 & (kUnits - 1)));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to + slot)), "l"(p + (has ? from : 0)), "r"(has ? 16 : 0) : "memory");
+        }
+    }
+    static __device__ __forceinline__ Row<T> take(const uint4 *from, int lane) {
+        uint4 x[kUnits];
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) x[i] = from[place(lane, i)];
+        return {*reinterpret_cast<const Piece<T> *>(&x[0]), *reinterpret_cast<const Piece<T> *>(&x[kUnits / 2])};
+    }
+};
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait_but_one() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
 __device__ __forceinline__ uint64_t both(float x) { return pack2f(x, x); }
 
-// FP32 tables in shared memory, read 8 in a row by a lane (two 16-byte loads) without
-// bank conflicts: entry e lies at table_at(e).
+// FP32 tables in shared memory without bank conflicts: entry e lies at table_at(e). Lanes
+// read 8 in a row (kHalves: two 16-byte loads) or 16 (four).
 constexpr int kTable = 256;
-__device__ __forceinline__ int table_at(int e) { return (e >> 2 & 1) * (kTable / 2) + (e >> 3) * 4 + (e & 3); }
+template <Pairing kPair>
+__device__ __forceinline__ int table_at(int e) {
+    return kPair == kHalves ? (e >> 2 & 1) * (kTable / 2) + (e >> 3) * 4 + (e & 3) : (e >> 2 & 3) * (kTable / 4) + (e >> 4) * 4 + (e & 3);
+}
+template <Pairing kPair>
 __device__ __forceinline__ void table8(const float *table, int first, uint64_t *v) {
-    const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(table + first / 2), b = *reinterpret_cast<const ulonglong2 *>(table + kTable / 2 + first / 2);
+    const ulonglong2 a = *reinterpret_cast<const ulonglong2 *>(table + table_at<kPair>(first)), b = *reinterpret_cast<const ulonglong2 *>(table + table_at<kPair>(first + 4));
     v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
 }
 
@@ -197,13 +239,13 @@ struct Turn {
                 c *= args.gain, s *= kBack ? -args.gain : args.gain;
             }
             if constexpr (kPair == kNeighbours) {
-                *reinterpret_cast<float2 *>(a + table_at(2 * i)) = make_float2(c, c);
-                *reinterpret_cast<float2 *>(b + table_at(2 * i)) = make_float2(-s, s);
+                *reinterpret_cast<float2 *>(a + table_at<kPair>(2 * i)) = make_float2(c, c);
+                *reinterpret_cast<float2 *>(b + table_at<kPair>(2 * i)) = make_float2(-s, s);
             } else if constexpr (kPair == kHalves) {
-                a[table_at(i)] = c, b[table_at(i)] = s, n[table_at(i)] = -s;
+                a[table_at<kPair>(i)] = c, b[table_at<kPair>(i)] = s, n[table_at<kPair>(i)] = -s;
             } else {  // i beyond the pairs: two of the elements that pass
                 const int half = args.rotary / 2, e = i < half ? i : 2 * i, pair = i < half ? i + half : 2 * i + 1;
-                a[table_at(e)] = c, b[table_at(e)] = -s, a[table_at(pair)] = c, b[table_at(pair)] = s;
+                a[table_at<kPair>(e)] = c, b[table_at<kPair>(e)] = -s, a[table_at<kPair>(pair)] = c, b[table_at<kPair>(pair)] = s;
             }
         }
         __syncwarp();
@@ -215,7 +257,7 @@ struct Turn {
         if constexpr (kPair == kHalves) {
             if (16 * chunk >= rotary) return;
             uint64_t c[4], s[4], m[4];
-            table8(a, 8 * chunk, c), table8(b, 8 * chunk, s), table8(n, 8 * chunk, m);
+            table8<kPair>(a, 8 * chunk, c), table8<kPair>(b, 8 * chunk, s), table8<kPair>(n, 8 * chunk, m);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint64_t lo = x.v[i], hi = x.v[4 + i];
@@ -224,7 +266,7 @@ struct Turn {
             }
         } else if constexpr (kPair == kNeighbours) {
             uint64_t c[8], s[8];
-            table8(a, 16 * chunk, c), table8(a, 16 * chunk + 8, c + 4), table8(b, 16 * chunk, s), table8(b, 16 * chunk + 8, s + 4);
+            table8<kPair>(a, 16 * chunk, c), table8<kPair>(a, 16 * chunk + 8, c + 4), table8<kPair>(b, 16 * chunk, s), table8<kPair>(b, 16 * chunk + 8, s + 4);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 float p, q;
@@ -240,10 +282,10 @@ struct Turn {
             for (int i = 0; i < 16; ++i) row[row_at(16 * chunk) + i] = y[i];
             __syncwarp();
             uint64_t c[8], s[8];
-            table8(a, 16 * chunk, c), table8(a, 16 * chunk + 8, c + 4), table8(b, 16 * chunk, s), table8(b, 16 * chunk + 8, s + 4);
+            table8<kPair>(a, 16 * chunk, c), table8<kPair>(a, 16 * chunk + 8, c + 4), table8<kPair>(b, 16 * chunk, s), table8<kPair>(b, 16 * chunk + 8, s + 4);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int4 at = *reinterpret_cast<const int4 *>(partners + table_at(16 * chunk + 4 * i));
+                const int4 at = *reinterpret_cast<const int4 *>(partners + table_at<kPair>(16 * chunk + 4 * i));
                 x.v[2 * i] = fma2(x.v[2 * i], c[2 * i], mul2(pack2f(row[at.x], row[at.y]), s[2 * i]));
                 x.v[2 * i + 1] = fma2(x.v[2 * i + 1], c[2 * i + 1], mul2(pack2f(row[at.z], row[at.w]), s[2 * i + 1]));
             }
@@ -253,25 +295,27 @@ struct Turn {
 
 // Where each element's partner lies in a row; a zero for those that pass (whole block; a
 // barrier is due before its use).
+template <Pairing kPair>
 __device__ __forceinline__ void partner_table(const RopeArgs &a, int *partners) {
     for (int e = threadIdx.x; e < kTable; e += kThreads) {
         const int half = a.rotary / 2;
-        partners[table_at(e)] = e < 2 * half ? row_at(e < half ? e + half : e - half) : kZeroAt;
+        partners[table_at<kPair>(e)] = e < 2 * half ? row_at(e < half ? e + half : e - half) : kZeroAt;
     }
 }
 
 // The norm weights of queries and keys as tables (whole block; a barrier is due before their use).
-template <typename T>
+template <typename T, Pairing kPair>
 __device__ __forceinline__ void weight_tables(const RopeArgs &a, float (*w)[kTable]) {
     if (!a.norm) return;
     for (int e = threadIdx.x; e < kTable; e += kThreads) {  // 0 beyond the head: lanes read whole pieces
-        w[0][table_at(e)] = e < a.dim ? to_f32<T>(static_cast<const T *>(a.q_weight)[e]) : 0.0f;
-        w[1][table_at(e)] = e < a.dim ? to_f32<T>(static_cast<const T *>(a.k_weight)[e]) : 0.0f;
+        w[0][table_at<kPair>(e)] = e < a.dim ? to_f32<T>(static_cast<const T *>(a.q_weight)[e]) : 0.0f;
+        w[1][table_at<kPair>(e)] = e < a.dim ? to_f32<T>(static_cast<const T *>(a.k_weight)[e]) : 0.0f;
     }
 }
+template <Pairing kPair>
 __device__ __forceinline__ void load_weights(Elements &w, const float *table, const Place &at) {
-    table8(table, at.lo, w.v);
-    table8(table, at.hi & (kTable - 1), w.v + 4);  // a piece that the head lacks is not stored
+    table8<kPair>(table, at.lo, w.v);
+    table8<kPair>(table, at.hi & (kTable - 1), w.v + 4);  // a piece that the head lacks is not stored
 }
 
 // Sum over the kLanes lanes of a row.
@@ -313,9 +357,9 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
     const Rounds<kLanes> rounds(a);
     float *row = shared_rows[kPair == kGeneral ? warp : 0] + sub * (kLanes * 17);
     Turn<kLanes, kPair, false> turn(tables[warp]);
-    weight_tables<T>(a, weights);
+    weight_tables<T, kPair>(a, weights);
     if constexpr (kPair == kGeneral) {
-        partner_table(a, partners);
+        partner_table<kPair>(a, partners);
         if (chunk == 0) row[kZeroAt] = 0.0f;
     }
     __syncthreads();
@@ -360,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
                 y.from(x[u]);
                 if (a.norm) {
                     Elements w;
-                    load_weights(w, weights[kind], at);
+                    load_weights<kPair>(w, weights[kind], at);
                     const uint64_t scale = both(rsqrtf(fmaf(row_sum<kLanes>(y.dot(y)), a.inv_dim, a.epsilon)));
 #pragma unroll
                     for (int i = 0; i < 8; ++i) y.v[i] = mul2(mul2(y.v[i], scale), w.v[i]);
@@ -374,10 +418,16 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
 }
 
 // A persistent warp walks over items (a token, a part of its heads) and keeps its sums
-// of the weights' gradients.
+// of the weights' gradients. While it works on a step's rows, each lane's pieces of the
+// next step's, of the next item's where this one ends, come by asynchronous copies.
+constexpr int kStepUnits = 8;  // 16-byte pieces of a lane and step
+constexpr int kGradStaged = kWarps * 2 * kStepUnits * 32 * 16;
+
 template <typename T, int kLanes, Pairing kPair>
 __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a) {
-    constexpr int kAhead = 2;
+    using Stage = Staged<T, kLanes, kPair>;
+    constexpr int kUnits = Stage::kUnits, kStep = kStepUnits / (2 * kUnits);  // rounds of a step
+    extern __shared__ uint4 staged[];
     __shared__ __align__(16) float tables[kWarps][Turn<kLanes, kPair, true>::kFloats];
     __shared__ __align__(16) float weights[2][kTable];
     __shared__ float shared_rows[kWarps][kPair == kGeneral ? 32 * 17 : kTable];
@@ -388,9 +438,9 @@ __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a
     float *row = shared_rows[warp] + (kPair == kGeneral ? sub * (kLanes * 17) : 0);
     const int q_step = a.seq * a.dim;
     Turn<kLanes, kPair, true> turn(tables[warp]);
-    weight_tables<T>(a, weights);
+    weight_tables<T, kPair>(a, weights);
     if constexpr (kPair == kGeneral) {
-        partner_table(a, partners);
+        partner_table<kPair>(a, partners);
         if (chunk == 0) row[kZeroAt] = 0.0f;
     }
     __syncthreads();
@@ -398,63 +448,83 @@ __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a
 #pragma unroll
     for (int i = 0; i < 8; ++i) dwq.v[i] = dwk.v[i] = 0;
     const int items = a.batch * a.seq * a.parts;
-    for (int item = blockIdx.x * kWarps + warp; item < items; item += gridDim.x * kWarps) {
+    // the next step: its item, rounds r .. of r1, and the rows of its token
+    int item = blockIdx.x * kWarps + warp, r = 0, r1 = 0, position = 0, stage = 0;
+    size_t packed = 0, query = 0, slot = 0;
+    auto open = [&] {
         const int token = item / a.parts, part = item - token * a.parts, b = token / a.seq, t = token - b * a.seq;
-        const int r0 = rounds.total * part / a.parts, r1 = rounds.total * (part + 1) / a.parts;
-        const int position = __ldg(a.positions + token);
-        const size_t packed = (size_t)token * (a.heads + 2 * a.kv_heads) * a.dim;
-        const T *in = static_cast<const T *>(a.qkv) + packed;
-        T *out = static_cast<T *>(a.dqkv) + packed;
-        const T *q = static_cast<const T *>(a.q) + ((size_t)b * a.heads * a.seq + t) * a.dim;
-        const size_t slot = ((size_t)b * a.kv_heads * a.seq + t) * a.dim;
-        for (int r = r0; r < r1; r += kAhead) {
-            Row<T> g[kAhead], x[kAhead];
-            int to[kAhead];
-            bool on[kAhead];
+        r = rounds.total * part / a.parts, r1 = rounds.total * (part + 1) / a.parts;
+        position = __ldg(a.positions + token);
+        packed = (size_t)token * (a.heads + 2 * a.kv_heads) * a.dim;
+        query = ((size_t)b * a.heads * a.seq + t) * a.dim, slot = ((size_t)b * a.kv_heads * a.seq + t) * a.dim;
+    };
+    auto pieces = [&](int stage, int u) { return staged + ((warp * 2 + stage) * kStepUnits + 2 * kUnits * u) * 32; };
+    auto offset = [&](int kind, int h) { return ((kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads) + h) * a.dim; };
+    auto copy = [&](int stage) {
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                int kind, h;
-                on[u] = rounds.at(a, r + u, sub, kind, h) && r + u < r1;
-                to[u] = ((kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads) + h) * a.dim;
-                g[u].load((kind == 0 ? q : static_cast<const T *>(kind == 1 ? a.k : a.v) + slot) + h * q_step, at, on[u]);
-                x[u].load(in + to[u], at, on[u] && a.norm && kind < 2);
-            }
-            if (r == r0 && r < rounds.k) turn.form(a, position, lane);
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                if (r + u >= r1) break;
-                if (r + u < rounds.k) {
-                    Elements d;
-                    d.from(g[u]);
-                    turn.apply(d, row, partners, chunk, a.rotary);
-                    if (a.norm) {
-                        const int kind = r + u < rounds.q ? 0 : 1;
-                        Elements y;
-                        y.from(x[u]);
-                        const float scale = rsqrtf(fmaf(row_sum<kLanes>(y.dot(y)), a.inv_dim, a.epsilon));
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], both(scale));
-                        // lanes without a row hold zeros
-                        if (kind == 0) {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) dwq.v[i] = fma2(d.v[i], y.v[i], dwq.v[i]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 8; ++i) dwk.v[i] = fma2(d.v[i], y.v[i], dwk.v[i]);
-                        }
-                        Elements w;
-                        load_weights(w, weights[kind], at);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) d.v[i] = mul2(d.v[i], w.v[i]);
-                        const float mean = -row_sum<kLanes>(d.dot(y)) * a.inv_dim;
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) d.v[i] = mul2(both(scale), fma2(y.v[i], both(mean), d.v[i]));
-                    }
-                    d.to(g[u]);
-                }
-                g[u].store(out + to[u], at, on[u]);
-            }
+        for (int u = 0; u < kStep; ++u) {
+            int kind, h;
+            const bool on = rounds.at(a, r + u, sub, kind, h) && r + u < r1;
+            if (!on) h = 0;
+            Stage::copy(pieces(stage, u), static_cast<const T *>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (kind == 0 ? query : slot) + h * q_step, at, on, lane, a.dim);
+            Stage::copy(pieces(stage, u) + 32 * kUnits, static_cast<const T *>(a.qkv) + packed + offset(kind, h), at, on && a.norm && kind < 2, lane, a.dim);
         }
+        copies_commit();
+    };
+    bool more = item < items, fresh = true;
+    if (more) open(), copy(0);
+    while (more) {
+        const int now = r, end = r1, angle = position;
+        const bool first = fresh;
+        T *out = static_cast<T *>(a.dqkv) + packed;
+        r += kStep, fresh = r >= r1;
+        if (fresh) {
+            item += gridDim.x * kWarps, more = item < items;
+            if (more) open();
+        }
+        if (more) copy(stage ^ 1);
+        else copies_commit();
+        if (first && now < rounds.k) turn.form(a, angle, lane);
+        copies_wait_but_one();
+        if (kPair != kHalves) __syncwarp();
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) {
+            if (now + u >= end) break;
+            int kind, h;
+            const bool on = rounds.at(a, now + u, sub, kind, h);
+            Row<T> g = Stage::take(pieces(stage, u), lane);
+            if (kind < 2) {
+                Elements d;
+                d.from(g);
+                turn.apply(d, row, partners, chunk, a.rotary);
+                if (a.norm) {
+                    Elements y;
+                    y.from(Stage::take(pieces(stage, u) + 32 * kUnits, lane));
+                    const float scale = rsqrtf(fmaf(row_sum<kLanes>(y.dot(y)), a.inv_dim, a.epsilon));
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], both(scale));
+                    // lanes without a row hold zeros
+                    if (kind == 0) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dwq.v[i] = fma2(d.v[i], y.v[i], dwq.v[i]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) dwk.v[i] = fma2(d.v[i], y.v[i], dwk.v[i]);
+                    }
+                    Elements w;
+                    load_weights<kPair>(w, weights[kind], at);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d.v[i] = mul2(d.v[i], w.v[i]);
+                    const float mean = -row_sum<kLanes>(d.dot(y)) * a.inv_dim;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) d.v[i] = mul2(both(scale), fma2(y.v[i], both(mean), d.v[i]));
+                }
+                d.to(g);
+            }
+            g.store(out + offset(kind, on ? h : 0), at, on);
+        }
+        stage ^= 1;
+        if (kPair != kHalves) __syncwarp();  // the stage has been read
     }
     grid_dependency_trigger();
     if (!a.norm) return;
@@ -540,8 +610,10 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
     // there are tokens for many waves, down to one round a warp for few tokens.
     const int per = 32 / kLanes, rounds = rounds_of((int)s.heads, per) + 2 * rounds_of((int)s.kv_heads, per), dim = s.dim;
     int per_sm = 0;
+    const int staged = grad ? kGradStaged : 0;
     const void *kernel = grad ? reinterpret_cast<const void *>(rope_grad_kernel<T, kLanes, kPair>) : reinterpret_cast<const void *>(rope_kernel<T, kLanes, kPair>);
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, 0) != cudaSuccess || per_sm < 1)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, staged) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, staged) != cudaSuccess || per_sm < 1)
         throw IrError("the rotation kernel does not fit on an SM");
     const long long tokens = (long long)s.batch * s.seq, resident = (long long)per_sm * ctx->sm_count * kWarps;
     base.parts = (int)std::max(1ll, std::min<long long>(rounds, kPartWaves * resident / tokens));
@@ -568,7 +640,7 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
             return cudaGetLastError();
         }
         a.dqkv = b[i++];
-        rope_grad_kernel<T, kLanes, kPair><<<blocks, kThreads, 0, st>>>(a);
+        rope_grad_kernel<T, kLanes, kPair><<<blocks, kThreads, staged, st>>>(a);
         if (!norm) return cudaGetLastError();
         const cudaError_t e = launch_after(st, rope_weight_grad_kernel, (2 * dim + 31) / 32, 1024, 0, static_cast<const float *>(a.partial), blocks,
                                            dim, static_cast<float *>(b[i]), static_cast<float *>(b[i + 1]));
