@@ -42,16 +42,18 @@ __device__ __forceinline__ bool sees(const TreeArgs &a, int b, int row, int j, i
 // cache, come by bulk copies through a ring. Warps take row groups
 // of four rows, in registers with their sums, and a group's warps share the tile's keys.
 // kLanes lanes hold a key's elements (four at 4 lane + 4 kLanes i), so a warp works on
-// 32 / kLanes keys at once and twice as many an iteration: 4 rows x 2 keys of scores per
-// lane are summed by halving exchanges (7 shuffles, not 24) that leave each lane one
+// 32 / kLanes keys at once and on kSets times twice as many an iteration (more of them hide
+// more latency: 64 rows below 153 us with one set, 137 with two, 129 with four): a set's 4
+// rows x 2 keys of scores per lane are summed by halving exchanges (7 shuffles, not 24) that leave each lane one
 // score, whose exponential it forms alone and hands back to the others. Maxima and sums
 // are per lane group and joined at the end; sums are rescaled only when a maximum grows
 // by more than 2^8. K and V cross shared memory once per row group.
 // Bound by HBM for a few rows, else by FFMA issue beside shuffles and shared-memory reads.
 // Measured on B200, FP32, dim 128: 64 heads of 1,000 to 8,000 keys, 4 rows (295 MB), 62 us
-// with the join = 4.8 TB/s; 32 heads of 1,000 to 4,000, 4 / 16 / 64 rows: 26 / 47 / 153 us;
-// 16 heads of up to 4,000, 512 rows, 442 us = 23 TFLOP/s. No fifth warp for the copies: it
-// would cap the others at 168 registers, and the spills cost more (62 us for 47).
+// with the join = 4.8 TB/s; 32 heads of 1,000 to 4,000, 4 / 16 / 64 rows: 26 / 42 / 129 us;
+// 16 heads of up to 4,000, 512 rows, 378 us = 27 TFLOP/s. No fifth warp for the copies: it
+// would cap the others at 168 registers, and the spills cost more (16 rows, one set: 62 us
+// for 49).
 constexpr int kStreamWarps = 4, kStreamThreads = 32 * kStreamWarps, kStreamStages = 3, kGroupRows = 4;
 constexpr int kStreamPad = 1024;  // behind the ring: the last V row is read up to the lanes' width
 
@@ -108,7 +110,7 @@ __device__ __forceinline__ float scattered_sum(float (&v)[8], int c) {
 }
 
 // grid: (row blocks of `groups` row groups, splits, batch * kv_heads)
-template <typename T, int kLanes, int kPieces, bool kWhole>
+template <typename T, int kLanes, int kPieces, bool kWhole, int kSets>
 __global__ void __launch_bounds__(kStreamThreads, 2) tree_stream_kernel(const TreeArgs a, int splits, int groups, int tile_keys) {
     constexpr int kKeys = 32 / kLanes, kSame = kLanes / 8;  // keys at once; lanes that get the same score
     extern __shared__ __align__(128) uint8_t ring_smem[];
@@ -166,18 +168,23 @@ __global__ void __launch_bounds__(kStreamThreads, 2) tree_stream_kernel(const Tr
         const float threshold = kRescaleThreshold / a.scale_log2;
         auto pass = [&](const T *k, const T *v, int j0, int count, auto careful) {
 #pragma unroll 1
-            for (int k0 = kw * 2 * kKeys; k0 < count; k0 += key_warps * 2 * kKeys) {
-                float s8[8];
+            for (int k0 = kw * 2 * kSets * kKeys; k0 < count; k0 += key_warps * 2 * kSets * kKeys) {
+                float s8[kSets][8], p[kSets], top = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int u = 0; u < 2 * kSets; ++u) {
                     uint64_t x[2 * kPieces];
                     load_pieces<kWhole, kLanes, kPieces>(x, k + (k0 + u * kKeys + g) * a.dim, c, a.dim);
 #pragma unroll
-                    for (int r = 0; r < kGroupRows; ++r) s8[2 * r + u] = dot(q[r], x);
+                    for (int r = 0; r < kGroupRows; ++r) s8[u / 2][2 * r + u % 2] = dot(q[r], x);
                 }
-                float s = scattered_sum<kLanes>(s8, c);
-                if (careful) s = k0 + my_key < count && sees(a, b, my_row, j0 + k0 + my_key, length) ? s : -INFINITY;
-                const float top = fmaxf(s, __shfl_xor_sync(0xffffffffu, s, kSame));
+#pragma unroll
+                for (int h = 0; h < kSets; ++h) {
+                    const int key = k0 + 2 * h * kKeys + my_key;
+                    p[h] = scattered_sum<kLanes>(s8[h], c);
+                    if (careful) p[h] = key < count && sees(a, b, my_row, j0 + key, length) ? p[h] : -INFINITY;
+                    top = fmaxf(top, p[h]);
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, kSame));
                 if (__any_sync(0xffffffffu, top > m + threshold)) {
                     const float m_new = fmaxf(m, top), alpha = exp2f((m - (m_new == -INFINITY ? 0.0f : m_new)) * a.scale_log2);
                     m = m_new;
@@ -189,15 +196,18 @@ __global__ void __launch_bounds__(kStreamThreads, 2) tree_stream_kernel(const Tr
                         for (int i = 0; i < 2 * kPieces; ++i) o[r][i] = mul2(o[r][i], pack2f(f, f));
                     }
                 }
-                const float p = exp2f((s - (m == -INFINITY ? 0.0f : m)) * a.scale_log2);
-                l += p;
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
+                for (int h = 0; h < kSets; ++h) {
+                    p[h] = exp2f((p[h] - (m == -INFINITY ? 0.0f : m)) * a.scale_log2);
+                    l += p[h];
+                }
+#pragma unroll
+                for (int u = 0; u < 2 * kSets; ++u) {
                     uint64_t x[2 * kPieces];
                     load_pieces<true, kLanes, kPieces>(x, v + (k0 + u * kKeys + g) * a.dim, c, a.dim);  // columns beyond the head are not written
 #pragma unroll
                     for (int r = 0; r < kGroupRows; ++r) {
-                        const float w = __shfl_sync(0xffffffffu, p, g * kLanes + (2 * r + u) * kSame);
+                        const float w = __shfl_sync(0xffffffffu, p[u / 2], g * kLanes + (2 * r + u % 2) * kSame);
                         if (!careful || w != 0.0f)  // drafts: no product with one that the row does not see
 #pragma unroll
                             for (int i = 0; i < 2 * kPieces; ++i) o[r][i] = fma2(pack2f(w, w), x[i], o[r][i]);
@@ -399,13 +409,13 @@ __global__ void __launch_bounds__(kStreamThreads) tree_finish_kernel(const TreeA
 }
 
 // The kernels of a head dimension (16-bit types come here above 128 only).
-template <typename T>
+template <typename T, int kSets>
 auto kernel_of(int dim) -> void (*)(TreeArgs, int, int, int) {
     if constexpr (std::is_same<T, float>::value) {
-        if (dim <= 64) return dim == 64 ? tree_stream_kernel<T, 8, 2, true> : tree_stream_kernel<T, 8, 2, false>;
-        if (dim <= 128) return dim == 128 ? tree_stream_kernel<T, 8, 4, true> : tree_stream_kernel<T, 8, 4, false>;
+        if (dim <= 64) return dim == 64 ? tree_stream_kernel<T, 8, 2, true, kSets> : tree_stream_kernel<T, 8, 2, false, kSets>;
+        if (dim <= 128) return dim == 128 ? tree_stream_kernel<T, 8, 4, true, kSets> : tree_stream_kernel<T, 8, 4, false, kSets>;
     }
-    return dim == 256 ? tree_stream_kernel<T, 16, 4, true> : tree_stream_kernel<T, 16, 4, false>;
+    return dim == 256 ? tree_stream_kernel<T, 16, 4, true, kSets> : tree_stream_kernel<T, 16, 4, false, kSets>;
 }
 template <typename T>
 auto finish_of(int dim) -> void (*)(TreeArgs, int, int, int, int) {
@@ -434,7 +444,8 @@ LaunchFn simt_launch(Context *ctx, const Spec &s) {
     const int width = s.dim <= 64 ? 64 : s.dim <= 128 ? 128 : 256;
     const size_t joined = kStreamWarps * kGroupRows * (width * sizeof(float) + sizeof(float2));
     const size_t smem = std::max(2 * kStreamStages * tile_keys * s.dim * sizeof(T) + kStreamPad, joined);
-    const auto kernel = kernel_of<T>(s.dim);
+    // key sets of an iteration: as many as give each of a row group's warps keys of every tile
+    const auto kernel = groups > 2 ? kernel_of<T, 4>(s.dim) : groups > 1 ? kernel_of<T, 2>(s.dim) : kernel_of<T, 1>(s.dim);
     const auto finish = finish_of<T>(s.dim);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         throw IrError("cannot reserve shared memory for attention_tree");
