@@ -282,6 +282,38 @@ def test_attention_tree(rt, case, dtype):
     check_tree(got, TREES[case], x, sees, dtype)
 
 
+# off the tensor core: every count of row groups and of warps that share a tile's keys, lengths
+# around tiles of 16 and 32 keys, many tiles a block, heads that do not fill a warp's lanes
+NARROW = [
+    dict(batch=6, seq=1, heads=3, kv_heads=3, dim=136, capacity=99, lengths=[98, 0, 15, 16, 31, 32]),
+    dict(batch=3, seq=5, heads=2, kv_heads=2, dim=256, capacity=400, lengths=[395, 11, 27]),  # two groups
+    dict(batch=2, seq=3, heads=8, kv_heads=2, dim=200, capacity=700, lengths=[697, 30]),  # three
+    dict(batch=2, seq=13, heads=1, kv_heads=1, dim=248, capacity=2500, lengths=[2400, 51]),  # four, the last with one row
+    dict(batch=2, seq=19, heads=2, kv_heads=2, dim=192, capacity=300, lengths=[281, 13]),  # five: blocks of three
+    dict(batch=40, seq=1, heads=16, kv_heads=16, dim=144, capacity=500, lengths=[(131 * b) % 500 for b in range(40)]),
+    dict(batch=2, seq=125, heads=4, kv_heads=2, dim=160, capacity=260, lengths=[135, 0]),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("case", range(len(NARROW)))
+def test_attention_tree_wide_heads(rt, case, dtype):
+    x, sees = tree_inputs(NARROW[case], dtype, 50 + case)
+    got = R.run(rt, tree_spec(NARROW[case], dtype), x)
+    check_tree(got, NARROW[case], x, sees, dtype)
+    again = R.run(rt, tree_spec(NARROW[case], dtype), x)
+    np.testing.assert_array_equal(got["out"], again["out"])
+    np.testing.assert_array_equal(got["weights"], again["weights"])
+
+
+@pytest.mark.parametrize("dim", [8, 24, 64, 88, 128])
+@pytest.mark.parametrize("rows", [1, 4, 6, 12, 16, 21, 35])
+def test_attention_tree_fp32_rows(rt, rows, dim):
+    case = dict(batch=3, seq=rows, heads=2, kv_heads=2, dim=dim, capacity=1000, lengths=[960, 31 - rows if rows < 31 else 3, 0])
+    x, sees = tree_inputs(case, "fp32", 60 + rows)
+    check_tree(R.run(rt, tree_spec(case, "fp32"), x), case, x, sees, "fp32")
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_attention_tree_without_weights_is_the_same(rt, dtype):
     x, _ = tree_inputs(TREES[4], dtype, 4)
@@ -308,7 +340,15 @@ def test_attention_tree_large_scores(rt, case, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("case", [3, 4, 8])
 def test_attention_tree_masked_nan_and_infinity_stay_away(rt, case, dtype):
-    case = TREES[case]
+    masked_nan_and_infinity(rt, TREES[case], dtype)
+
+
+@pytest.mark.parametrize("case", [2, 4, 6])
+def test_attention_tree_wide_heads_masked_nan_and_infinity_stay_away(rt, case):
+    masked_nan_and_infinity(rt, NARROW[case], "fp16")
+
+
+def masked_nan_and_infinity(rt, case, dtype):
     x, sees = tree_inputs(case, dtype, 30)
     T = case["seq"]
     hidden = T // 2  # a draft that only itself sees
