@@ -23,15 +23,16 @@
 //
 // Both kernels are bound by HBM (each row read and written once), with the issue rate
 // close behind: 16 elements a lane, 32 / kLanes rows a warp (a round), packed FP32x2
-// arithmetic. A warp takes heads of one token, whose sines and cosines it forms once,
-// a few a lane, in shared memory; the rows of the next rounds load meanwhile. Angles
-// and norm weights are read from shared memory for every round: registers hold rows
-// only, so that enough warps are resident. No block barrier per token, so that warps
-// drift apart and memory stays busy. Measured on B200, BF16, 4 x 2048 tokens of 16 + 2 x 16
-// heads of 128 (201 MB moved; a plain copy of them takes 36 us): 42 us = 4.7 TB/s with
-// halves, 44 with neighbours, 51 with a rotary that is no multiple of 16; the gradient (268
-// MB) 58, 58 and 66 us = 4.7 TB/s (64 with each step's rows loaded to registers and waited
-// for). One token: 4.2 us.
+// arithmetic. A persistent warp walks over items, a token's heads or a part of them, and
+// forms the token's sines and cosines once, a few a lane, in shared memory. While it works
+// on a step of rounds, the next step's rows, of the next item where this one ends, come by
+// asynchronous copies. Angles and norm weights are read from shared memory for every
+// round: registers hold one round's rows only, so that enough warps are resident. No block
+// barrier per token, so that warps drift apart and memory stays busy. Measured on B200, BF16, 4 x 2048 tokens of 16 + 2 x 16
+// heads of 128 (201 MB moved; a plain copy of them takes 36 us): 41 us = 4.9 TB/s with
+// halves, 41 with neighbours, 52 with a rotary that is no multiple of 16; the gradient (268
+// MB) 59, 60 and 67 us = 4.6 TB/s. With rows loaded to registers: 43, 45 and 51, 64, 71 and
+// 83. One token: 4.4 us.
 #include <climits>
 #include <cmath>
 #include <type_traits>
@@ -90,15 +91,6 @@ struct Piece { uint4 u; };
 template <>
 struct Piece<float> { float4 a, b; };
 
-__device__ __forceinline__ void load_piece(Piece<float> &x, const float *p, bool on) {
-    x.a = x.b = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (on) x.a = __ldcs(reinterpret_cast<const float4 *>(p)), x.b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-}
-template <typename T>
-__device__ __forceinline__ void load_piece(Piece<T> &x, const T *p, bool on) {
-    x.u = make_uint4(0, 0, 0, 0);
-    if (on) x.u = __ldcs(reinterpret_cast<const uint4 *>(p));
-}
 __device__ __forceinline__ void store_piece(float *p, const Piece<float> &x) {
     reinterpret_cast<float4 *>(p)[0] = x.a;
     reinterpret_cast<float4 *>(p)[1] = x.b;
@@ -140,10 +132,6 @@ __device__ __forceinline__ void narrow(Piece<T> &x, const uint64_t *v) {
 template <typename T>
 struct Row {  // a lane's share of a head
     Piece<T> lo, hi;
-    __device__ __forceinline__ void load(const T *p, const Place &at, bool on) {
-        load_piece(lo, p + at.lo, on && at.has_lo);
-        load_piece(hi, p + at.hi, on && at.has_hi);
-    }
     __device__ __forceinline__ void store(T *p, const Place &at, bool on) const {
         if (on && at.has_lo) store_piece(p + at.lo, lo);
         if (on && at.has_hi) store_piece(p + at.hi, hi);
@@ -151,32 +139,42 @@ struct Row {  // a lane's share of a head
 };
 
 // A round's rows on their way through shared memory, in units of 16 bytes that leave
-// memory in whole sectors. kHalves: every lane copies its own pieces (its neighbours'
-// lie beside them). Else the lanes of a row copy its units in turn, and lane c takes
-// units kUnits c ..; unit n is kept at n ^ (n / 8 mod kUnits), clear of bank conflicts.
+// memory in whole sectors. A piece of kHalves in 16 bits is a unit whose neighbours lie
+// beside it: every lane copies its own. Else the lanes of a row copy its units in turn;
+// unit n is kept at n ^ (n / 8 mod kUnits), clear of bank conflicts.
 template <typename T, int kLanes, Pairing kPair>
 struct Staged {
     static constexpr int kUnits = 2 * sizeof(Piece<T>) / 16, kEach = 16 / sizeof(T);
-    static __device__ __forceinline__ int place(int lane, int i) {
-        if (kPair == kHalves) return 32 * i + lane;
-        const int n = kUnits * (lane % kLanes) + i;
-        return lane / kLanes * (kLanes * kUnits) + (n ^ (n >> 3 & (kUnits - 1)));
-    }
+    static constexpr bool kOwn = kPair == kHalves && sizeof(T) == 2;
+    static __device__ __forceinline__ int slot(int lane, int n) { return lane / kLanes * (kLanes * kUnits) + (n ^ (n >> 3 & (kUnits - 1))); }
     static __device__ __forceinline__ void copy(uint4 *to, const T *p, const Place &at, bool on, int lane, int dim) {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-            const int n = lane % kLanes + kLanes * i, hi = i >= kUnits / 2;
-            const bool has = on && (kPair == kHalves ? (hi ? at.has_hi : at.has_lo) : n * kEach < dim);
-            const int from = kPair == kHalves ? (hi ? at.hi : at.lo) + i % (kUnits / 2) * kEach : n * kEach;
-            const int slot = kPair == kHalves ? 32 * i + lane : lane / kLanes * (kLanes * kUnits) + (n ^ (n >> 3 & (kUnits - 1)));
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to + slot)), "l"(p + (has ? from : 0)), "r"(has ? 16 : 0) : "memory");
+            const int n = lane % kLanes + kLanes * i;
+            const bool has = on && (kOwn ? (i ? at.has_hi : at.has_lo) : n * kEach < dim);
+            const int from = kOwn ? (i ? at.hi : at.lo) : n * kEach;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to + (kOwn ? 32 * i + lane : slot(lane, n)))),
+                         "l"(p + (has ? from : 0)), "r"(has ? 16 : 0)
+                         : "memory");
         }
     }
-    static __device__ __forceinline__ Row<T> take(const uint4 *from, int lane) {
+    // zeros where the lane has no piece
+    static __device__ __forceinline__ Row<T> take(const uint4 *from, const Place &at, int lane) {
         uint4 x[kUnits];
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) x[i] = from[place(lane, i)];
+        for (int i = 0; i < kUnits; ++i) {
+            const bool hi = i >= kUnits / 2;
+            if (kOwn) x[i] = from[32 * i + lane];
+            else {
+                x[i] = make_uint4(0, 0, 0, 0);
+                if (hi ? at.has_hi : at.has_lo) x[i] = from[slot(lane, (hi ? at.hi : at.lo) / kEach + i % (kUnits / 2))];
+            }
+        }
         return {*reinterpret_cast<const Piece<T> *>(&x[0]), *reinterpret_cast<const Piece<T> *>(&x[kUnits / 2])};
+    }
+    // other lanes' copies have landed; the stage has been read by all
+    static __device__ __forceinline__ void meet() {
+        if (!kOwn) __syncwarp();
     }
 };
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -345,9 +343,15 @@ struct Rounds {
     }
 };
 
+// 16-byte pieces of a lane and step: two rounds in 16 bits (four: 42.7 us for 41.0), one in 32
+constexpr int kForwardUnits = 4;
+constexpr int kForwardStaged = kWarps * 2 * kForwardUnits * 32 * 16;
+
 template <typename T, int kLanes, Pairing kPair>
-__global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
-    constexpr int kAhead = 2;  // rounds worked on, and as many loading
+__global__ void __launch_bounds__(kThreads, 5) rope_kernel(const RopeArgs a) {
+    using Stage = Staged<T, kLanes, kPair>;
+    constexpr int kUnits = Stage::kUnits, kStep = kForwardUnits / kUnits;  // rounds of a step
+    extern __shared__ uint4 staged[];
     __shared__ __align__(16) float tables[kWarps][Turn<kLanes, kPair, false>::kFloats];
     __shared__ __align__(16) float weights[2][kTable];
     __shared__ float shared_rows[kPair == kGeneral ? kWarps : 1][32 * 17];
@@ -363,45 +367,56 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
         if (chunk == 0) row[kZeroAt] = 0.0f;
     }
     __syncthreads();
-    const int item = blockIdx.x * kWarps + warp;
-    if (item >= a.batch * a.seq * a.parts) return;
-    const int token = item / a.parts, part = item - token * a.parts, b = token / a.seq, t = token - b * a.seq;
-    const int r0 = rounds.total * part / a.parts, r1 = rounds.total * (part + 1) / a.parts;
-    const int position = __ldg(a.positions + token), start = a.starts ? __ldg(a.starts + b) : 0;
-    const T *in = static_cast<const T *>(a.qkv) + (size_t)token * (a.heads + 2 * a.kv_heads) * a.dim;
-    // first row of the token's queries, and its slot of the first head's keys and values
-    T *q = static_cast<T *>(a.q) + ((size_t)b * a.heads * a.seq + t) * a.dim;
-    const size_t slot = ((size_t)b * a.kv_heads * a.rows + start + t) * a.dim;
-    const int q_step = a.seq * a.dim;
+    const int q_step = a.seq * a.dim, items = a.batch * a.seq * a.parts;
     const long long kv_step = (long long)a.rows * a.dim;
-    Row<T> next[kAhead];
-    auto load = [&](int r) {
+    // the next step: its item, rounds r .. of r1, and the rows of its token
+    int item = blockIdx.x * kWarps + warp, r = 0, r1 = 0, position = 0, start = 0, token = 0, stage = 0;
+    auto open = [&] {
+        token = item / a.parts;
+        const int part = item - token * a.parts;
+        r = rounds.total * part / a.parts, r1 = rounds.total * (part + 1) / a.parts;
+        position = __ldg(a.positions + token);
+        start = a.starts ? __ldg(a.starts + token / a.seq) : 0;
+    };
+    auto pieces = [&](int stage, int u) { return staged + ((warp * 2 + stage) * kForwardUnits + kUnits * u) * 32; };
+    auto copy = [&](int stage) {
+        const T *in = static_cast<const T *>(a.qkv) + (size_t)token * (a.heads + 2 * a.kv_heads) * a.dim;
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
+        for (int u = 0; u < kStep; ++u) {
             int kind, h;
             const bool on = rounds.at(a, r + u, sub, kind, h) && r + u < r1;
-            next[u].load(in + ((kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads) + h) * a.dim, at, on);
+            Stage::copy(pieces(stage, u), in + (on ? ((kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads) + h) * a.dim : 0), at, on, lane, a.dim);
         }
+        copies_commit();
     };
-    load(r0);
-    if (start < 0 || start > a.rows - a.seq) {
-        if (lane == 0) atomicCAS(a.err, 0, kErrCacheLength);
-        return;
-    }
-    if (r0 < rounds.k) turn.form(a, position, lane);
-    for (int r = r0; r < r1; r += kAhead) {
-        Row<T> x[kAhead];
+    bool more = item < items, fresh = true;
+    if (more) open(), copy(0);
+    while (more) {
+        const int now = r, end = r1, angle = position, slot0 = start, b = token / a.seq, t = token - b * a.seq;
+        const bool first = fresh;
+        r += kStep, fresh = r >= r1;
+        if (fresh) {
+            item += gridDim.x * kWarps, more = item < items;
+            if (more) open();
+        }
+        if (more) copy(stage ^ 1);
+        else copies_commit();
+        const bool fits = slot0 >= 0 && slot0 <= a.rows - a.seq;
+        if (!fits && lane == 0) atomicCAS(a.err, 0, kErrCacheLength);
+        if (first && now < rounds.k) turn.form(a, angle, lane);
+        T *q = static_cast<T *>(a.q) + ((size_t)b * a.heads * a.seq + t) * a.dim;
+        const size_t slot = ((size_t)b * a.kv_heads * a.rows + slot0 + t) * a.dim;
+        copies_wait_but_one();
+        Stage::meet();
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) x[u] = next[u];
-        if (r + kAhead < r1) load(r + kAhead);
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (r + u >= r1) break;
+        for (int u = 0; u < kStep; ++u) {
+            if (now + u >= end) break;
             int kind, h;
-            const bool on = rounds.at(a, r + u, sub, kind, h);
+            const bool on = rounds.at(a, now + u, sub, kind, h) && fits;
+            Row<T> x = Stage::take(pieces(stage, u), at, lane);
             if (kind < 2) {
                 Elements y;
-                y.from(x[u]);
+                y.from(x);
                 if (a.norm) {
                     Elements w;
                     load_weights<kPair>(w, weights[kind], at);
@@ -410,16 +425,16 @@ __global__ void __launch_bounds__(kThreads, 4) rope_kernel(const RopeArgs a) {
                     for (int i = 0; i < 8; ++i) y.v[i] = mul2(mul2(y.v[i], scale), w.v[i]);
                 }
                 turn.apply(y, row, partners, chunk, a.rotary);
-                y.to(x[u]);
+                y.to(x);
             }
-            x[u].store(kind == 0 ? q + h * q_step : static_cast<T *>(kind == 1 ? a.k : a.v) + slot + h * kv_step, at, on);
+            x.store(kind == 0 ? q + h * q_step : static_cast<T *>(kind == 1 ? a.k : a.v) + slot + h * kv_step, at, on);
         }
+        stage ^= 1;
+        Stage::meet();
     }
 }
 
-// A persistent warp walks over items (a token, a part of its heads) and keeps its sums
-// of the weights' gradients. While it works on a step's rows, each lane's pieces of the
-// next step's, of the next item's where this one ends, come by asynchronous copies.
+// As rope_kernel; a warp keeps its sums of the weights' gradients over all its items.
 constexpr int kStepUnits = 8;  // 16-byte pieces of a lane and step
 constexpr int kGradStaged = kWarps * 2 * kStepUnits * 32 * 16;
 
@@ -486,20 +501,20 @@ __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a
         else copies_commit();
         if (first && now < rounds.k) turn.form(a, angle, lane);
         copies_wait_but_one();
-        if (kPair != kHalves) __syncwarp();
+        Stage::meet();
 #pragma unroll
         for (int u = 0; u < kStep; ++u) {
             if (now + u >= end) break;
             int kind, h;
             const bool on = rounds.at(a, now + u, sub, kind, h);
-            Row<T> g = Stage::take(pieces(stage, u), lane);
+            Row<T> g = Stage::take(pieces(stage, u), at, lane);
             if (kind < 2) {
                 Elements d;
                 d.from(g);
                 turn.apply(d, row, partners, chunk, a.rotary);
                 if (a.norm) {
                     Elements y;
-                    y.from(Stage::take(pieces(stage, u) + 32 * kUnits, lane));
+                    y.from(Stage::take(pieces(stage, u) + 32 * kUnits, at, lane));
                     const float scale = rsqrtf(fmaf(row_sum<kLanes>(y.dot(y)), a.inv_dim, a.epsilon));
 #pragma unroll
                     for (int i = 0; i < 8; ++i) y.v[i] = mul2(y.v[i], both(scale));
@@ -524,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 4) rope_grad_kernel(const RopeArgs a
             g.store(out + offset(kind, on ? h : 0), at, on);
         }
         stage ^= 1;
-        if (kPair != kHalves) __syncwarp();  // the stage has been read
+        Stage::meet();
     }
     grid_dependency_trigger();
     if (!a.norm) return;
@@ -610,7 +625,7 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
     // there are tokens for many waves, down to one round a warp for few tokens.
     const int per = 32 / kLanes, rounds = rounds_of((int)s.heads, per) + 2 * rounds_of((int)s.kv_heads, per), dim = s.dim;
     int per_sm = 0;
-    const int staged = grad ? kGradStaged : 0;
+    const int staged = grad ? kGradStaged : kForwardStaged;
     const void *kernel = grad ? reinterpret_cast<const void *>(rope_grad_kernel<T, kLanes, kPair>) : reinterpret_cast<const void *>(rope_kernel<T, kLanes, kPair>);
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, staged) != cudaSuccess ||
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, staged) != cudaSuccess || per_sm < 1)
@@ -618,7 +633,7 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
     const long long tokens = (long long)s.batch * s.seq, resident = (long long)per_sm * ctx->sm_count * kWarps;
     base.parts = (int)std::max(1ll, std::min<long long>(rounds, kPartWaves * resident / tokens));
     if (tokens * base.parts > INT_MAX / 2) throw IrError("too many tokens for one launch");
-    const int blocks = (int)std::min((tokens * base.parts + kWarps - 1) / kWarps, grad ? resident / kWarps : 1ll << 31);
+    const int blocks = (int)std::min((tokens * base.parts + kWarps - 1) / kWarps, resident / kWarps);
     // the frequencies, and behind them the gradient's partial sums
     const std::vector<uint64_t> turns = turn_fractions(s);
     const size_t table = (turns.size() * 8 + 255) / 256 * 256;
@@ -636,7 +651,7 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
         if (cached) a.starts = static_cast<const int *>(b[i++]);
         a.q = b[i++], a.k = b[i++], a.v = b[i++];
         if (!grad) {
-            rope_kernel<T, kLanes, kPair><<<blocks, kThreads, 0, st>>>(a);
+            rope_kernel<T, kLanes, kPair><<<blocks, kThreads, staged, st>>>(a);
             return cudaGetLastError();
         }
         a.dqkv = b[i++];
