@@ -334,17 +334,17 @@ __device__ __forceinline__ void add_weights(const TreeArgs &a, int splits, int f
     __shared__ float2 stats[kWeightRows];  // maximum (0 if the row sees nothing), 1 / sum
     const int b = bh / a.kv_heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane / kLanes, c = lane % kLanes, mine = c / kSame;
     const int length = a.lengths[b], n = length + a.seq;
-    if (length < 0 || length > a.capacity - a.seq) return;
+    if (length < 0 || length > a.capacity - a.seq) return grid_dependency_wait();
     const T *k = static_cast<const T *>(a.k) + (size_t)bh * a.capacity * a.dim, *queries = static_cast<const T *>(a.q) + (size_t)bh * a.rows * a.dim;
-    auto stage = [&](int r0) {
-        __syncthreads();
+    auto stage_rows = [&](int r0) {
         for (int i = threadIdx.x; i < kWeightRows * kWidth / 4; i += kStreamThreads) {
             const int r = i / (kWidth / 4), d = 4 * (i % (kWidth / 4));
             Four f{0, 0};
             if (r0 + r < a.rows && d < a.dim) f = four_of(queries + (size_t)(r0 + r) * a.dim + d);
             *reinterpret_cast<ulonglong2 *>(q + 4 * i) = make_ulonglong2(f.lo, f.hi);
         }
-        // four threads a row
+    };
+    auto stage_stats = [&](int r0) {  // four threads a row
         const int row = min(r0 + (int)(threadIdx.x >> 2), a.rows - 1), part = threadIdx.x & 3;
         const float2 *ml = a.part_ml + ((size_t)bh * a.rows + row) * splits;
         float m = -INFINITY, l = 0.0f;
@@ -356,17 +356,32 @@ __device__ __forceinline__ void add_weights(const TreeArgs &a, int splits, int f
 #pragma unroll
         for (int x = 1; x < 4; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
         if (part == 0) stats[threadIdx.x >> 2] = make_float2(shift, l > 0.0f || l != l ? 1.0f / l : 0.0f);
-        __syncthreads();
     };
-    for (int block = first; block * kStreamWarps * kUnit < n; block += step) {
-        const int key0 = (block * kStreamWarps + warp) * kUnit + (mine & 1) * kKeys + g;  // of this lane's first score, the second 2 kKeys on
-        uint64_t x[4][2 * kPieces];
+    uint64_t x[4][2 * kPieces];
+    auto load_keys = [&](int block) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
             load_pieces<false, kLanes, kPieces>(x[u], k + (size_t)min((block * kStreamWarps + warp) * kUnit + u * kKeys + g, n - 1) * a.dim, c, a.dim);
+    };
+    // the first keys and rows do not depend on the splits
+    load_keys(first);
+    stage_rows(0);
+    grid_dependency_wait();
+    stage_stats(0);
+    __syncthreads();
+    bool staged = true;  // rows 0 ..
+    for (int block = first; block * kStreamWarps * kUnit < n; block += step) {
+        const int key0 = (block * kStreamWarps + warp) * kUnit + (mine & 1) * kKeys + g;  // of this lane's first score, the second 2 kKeys on
+        if (block != first) load_keys(block);
         float acc[2] = {};
         for (int r0 = 0; r0 < a.rows; r0 += kWeightRows) {
-            if (block == first || a.rows > kWeightRows) stage(r0);
+            if (!staged) {
+                __syncthreads();
+                stage_rows(r0);
+                stage_stats(r0);
+                __syncthreads();
+            }
+            staged = a.rows <= kWeightRows;
             const int rows = min(kWeightRows, a.rows - r0);
 #pragma unroll 1
             for (int r = 0; r < rows; r += kGroupRows) {
@@ -402,8 +417,10 @@ __device__ __forceinline__ void add_weights(const TreeArgs &a, int splits, int f
 // (which read the splits' maxima and sums themselves, so neither waits for the other).
 template <typename T, int kLanes, int kPieces>
 __global__ void __launch_bounds__(kStreamThreads) tree_finish_kernel(const TreeArgs a, int splits, int total_rows, int join_blocks, int key_blocks) {
-    grid_dependency_wait();
-    if ((int)blockIdx.x < join_blocks) return join_rows<T>(a, splits, total_rows, blockIdx.x);
+    if ((int)blockIdx.x < join_blocks) {
+        grid_dependency_wait();
+        return join_rows<T>(a, splits, total_rows, blockIdx.x);
+    }
     const int i = blockIdx.x - join_blocks, bh = i / key_blocks;
     add_weights<T, kLanes, kPieces>(a, splits, i - bh * key_blocks, key_blocks, bh);
 }
