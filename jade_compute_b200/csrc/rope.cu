@@ -588,9 +588,21 @@ __global__ void __launch_bounds__(1024) rope_weight_grad_kernel(const float *par
     }
 }
 
-// A token's heads are dealt to several warps while that leaves the GPU's warps (as many
-// as are resident) at most this many items each.
-constexpr int kPartWaves = 2;
+// Warps that share a token's heads: the number for which the resident warps take fewest
+// rounds in a row, an item's angles counted as one more (they cost about that). Against
+// one warp a token, of 48 heads of 128: 700 tokens 8.4 us for 12, 3,000 tokens 17.5 for 20.6.
+// From two items a warp on their ends fall apart by themselves (gradient of 8,192 tokens:
+// 59 us with one warp a token, 63 with two; neighbours forward 41 and 45).
+int parts_of(long long tokens, int rounds, long long resident) {
+    if (tokens >= 2 * resident) return 1;
+    int best = 1;
+    long long least = LLONG_MAX;
+    for (int parts = 1; parts <= rounds; ++parts) {
+        const long long cost = (tokens * parts + resident - 1) / resident * ((rounds + parts - 1) / parts + 1);
+        if (cost < least) best = parts, least = cost;
+    }
+    return best;
+}
 
 // theta_i / 2 pi as 0.64 fixed-point fractions of a turn.
 std::vector<uint64_t> turn_fractions(const Spec &s) {
@@ -621,8 +633,6 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
     base.err = ctx->err_dev;
     const bool grad = s.op == Op::QkNormRopeGrad, norm = s.norm, cached = s.capacity != 0;
     base.inv_dim = 1.0f / (float)s.dim;
-    // A warp's rounds: enough to spread the cost of its angles (about one round's) where
-    // there are tokens for many waves, down to one round a warp for few tokens.
     const int per = 32 / kLanes, rounds = rounds_of((int)s.heads, per) + 2 * rounds_of((int)s.kv_heads, per), dim = s.dim;
     int per_sm = 0;
     const int staged = grad ? kGradStaged : kForwardStaged;
@@ -631,7 +641,7 @@ LaunchFn rope_launch(Context *ctx, const Spec &s) {
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, staged) != cudaSuccess || per_sm < 1)
         throw IrError("the rotation kernel does not fit on an SM");
     const long long tokens = (long long)s.batch * s.seq, resident = (long long)per_sm * ctx->sm_count * kWarps;
-    base.parts = (int)std::max(1ll, std::min<long long>(rounds, kPartWaves * resident / tokens));
+    base.parts = parts_of(tokens, rounds, resident);
     if (tokens * base.parts > INT_MAX / 2) throw IrError("too many tokens for one launch");
     const int blocks = (int)std::min((tokens * base.parts + kWarps - 1) / kWarps, resident / kWarps);
     // the frequencies, and behind them the gradient's partial sums
