@@ -1,0 +1,62 @@
+"""attention_tree over caches that hold infinities and NaN in committed entries, and over
+weights that span many powers of two: outputs and accumulated weights against the 64-bit
+definition (tests/cached_reference.py; tolerances: tests/test_gpu_cached_attention.py),
+in each form of the kernel: four, two and one copies of the rows, two row tiles (more
+than 128 rows), FP32, and 16-bit heads above 128."""
+import numpy as np
+import pytest
+
+import jade_compute_b200 as jc
+from tests import cached_reference as R
+from tests import test_gpu_cached_attention as base
+
+pytestmark = pytest.mark.gpu
+
+# (dtype, dim, rows): every kernel form
+FORMS = [("bf16", 64, 4), ("fp16", 128, 32), ("bf16", 128, 40), ("fp16", 64, 64), ("bf16", 128, 72), ("fp16", 128, 128), ("bf16", 64, 132),
+         ("fp16", 128, 200), ("bf16", 128, 256), ("fp16", 64, 300), ("fp32", 64, 4), ("fp32", 128, 40), ("bf16", 136, 20), ("fp16", 256, 6)]
+
+
+@pytest.fixture(scope="module")
+def rt():
+    r = jc.Runtime(0)
+    yield r
+    r.close()
+
+
+def inputs(dtype, dim, rows, batch, length, seed, kv_heads=2, q_sign=0):
+    """seq * group = rows; q_sign: element 0 of every query is positive, so that an infinite
+    element 0 of a key is an infinite score of its sign in every row."""
+    seq = max(t for t in range(1, min(rows, 100) + 1) if rows % t == 0)
+    case = dict(batch=batch, seq=seq, heads=rows // seq * kv_heads, kv_heads=kv_heads, dim=dim, capacity=length + seq, lengths=[length] * batch)
+    x, sees = base.tree_inputs(case, dtype, seed)
+    if q_sign:
+        x["q"][..., 0] = R.rounded(np.abs(x["q"][..., 0]) + 0.25, dtype)
+    return case, x, sees
+
+
+def rows_of(got, case):
+    """[batch, kv_heads, seq, group, dim]"""
+    B, T, H, Hk, D = (case[n] for n in ("batch", "seq", "heads", "kv_heads", "dim"))
+    return got["out"].reshape(B, T, Hk, H // Hk, D).transpose(0, 2, 1, 3, 4)
+
+
+@pytest.mark.parametrize("value", ["nan", "inf"])
+@pytest.mark.parametrize("dtype,dim,rows", FORMS)
+def test_committed_key_that_is_nan_or_scores_infinity_makes_its_head_nan(rt, dtype, dim, rows, value):
+    # a NaN score is in every row's sum, an infinite one divides infinity by infinity: sequence
+    # b has it at key 256 + b, so at each place of 16, and in kv head 0 alone
+    case, x, sees = inputs(dtype, dim, rows, 16, 700, 70, q_sign=1)
+    clean = base.tree_reference(case, x, sees)
+    for b in range(16):
+        x["k"][b, 0, 256 + b, 0] = float(value)
+    got = R.run(rt, base.tree_spec(case, dtype), x)
+    out = rows_of(got, case)
+    assert np.isnan(out[:, 0]).all()
+    u, exp_error = R.ROUNDOFF[dtype], 2e-5 if dtype == "fp32" else 1e-4
+    ref, mag = (rows_of({"out": z}, case) for z in clean[:2])
+    base.close(out[:, 1], ref[:, 1], mag[:, 1], u, exp_error + (0 if dtype == "fp32" else u))
+    weights = got["weights"].reshape(16, 2, -1)
+    if value == "nan":  # every weight of the row is NaN
+        assert np.isnan(weights[:, 0, :700]).all()
+    assert np.isnan(weights[np.arange(16), 0, 256 + np.arange(16)]).all() and np.isfinite(weights[:, 1]).all()
