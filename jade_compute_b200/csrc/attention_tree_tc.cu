@@ -19,8 +19,11 @@
 //              works for one while the other's softmax runs
 //   warps 2-5, 6-9  softmax of chain 0 / 1, one thread per row: scores out of TMEM,
 //              running maximum and sum in FP32, P rounded to the input type back into
-//              TMEM (relative error 2^-9 / 2^-12 per weight; the sum is of unrounded
-//              weights), O rescaled only when a maximum grows by more than 2^8
+//              TMEM (the sum is of unrounded weights), O rescaled only when a maximum
+//              has grown by more than 2^8 (BF16) or 2^4 (FP16). Relative error 2^-9 / 2^-12
+//              per weight; FP16 has no exponents below 2^-14, so there P is kept 2^11
+//              times as large: full precision down to 2^-25 of the row's largest weight,
+//              an absolute error of 2^-36 of it below
 // M <= 128: the chains take alternate key tiles of the same rows and are joined at
 // the segment's end, both sums being in the same TMEM lanes. M > 128: the chains are
 // two row tiles that share each K and V tile. M <= 64: the tile holds two copies of the
@@ -50,7 +53,14 @@ namespace jade {
 namespace {
 
 constexpr int kThreads = 10 * 32, kTileKeys = 128, kTileRows = 128;
-constexpr float kRescaleThreshold = 8.0f;  // log2 units
+// P = 2^(score - m): m lies kHeadroom below the largest score when it is set, and is kept
+// until the largest has grown by kRescaleThreshold more (log2 units), so P <= 2^15 in FP16.
+// Without the headroom a key of weight 2^-25 beside one of weight 1 became 0, while the
+// row's sum counted it.
+template <uint32_t kFmt>
+struct Exponents {
+    static constexpr float kHeadroom = kFmt == 0 ? 11.0f : 0.0f, kRescaleThreshold = kFmt == 0 ? 4.0f : 8.0f;
+};
 // An item's end in tiles (see "work ranges"), more of them the more rows it writes.
 // Measured on B200, 4 rows, 128 items of 9 to 63 tiles: 73.8 us with 0, 67.3 with 2,
 // 65.7 with 4, 64.6 with 6, 64.5 with 8, 67.0 with 12; 128 rows, 32 items of 72 to 126
@@ -509,10 +519,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], sv[k + e], sv[k + 8 + e]);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], sv[kCopyKeys - 8 + e]);
-                    const float m_tile = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c;
+                    using E = Exponents<kFmt>;
+                    const float m_tile = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * c - E::kHeadroom;
                     float m_new = m_used, alpha = 1.0f;
                     if (first) m_new = m_tile;
-                    else if (m_tile > m_used + kRescaleThreshold) {
+                    else if (m_tile > m_used + E::kRescaleThreshold) {
                         m_new = m_tile;
                         alpha = mufu_exp2(m_used - m_new);
                     }

@@ -60,3 +60,31 @@ def test_committed_key_that_is_nan_or_scores_infinity_makes_its_head_nan(rt, dty
     if value == "nan":  # every weight of the row is NaN
         assert np.isnan(weights[:, 0, :700]).all()
     assert np.isnan(weights[np.arange(16), 0, 256 + np.arange(16)]).all() and np.isfinite(weights[:, 1]).all()
+
+
+@pytest.mark.parametrize("rows", [4, 40, 72, 128, 132, 256])
+def test_fp16_keeps_a_long_tail_of_small_weights(rt, rows):
+    # One key of weight 1 and 1,023 of e^-17.5 = 2^-25.2 whose values alone are not 0: the
+    # output is their sum. Two values round here: p, of at least 2^-25.2 of the largest, to the
+    # type (relative error u down to 2^-25 of the largest weight, 2^-36 of it below), and the
+    # output. Enough heads that a block has whole sequences.
+    heads, length, dim = 160, 1023, 64
+    seq = max(t for t in range(1, min(rows, 100) + 1) if rows % t == 0)
+    case = dict(batch=1, seq=seq, heads=rows // seq * heads, kv_heads=heads, dim=dim, capacity=length + seq, lengths=[length])
+    sees = np.zeros((1, seq, seq), bool)
+    x = {"q": np.zeros((1, case["heads"], seq, dim)), "k": np.zeros((1, heads, length + seq, dim)), "v": np.zeros((1, heads, length + seq, dim)),
+         "lengths": np.array([length], np.int32), "tree": R.tree_words(sees)}
+    x["q"][..., 0] = 8.0
+    x["k"][0, :, 0, 0] = 17.5  # score 17.5, the others 0
+    x["v"][0, :, 1:length] = 1000.0
+    ref, mag, _ = base.tree_reference(case, {**x, "weights": np.zeros((1, heads, length + seq))}, sees)
+    got = R.run(rt, base.tree_spec(case, "fp16", False), x)["out"].reshape(ref.shape)
+    u = R.ROUNDOFF["fp16"]
+    small = 2.0 ** -36 * 1000.0 * length
+    base.close(got, ref, mag + small / (u + 1e-4), u, u + 1e-4)
+
+
+@pytest.mark.parametrize("case", [1, 3, 5])
+def test_fp16_large_scores(rt, case):
+    # the running maximum grows again and again, in smaller steps than in BF16
+    base.test_attention_tree_large_scores(rt, case, "fp16")
