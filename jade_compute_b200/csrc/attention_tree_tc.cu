@@ -285,8 +285,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *g_full = bars + 44, *g_empty = bars + 46;  // joining the copies [chain]
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 48);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
-    uint32_t *bad = tmem_slot + 4;  // [3][4]: drafts with non-finite V, by segment number modulo 3
-    int *plan = reinterpret_cast<int *>(tmem_slot + 16);  // the range's first b, sub, tile and (64 bits) length
+    uint32_t *bad = tmem_slot + 4;  // [4][4]: drafts with non-finite V, by segment number modulo 4
+    int *plan = reinterpret_cast<int *>(tmem_slot + 20);  // the range's first b, sub, tile and (64 bits) length
     float2 *exchange = reinterpret_cast<float2 *>(smem + L::kExchange);  // [chain][row]
     static_assert(16 + 2 * kStages <= 44, "barriers");
 
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(x_full, 256); mbar_init(x_empty, 256); mbar_init(mma_done, 1);
         for (int s = 0; s < kStages; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], 1);
         *abort_flag = 0;
-        for (int i = 0; i < 12; ++i) bad[i] = 0;
+        for (int i = 0; i < 16; ++i) bad[i] = 0;
         fence_barrier_init();
         fence_proxy_async();
     }
@@ -475,9 +475,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int item_row = kTwoTiles ? s.rb * 256 + t * 128 + row : copy_row;  // row of the item's M
             const bool live = __any_sync(0xffffffffu, item_row < ta.rows);      // some row of this warp is one
             uint32_t bits[4] = {0, 0, 0, 0};
-            uint32_t *bad_now = bad + (sn % 3) * 4;
+            // The next segment's notes are cleared here by chain 0. With two row tiles chain 1 may
+            // still read those of segment sn - 2, as O_0 of a segment of one tile is ready without
+            // chain 1's P; but not those of sn - 3: the MMA warp has seen o_free[1] of that segment
+            // before its first P_1 V of sn - 2, and so before anything of sn - 1.
+            uint32_t *bad_now = bad + (sn & 3) * 4;
             if (threadIdx.x == 64)
-                for (int i = 0; i < 4; ++i) bad[((sn + 1) % 3) * 4 + i] = 0;
+                for (int i = 0; i < 4; ++i) bad[((sn + 1) & 3) * 4 + i] = 0;
             if (item_row < ta.rows)
                 for (int w = 0; w < 4; ++w)
                     if (w < ta.words) bits[w] = __ldg(ta.tree + ((size_t)s.b * ta.seq + item_row % ta.seq) * ta.words + w);

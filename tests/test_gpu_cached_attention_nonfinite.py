@@ -88,3 +88,20 @@ def test_fp16_keeps_a_long_tail_of_small_weights(rt, rows):
 def test_fp16_large_scores(rt, case):
     # the running maximum grows again and again, in smaller steps than in BF16
     base.test_attention_tree_large_scores(rt, case, "fp16")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows", [132, 256])
+def test_visible_infinities_of_many_single_tile_sequences(rt, dtype, rows):
+    # Sequences of one key tile each, several a block: whether a draft's values are infinite is
+    # noted per sequence, and the two row tiles of a sequence finish apart from the next one's
+    case, x, sees = inputs(dtype, 64, rows, 700, 20, 74)
+    draft = np.arange(700) % case["seq"]
+    odd = np.arange(700) % 3 != 1
+    for b in np.nonzero(odd)[0]:
+        x["v"][b, :, 20 + draft[b], b % 64] = np.inf
+    out = rows_of(R.run(rt, base.tree_spec(case, dtype, False), x), case)
+    for b in range(700):
+        see = sees[b, :, draft[b]] if odd[b] else np.zeros(case["seq"], bool)
+        assert np.isposinf(out[b][:, see, :, b % 64]).all()
+        assert np.isfinite(out[b][:, ~see]).all() and np.isfinite(np.delete(out[b][:, see], b % 64, axis=-1)).all()
