@@ -532,12 +532,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                         alpha = mufu_exp2(m_used - m_new);
                     }
                     m_used = m_new;
-                    // a row that has seen nothing yet has maximum -inf: its weights are e^-inf = 0
+                    // a row that has seen nothing yet, or only scores of -inf, has maximum -inf: its weights are e^-inf = 0
                     const uint32_t tp = ts + copy * (kCopyKeys / 2);
                     // Every exponential on the special-function units: the polynomial that the prompt kernel
                     // gives a share to clamps a NaN, so that a NaN key would drop out of its row, and
                     // gains nothing here (131,000 keys, 256 rows: 155 us with it and without).
-                    const float psum = store_p<kFmt, false, kCopyKeys>(sv, c, masked && m_used == -INFINITY ? 0.0f : m_used, tp);
+                    const float psum = store_p<kFmt, false, kCopyKeys>(sv, c, m_used == -INFINITY ? 0.0f : m_used, tp);
                     if constexpr (kCopies > 1) {
                         const uint32_t zeros[8] = {};
 #pragma unroll

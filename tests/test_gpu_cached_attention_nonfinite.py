@@ -105,3 +105,13 @@ def test_visible_infinities_of_many_single_tile_sequences(rt, dtype, rows):
         see = sees[b, :, draft[b]] if odd[b] else np.zeros(case["seq"], bool)
         assert np.isposinf(out[b][:, see, :, b % 64]).all()
         assert np.isfinite(out[b][:, ~see]).all() and np.isfinite(np.delete(out[b][:, see], b % 64, axis=-1)).all()
+
+
+@pytest.mark.parametrize("dtype,dim,rows", FORMS)
+def test_committed_keys_that_score_minus_infinity_weigh_nothing(rt, dtype, dim, rows):
+    # single keys, whole tiles of 128 at a sequence's start, in its middle and over all its
+    # committed keys but one: outputs are those of the other keys
+    case, x, sees = inputs(dtype, dim, rows, 4, 700, 71, q_sign=1)
+    for b, gone in enumerate(([0, 17, 130, 699], np.arange(128), np.r_[0:256, 384:512], np.delete(np.arange(700), 650))):
+        x["k"][b, :, gone, 0] = -np.inf
+    base.check_tree(R.run(rt, base.tree_spec(case, dtype, False), x), case, x, sees, dtype, weights=False)
