@@ -945,7 +945,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_after();
                     float sum = 0.0f;
                     if (i * kTileKeys + kTileKeys <= s.length) {
-                        // columns beyond the rows are products with zeros, their exponent is -inf
+                        // columns beyond the rows: their exponent is -inf, and the score is a product
+                        // with zeros, but NaN if the key is infinite
                         uint64_t sums[2] = {0, 0};
                         float sv[32];
                         tmem_ld32f(ts, sv);
@@ -957,6 +958,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int k = 0; k < 32; ++k) e[k] = sv[k];
                             if (n + 32 < count) tmem_ld32f(ts + n + 32, sv);
+                            if (n + 32 > count) {
+#pragma unroll
+                                for (int k = 0; k < 32; ++k)
+                                    if (n + k >= count) e[k] = 0.0f;
+                            }
 #pragma unroll
                             for (int k = 0; k < 32; k += 4) {
                                 const ulonglong2 x = *reinterpret_cast<const ulonglong2 *>(stats + n + k);

@@ -115,3 +115,15 @@ def test_committed_keys_that_score_minus_infinity_weigh_nothing(rt, dtype, dim, 
     for b, gone in enumerate(([0, 17, 130, 699], np.arange(128), np.r_[0:256, 384:512], np.delete(np.arange(700), 650))):
         x["k"][b, :, gone, 0] = -np.inf
     base.check_tree(R.run(rt, base.tree_spec(case, dtype, False), x), case, x, sees, dtype, weights=False)
+
+
+@pytest.mark.parametrize("dtype,dim,rows", FORMS)
+def test_weights_of_keys_that_score_minus_infinity_stay(rt, dtype, dim, rows):
+    case, x, sees = inputs(dtype, dim, rows, 2, 700, 72, q_sign=1)
+    x["k"][0, :, [3, 300, 699], 0] = -np.inf
+    x["k"][1, :, 256:384, 0] = -np.inf
+    got = R.run(rt, base.tree_spec(case, dtype), x)
+    base.check_tree(got, case, x, sees, dtype)
+    weights = got["weights"].reshape(x["weights"].shape)
+    np.testing.assert_array_equal(weights[0][:, [3, 300, 699]], x["weights"][0][:, [3, 300, 699]])
+    np.testing.assert_array_equal(weights[1][:, 256:384], x["weights"][1][:, 256:384])
