@@ -260,6 +260,26 @@ __device__ __forceinline__ void clean_v(uint8_t *v, int thread, int j0, int leng
     }
 }
 
+// The infinities and NaN in 32 columns of `keys` rows of V, as a bit per column: {+inf, -inf,
+// NaN} (whole warp, a row a lane; the first `columns`, a multiple of 8, are the head's).
+template <typename T>
+__device__ __noinline__ uint3 non_finite_columns(const T *v, int keys, int dim, int columns) {
+    const uint32_t e = exponent_bits<T>();
+    uint32_t pos = 0, neg = 0, nan = 0;
+    for (int j = threadIdx.x & 31; j < keys; j += 32)
+#pragma unroll 1
+        for (int c = 0; c < min(32, columns); c += 8) {
+            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(v + (size_t)j * dim + c));
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t x = w[i / 2] >> 16 * (i & 1) & 0xffffu;
+                if ((x & e) == e) ((x & 0x7fffu) != e ? nan : x & 0x8000u ? neg : pos) |= 1u << (c + i);
+            }
+        }
+    return make_uint3(__reduce_or_sync(0xffffffffu, pos), __reduce_or_sync(0xffffffffu, neg), __reduce_or_sync(0xffffffffu, nan));
+}
+
 // ------------------------------------------------------------------ kernel
 template <int DP, typename T, bool kTwoTiles, int kCopies>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -639,6 +659,23 @@ __global__ void __launch_bounds__(kThreads, 1)
                             mbar_arrive(&g_empty[t]);
                         }
                         ++gn;
+                    }
+                    // An infinity of a committed V row times a P of 0 (another copy's columns, a weight below
+                    // the type's range) is NaN, where the row's value is that infinity: such a column is
+                    // read again. Never taken by a finite cache.
+                    bool odd = false;
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) odd |= !isfinite(r[k]);
+                    const int committed = min(s.last * kTileKeys, s.length) - s.first * kTileKeys;
+                    if (__any_sync(0xffffffffu, odd && valid) && committed > 0) {
+                        const uint3 at = non_finite_columns(static_cast<const T *>(ta.v) + ((size_t)bh * ta.capacity + (size_t)s.first * kTileKeys) * ta.dim + oc,
+                                                            committed, ta.dim, ta.dim - oc);
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if ((at.x | at.y | at.z) >> k & 1) {
+                                const float x = (at.z | (at.x & at.y)) >> k & 1 ? NAN : at.x >> k & 1 ? INFINITY : -INFINITY;
+                                r[k] = whole ? x * inv : x;
+                            }
                     }
                     if (extra[0] | extra[1] | extra[2] | extra[3]) {  // non-finite values that this row sees
 #pragma unroll

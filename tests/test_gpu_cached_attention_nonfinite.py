@@ -127,3 +127,27 @@ def test_weights_of_keys_that_score_minus_infinity_stay(rt, dtype, dim, rows):
     weights = got["weights"].reshape(x["weights"].shape)
     np.testing.assert_array_equal(weights[0][:, [3, 300, 699]], x["weights"][0][:, [3, 300, 699]])
     np.testing.assert_array_equal(weights[1][:, 256:384], x["weights"][1][:, 256:384])
+
+
+@pytest.mark.parametrize("length", [1, 100, 700, 5000])
+@pytest.mark.parametrize("dtype,dim,rows", FORMS)
+def test_committed_infinity_in_v_reaches_its_column_as_it_is(rt, dtype, dim, rows, length):
+    # p > 0 for every committed key, so p v is the infinity of v's sign in each of the head's
+    # rows, in that column alone; NaN where the column holds both signs, or a NaN
+    case, x, sees = inputs(dtype, dim, rows, 1, length, 73)
+    clean = base.tree_reference(case, x, sees)[:2]
+    places = [(5, 0, np.inf), (2, length // 2, -np.inf), (dim - 1, length - 1, np.inf), (0, length - 1, np.nan)]
+    for column, key, value in places:
+        x["v"][0, 0, key, column] = value
+    if length > 1:
+        x["v"][0, 0, 0, 3], x["v"][0, 0, length - 1, 3] = np.inf, -np.inf
+    got = R.run(rt, base.tree_spec(case, dtype), x)
+    out, ref, mag = (rows_of(z, case)[0] for z in (got, {"out": clean[0]}, {"out": clean[1]}))
+    assert np.isposinf(out[0][..., 5]).all() and np.isneginf(out[0][..., 2]).all() and np.isposinf(out[0][..., dim - 1]).all()
+    assert np.isnan(out[0][..., 0]).all() and (length == 1 or np.isnan(out[0][..., 3]).all())
+    others = np.delete(np.arange(dim), [0, 2, 5, dim - 1] + ([3] if length > 1 else []))
+    u = R.ROUNDOFF[dtype]
+    c = 2e-5 if dtype == "fp32" else 1e-4 + u
+    base.close(out[0][..., others], ref[0][..., others], mag[0][..., others], u, c)
+    base.close(out[1], ref[1], mag[1], u, c)
+    assert np.isfinite(got["weights"]).all()
