@@ -123,6 +123,10 @@ typedef struct jr_dispatch {
  * it on request (waiting for a timed event and reading it costs about 7 us per batch
  * on a B200 host, which callers of short batches need not pay). */
 #define JR_EXEC_DEFER_MS 4u
+/* With JR_EXEC_DEFER_MS: the batch's time outlives the context's later batches, and
+ * jr_held_ms returns it until the next batch with this flag starts (the Python binding
+ * runs its batches so, which may share a context with callers of this interface). */
+#define JR_EXEC_HOLD_MS 8u
 
 /* Validates every job (context ownership, registered buffers, exact byte sizes,
  * output aliasing - corex.rs:557-569, ir.rs:340-367) before any work is
@@ -132,8 +136,11 @@ typedef struct jr_dispatch {
 JR_API int jr_execute2(void *ctx, const jr_dispatch *jobs, size_t job_count, uint32_t repeats, uint32_t flags,
                 double *gpu_ms, double *job_ms, char *err, size_t cap);
 
-/* Event time of the context's last batch that completed, until its next one starts. */
+/* Event time of the context's last batch (jr_execute's too) if it succeeded, until its
+ * next one starts. */
 JR_API int jr_batch_ms(void *ctx, double *gpu_ms, char *err, size_t cap);
+/* Event time of the context's last batch with JR_EXEC_HOLD_MS. */
+JR_API int jr_held_ms(void *ctx, double *gpu_ms, char *err, size_t cap);
 
 /* Registry queries and pinned host memory for transfer jobs (spec op "copy"). */
 JR_API int jr_buffer_bytes(void *ctx, const void *ptr, size_t *bytes);

@@ -28,6 +28,9 @@ struct Context {
     cudaEvent_t start = nullptr, stop = nullptr;
     cudaEvent_t done = nullptr;  // end of a batch whose time is read later (untimed)
     bool timed = false;          // start and stop bracket a batch that has ended
+    // the last batch with JR_EXEC_HOLD_MS: none, still between start and stop, or read
+    enum class Held { None, Bracketed, Read } held = Held::None;
+    double held_ms = 0;
     std::map<uintptr_t, Allocation> allocations;
     int *err_host = nullptr;  // mapped, written by kernels (first error wins)
     int *err_dev = nullptr;

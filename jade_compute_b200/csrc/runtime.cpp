@@ -206,6 +206,19 @@ double bracket_ms(Context &ctx) {
     if (!std::isfinite(ms) || ms < 0) raise(JR_ECUDA, "invalid GPU-event duration");
     return ms;
 }
+void read_held(Context &ctx) {
+    if (ctx.held != Context::Held::Bracketed) return;
+    ctx.held_ms = bracket_ms(ctx);
+    ctx.held = Context::Held::Read;
+}
+// Records the start of a batch, after the time of one that is held has been read from
+// the same events (or is given up: hold).
+void begin_timing(Context &ctx, bool hold = false) {
+    if (hold) ctx.held = Context::Held::None;
+    read_held(ctx);
+    ctx.timed = false;
+    check_cuda(cudaEventRecord(ctx.start, ctx.stream), "record start event");
+}
 
 // 16-bit attention kernel choice: JADE_ATTENTION_KERNEL=pair or two_tile forces
 // one (read when a kernel is compiled); otherwise the measured rule of
@@ -306,8 +319,7 @@ extern "C" int jr_execute(void *handle, const jr_job *jobs, size_t job_count, ui
                 raise(JR_EINVAL, "null buffer in job %zu", j);
         }
         Context &ctx = enter(handle);
-        ctx.timed = false;
-        check_cuda(cudaEventRecord(ctx.start, ctx.stream), "record start event");
+        begin_timing(ctx);
         for (uint64_t launch = 0, total = (uint64_t)repeats * job_count; launch < total; ++launch) {
             const jr_job &job = jobs[launch % job_count];
             const auto st = static_cast<cudaError_t>(job.launch(static_cast<void *>(ctx.stream), job.buffers));
@@ -322,6 +334,7 @@ extern "C" int jr_execute(void *handle, const jr_job *jobs, size_t job_count, ui
             check_cuda(stop, "record stop event");
         }
         check_cuda(cudaEventSynchronize(ctx.stop), "kernel synchronization");
+        ctx.timed = true;
         *gpu_ms = bracket_ms(ctx);
     });
 }
@@ -670,7 +683,8 @@ extern "C" int jr_execute2(void *handle, const jr_dispatch *jobs, size_t job_cou
     return jade::c_entry(err, cap, [&] {
         require(jobs && job_count && repeats && gpu_ms, "empty dispatch sequence or missing timing output");
         const bool graph = flags & JR_EXEC_GRAPH, lanes = flags & JR_EXEC_STREAMS;
-        if (flags & ~(JR_EXEC_GRAPH | JR_EXEC_STREAMS | JR_EXEC_DEFER_MS)) raise(JR_EINVAL, "unknown execution flags 0x%x", flags);
+        if (flags & ~(JR_EXEC_GRAPH | JR_EXEC_STREAMS | JR_EXEC_DEFER_MS | JR_EXEC_HOLD_MS)) raise(JR_EINVAL, "unknown execution flags 0x%x", flags);
+        require(!(flags & JR_EXEC_HOLD_MS) || flags & JR_EXEC_DEFER_MS, "a batch's time is held only where it is deferred");
         require(!(graph && job_ms), "per-job timing is not available with graph replay");
         require(!(graph && lanes), "graph replay and dependency-scheduled streams cannot be combined");
         auto *raw = static_cast<Context *>(handle);
@@ -691,10 +705,9 @@ extern "C" int jr_execute2(void *handle, const jr_dispatch *jobs, size_t job_cou
                 if (!*s) check_cuda(cudaStreamCreateWithFlags(s, cudaStreamNonBlocking), what);
             reserve_events(ctx.dep_events, launches, cudaEventDisableTiming, what);
         }
-        ctx.timed = false;
         CapturedPass pass;
         if (graph) pass.capture(ctx.stream, jobs, job_count);
-        check_cuda(cudaEventRecord(ctx.start, ctx.stream), "record start event");
+        begin_timing(ctx, flags & JR_EXEC_HOLD_MS);
         std::unique_ptr<LaneScheduler> sched;
         try {
             if (lanes) sched = std::make_unique<LaneScheduler>(ctx, launches);
@@ -734,6 +747,7 @@ extern "C" int jr_execute2(void *handle, const jr_dispatch *jobs, size_t job_cou
         await_event(ctx, defer ? ctx.done : ctx.stop, collective);
         raise_device_wait_error(ctx);
         ctx.timed = true;
+        if (flags & JR_EXEC_HOLD_MS) ctx.held = Context::Held::Bracketed;
         if (!(flags & JR_EXEC_DEFER_MS)) *gpu_ms = bracket_ms(ctx);
         if (job_ms)
             for (size_t launch = 0; launch < launches; ++launch) {
@@ -751,6 +765,17 @@ extern "C" int jr_batch_ms(void *handle, double *gpu_ms, char *err, size_t cap) 
         Context &ctx = enter(handle);
         require(ctx.timed, "no completed batch to time");
         *gpu_ms = bracket_ms(ctx);
+    });
+}
+
+extern "C" int jr_held_ms(void *handle, double *gpu_ms, char *err, size_t cap) {
+    if (gpu_ms) *gpu_ms = 0;
+    return jade::c_entry(err, cap, [&] {
+        require(gpu_ms != nullptr, "missing timing output");
+        Context &ctx = enter(handle);
+        require(ctx.held != Context::Held::None, "no batch whose time is held");
+        read_held(ctx);
+        *gpu_ms = ctx.held_ms;
     });
 }
 

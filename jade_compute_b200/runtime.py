@@ -32,6 +32,7 @@ JR_OK, JR_EINVAL, JR_ECUDA, JR_ENOMEM, JR_ETIMEOUT = 0, 1, 2, 3, 4
 JR_EXEC_GRAPH = 1
 JR_EXEC_STREAMS = 2
 JR_EXEC_DEFER_MS = 4
+JR_EXEC_HOLD_MS = 8
 
 DTYPE_SIZE = {"fp32": 4, "tf32": 4, "bf16": 2, "fp16": 2, "u8": 1, "i32": 4}
 NP_DTYPE = {"fp32": np.float32, "tf32": np.float32, "bf16": np.uint16, "fp16": np.float16, "u8": np.uint8, "i32": np.int32}
@@ -88,6 +89,7 @@ def lib() -> ctypes.CDLL:
     L.jr_execute2.argtypes = [vp, vp, sz, u32, u32, ctypes.POINTER(ctypes.c_double),
                               ctypes.POINTER(ctypes.c_double), c_char_p, sz]
     L.jr_batch_ms.argtypes = [vp, ctypes.POINTER(ctypes.c_double), c_char_p, sz]
+    L.jr_held_ms.argtypes = [vp, ctypes.POINTER(ctypes.c_double), c_char_p, sz]
     L.jr_buffer_bytes.argtypes = [vp, vp, ctypes.POINTER(sz)]
     L.jr_host_alloc.argtypes = [vp, sz, ctypes.POINTER(vp), c_char_p, sz]
     L.jr_host_free.argtypes = [vp, vp]
@@ -228,21 +230,30 @@ class Kernel:
             self.handle = 0
 
 
+@dataclass
 class Execution:
-    """src/runtime/mod.rs:23-30 plus per-job device times. ``gpu_ms`` is read from the
-    device when it is asked for, or before the runtime's next batch at the latest."""
-    __slots__ = ("host_ms", "dispatches", "repeats", "job_ms", "_runtime", "_gpu_ms", "__weakref__")
+    """src/runtime/mod.rs:23-30 plus per-job device times. ``gpu_ms`` of a batch that has
+    run is read from the device when it is asked for, or before the runtime's next batch
+    at the latest."""
+    host_ms: float
+    gpu_ms: float | None
+    dispatches: int
+    repeats: int
+    job_ms: list | None = None
 
-    def __init__(self, runtime: "Runtime", host_ms: float, dispatches: int, repeats: int, job_ms: list | None = None):
-        self.host_ms, self.dispatches, self.repeats, self.job_ms = host_ms, dispatches, repeats, job_ms
-        self._runtime, self._gpu_ms = runtime, None
+    # Runtime.execute leaves gpu_ms unset and adds _runtime, a weak reference
+    def __getattr__(self, name):  # of attributes not set: gpu_ms that has not been read
+        if name != "gpu_ms" or "_runtime" not in self.__dict__:
+            raise AttributeError(name)
+        runtime = self._runtime()
+        if runtime is None:
+            raise JadeError(JR_EINVAL, "the batch's runtime is gone")
+        self.gpu_ms = runtime._held_ms()
+        return self.gpu_ms
 
-    @property
-    def gpu_ms(self) -> float | None:
-        if self._runtime is not None:
-            self._gpu_ms = self._runtime._batch_ms()
-            self._runtime = None
-        return self._gpu_ms
+    def __getstate__(self):
+        self.gpu_ms
+        return {k: v for k, v in self.__dict__.items() if k != "_runtime"}
 
 
 class _Dispatch(ctypes.Structure):
@@ -267,13 +278,14 @@ class Runtime:
         self.device_info = out.value.decode()
         self._kernels: list[Kernel] = []
         self._message = _err()  # of execute (a context is used serially)
-        self._last = None  # weak reference to the last batch's Execution
+        self._self = weakref.ref(self)
+        self._last = None  # weak reference to the last batch's Execution, and its attributes
 
     # -- lifetime
     def close(self) -> None:
         if self.ctx:
             try:
-                self._settle()
+                self._settle(closing=True)
             except JadeError:
                 pass  # a context that has failed has no time to give
             for k in self._kernels:
@@ -388,28 +400,32 @@ class Runtime:
         e = self._message
         gpu = ctypes.c_double(0)
         jm = (ctypes.c_double * len(jobs))() if per_job else None
-        flags = (JR_EXEC_GRAPH if graph else 0) | (JR_EXEC_STREAMS if streams else 0) | JR_EXEC_DEFER_MS
+        flags = (JR_EXEC_GRAPH if graph else 0) | (JR_EXEC_STREAMS if streams else 0) | JR_EXEC_DEFER_MS | JR_EXEC_HOLD_MS
         self._settle()
         t0 = time.perf_counter()
         rc = lib().jr_execute2(self.ctx, words.buffer_info()[0], len(jobs), repeats, flags, ctypes.byref(gpu), jm, e, len(e))
         host_ms = (time.perf_counter() - t0) * 1e3
         if rc != JR_OK:
             _check(rc, e)
-        done = Execution(self, host_ms, len(jobs) * repeats, repeats, list(jm) if per_job else None)
-        self._last = weakref.ref(done)
+        done = Execution.__new__(Execution)
+        done.__dict__ = known = {"host_ms": host_ms, "dispatches": len(jobs) * repeats, "repeats": repeats,
+                                 "job_ms": list(jm) if per_job else None, "_runtime": self._self}
+        self._last = weakref.ref(done), known
         return done
 
-    def _batch_ms(self) -> float | None:
+    def _held_ms(self) -> float | None:
         e, ms = _err(), ctypes.c_double(0)
-        _check(lib().jr_batch_ms(self.ctx, ctypes.byref(ms), e, len(e)), e)
+        _check(lib().jr_held_ms(self.ctx, ctypes.byref(ms), e, len(e)), e)
         return ms.value if ms.value > 0 else None
 
-    def _settle(self) -> None:
-        """Reads the last batch's time if its Execution is still held."""
-        held = self._last and self._last()
-        self._last = None
-        if held:
-            held.gpu_ms
+    def _settle(self, closing: bool = False) -> None:
+        """Reads the last batch's time if its Execution is still held (when the runtime is
+        collected as garbage its weak references are already cleared: read in any case)."""
+        if self._last is None:
+            return
+        (held, attributes), self._last = self._last, None
+        if (closing or held() is not None) and "gpu_ms" not in attributes:
+            attributes["gpu_ms"] = self._held_ms()
 
     # -- conveniences used by tests and benches
     def fill(self, buf: Buffer, dist: str, seed: int, stream: int = 0, lo: float = 0.0, hi: float = 1.0,
