@@ -48,7 +48,8 @@ def causal_tree(batch: int, seq: int) -> np.ndarray:
 
 class CachedAttention:
     """One layer on one device. ``keep`` > 0 accumulates attention weights and
-    allocates the second cache that ``evict`` moves entries into."""
+    allocates the second cache that ``evict`` moves entries into. ``rotation``: fields of
+    the qk_norm_rope spec; ``norm=False`` for a layer without head norms."""
 
     def __init__(self, rt: Runtime, batch: int, seq: int, width: int, heads: int, kv_heads: int, dim: int, capacity: int,
                  dtype: str = "bf16", eps: float = 1e-6, keep: int = 0, recent: int = 0, **rotation):
@@ -62,6 +63,7 @@ class CachedAttention:
         heads_of = {"batch": batch, "kv_heads": kv_heads, "dim": dim, "capacity": capacity, "dtype": dtype}
         gemm = {"op": "gemm", "tiled": True, "dtype": dtype, "out_dtype": dtype, "b_layout": "nk", "m": tokens}
         self.k_qkv = rt.compile({**gemm, "n": packed, "k": width})
+        norm = rotation.get("norm", True)
         self.k_rope = rt.compile({"op": "qk_norm_rope", "seq": seq, "heads": heads, "epsilon": eps, **heads_of, **rotation})
         self.k_attend = rt.compile({"op": "attention_tree", "seq": seq, "heads": heads, "weights": keep > 0, **heads_of})
         self.k_out = rt.compile({**gemm, "n": width, "k": heads * dim, "epilogue": "residual"})
@@ -74,14 +76,15 @@ class CachedAttention:
         cache = batch * kv_heads * capacity
         self.x, self.y = alloc(tokens * width), alloc(tokens * width)
         self.wqkv, self.wo = alloc(packed * width), alloc(width * heads * dim)
-        self.q_weight, self.k_weight = alloc(dim), alloc(dim)
+        self.q_weight, self.k_weight = (alloc(dim), alloc(dim)) if norm else (None, None)
+        self.norm_weights = [self.q_weight, self.k_weight] if norm else []
         self.qkv, self.q, self.out = alloc(tokens * packed), alloc(tokens * heads * dim), alloc(tokens * heads * dim)
         self.k, self.v = alloc(cache * dim), alloc(cache * dim)
         self.positions, self.tree = alloc(tokens, "i32"), alloc(tokens * (-(-seq // 32)), "i32")
         self.lengths, self.next_lengths = alloc(batch, "i32"), alloc(batch, "i32")
         self.path, self.counts = alloc(tokens, "i32"), alloc(batch, "i32")
-        self.buffers = [self.x, self.y, self.wqkv, self.wo, self.q_weight, self.k_weight, self.qkv, self.q, self.out, self.k, self.v,
-                        self.positions, self.tree, self.lengths, self.next_lengths, self.path, self.counts]
+        self.buffers = [self.x, self.y, self.wqkv, self.wo, *self.norm_weights, self.qkv, self.q, self.out, self.k, self.v, self.positions,
+                        self.tree, self.lengths, self.next_lengths, self.path, self.counts]
         if keep:
             self.k_evict = rt.compile({"op": "cache_evict", "keep": keep, "recent": recent, **heads_of})
             self.kernels.append(self.k_evict)
@@ -101,7 +104,7 @@ class CachedAttention:
     def step_jobs(self):
         accumulated = [self.weights] if self.keep else []
         return [(self.k_qkv, [self.x, self.wqkv, self.qkv]),
-                (self.k_rope, [self.qkv, self.q_weight, self.k_weight, self.positions, self.lengths, self.q, self.k, self.v]),
+                (self.k_rope, [self.qkv, *self.norm_weights, self.positions, self.lengths, self.q, self.k, self.v]),
                 (self.k_attend, [self.q, self.k, self.v, self.lengths, self.tree, self.out, *accumulated]),
                 (self.k_out, [self.out, self.wo, self.x, self.y])]
 
@@ -114,12 +117,16 @@ class CachedAttention:
         x = np.asarray(x, np.float32).ravel()
         return f32_to_bf16(x) if self.dtype == "bf16" else x.astype(np.float16)
 
-    def load(self, wqkv, wo, q_weight, k_weight) -> None:
-        """wqkv [width, (heads + 2 kv_heads) dim], wo [heads dim, width], norm weights [dim]."""
+    def load(self, wqkv, wo, q_weight=None, k_weight=None) -> None:
+        """wqkv [width, (heads + 2 kv_heads) dim], wo [heads dim, width], norm weights [dim]
+        (none for a layer without head norms)."""
+        weights = [w for w in (q_weight, k_weight) if w is not None]
+        if len(weights) != len(self.norm_weights):
+            raise ValueError(f"this layer has {len(self.norm_weights)} norm weights, not {len(weights)}")
         self.rt.upload(self.wqkv, self._to_dtype(np.asarray(wqkv, np.float32).reshape(self.width, -1).T))
         self.rt.upload(self.wo, self._to_dtype(np.asarray(wo, np.float32).reshape(-1, self.width).T))
-        self.rt.upload(self.q_weight, self._to_dtype(q_weight))
-        self.rt.upload(self.k_weight, self._to_dtype(k_weight))
+        for buf, weight in zip(self.norm_weights, weights):
+            self.rt.upload(buf, self._to_dtype(weight))
 
     def step(self, x, positions, tree=None) -> np.ndarray:
         """x [batch, seq, width], positions [batch, seq]; tree: bits as tree_words gives them

@@ -1,0 +1,83 @@
+"""CachedAttention's accumulated weights and its forms, against the 64-bit definition on the
+buffers that the layer's attention read (tolerances: tests/test_gpu_cached_attention.py)."""
+import numpy as np
+import pytest
+
+import jade_compute_b200 as jc
+from jade_compute_b200.cached_attention import CachedAttention, causal_tree, tree_words
+from tests import cached_reference as R
+
+pytestmark = pytest.mark.gpu
+B, T, WIDTH, H, HK, D, C = 2, 4, 64, 4, 2, 32, 60
+
+
+@pytest.fixture(scope="module")
+def rt():
+    r = jc.Runtime(0)
+    yield r
+    r.close()
+
+
+def make(rt, **options):
+    layer = CachedAttention(rt, B, T, WIDTH, H, HK, D, C, **options)
+    rng = np.random.default_rng(5)
+    layer.load(0.2 * rng.standard_normal((WIDTH, (H + 2 * HK) * D)), 0.2 * rng.standard_normal((H * D, WIDTH)), np.ones(D), np.ones(D))
+    return layer
+
+
+def added_weights(rt, layer, lengths, sees, rows=None):
+    """The definition's sum of weights of the layer's last step; rows [B, T]: those that count."""
+    def fetch(buf, *shape):
+        return rt.download_f32(buf).astype(np.float64).reshape(shape)
+
+    q, k, v = fetch(layer.q, B, H, T, D), fetch(layer.k, B, HK, C, D), fetch(layer.v, B, HK, C, D)
+    added = np.zeros((B, HK, C))
+    for b in range(B):
+        live = slice(0, lengths[b] + T)
+        mask = np.concatenate([np.ones((T, lengths[b]), bool), sees[b]], 1)
+        for h in range(HK):
+            p = R.attention(q[b, h * H // HK:(h + 1) * H // HK].reshape(-1, D), k[b, h, live], v[b, h, live], np.tile(mask, (H // HK, 1)))[2]
+            added[b, h, live] = (p.reshape(H // HK, T, -1) * (1 if rows is None else rows[b][:, None])).sum((0, 1))
+    return added
+
+
+def held_weights(rt, layer):
+    return rt.download_f32(layer.weights).astype(np.float64).reshape(B, HK, C)
+
+
+def near(got, ref):
+    bound = 1e-4 * ref + 1e-6
+    assert (np.abs(got - ref) <= bound).all(), np.max(np.abs(got - ref) - bound)
+
+
+CAUSAL = np.tile(np.tril(np.ones((T, T), bool)), (B, 1, 1))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_layer_without_head_norms(rt, dtype):
+    rng = np.random.default_rng(8)
+    layer = CachedAttention(rt, B, T, WIDTH, H, HK, D, C, dtype=dtype, norm=False)
+    wqkv = R.rounded(0.2 * rng.standard_normal((WIDTH, (H + 2 * HK) * D)), dtype)
+    layer.load(wqkv, 0.2 * rng.standard_normal((H * D, WIDTH)))
+    try:
+        at = np.tile(np.arange(T), (B, 1))
+        y = layer.step(rng.standard_normal((B, T, WIDTH)), at)
+        assert np.isfinite(y).all()
+        qkv = rt.download_f32(layer.qkv).astype(np.float64).reshape(B, T, H + 2 * HK, D)
+        (q, m), _, _ = R.norm_rope({"heads": H, "kv_heads": HK, "dim": D, "norm": False}, {"qkv": qkv, "positions": at})
+        got = rt.download_f32(layer.q).astype(np.float64).reshape(B, H, T, D)
+        u, tiny = R.ROUNDOFF[dtype], 2.0 ** -25 if dtype == "fp16" else 0.0
+        q, m = q.transpose(0, 2, 1, 3), m.transpose(0, 2, 1, 3)
+        assert (np.abs(got - q) <= np.maximum(u * np.abs(q), tiny) + 4e-6 * m).all()
+        assert layer.commit().tolist() == [T] * B
+    finally:
+        layer.release()
+
+
+def test_load_wants_the_norm_weights_that_the_layer_has(rt):
+    wqkv, wo = np.zeros((WIDTH, (H + 2 * HK) * D)), np.zeros((H * D, WIDTH))
+    for options, weights in (({}, []), ({}, [np.ones(D)]), ({"norm": False}, [np.ones(D)] * 2)):
+        layer = CachedAttention(rt, B, T, WIDTH, H, HK, D, C, **options)
+        with pytest.raises(ValueError, match="norm weights"):
+            layer.load(wqkv, wo, *weights)
+        layer.release()
