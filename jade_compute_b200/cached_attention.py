@@ -12,7 +12,10 @@ A step takes ``seq`` tokens of every sequence. Plain decoding is a tree of one t
 (``seq=1``); a prompt goes in pieces of ``seq`` tokens, each seeing the ones before it
 (``causal_tree``); speculative decoding passes a tree of drafts and commits the
 accepted branch. The step's tokens stay behind the committed entries until ``commit``
-names the ones to keep, so an uncommitted step is simply overwritten by the next.
+names the ones to keep, so an uncommitted step is simply overwritten by the next. The
+same holds for the accumulated weights: a step adds its own to those of the last commit.
+A committed step counts whole, drafts that its commit leaves out included (they have
+attended to the committed entries; their own entries go with them).
 
 Weights are FP32 host arrays in the reference's K x N layout; activations and the
 cache are BF16 or FP16, sums FP32.
@@ -88,9 +91,12 @@ class CachedAttention:
         if keep:
             self.k_evict = rt.compile({"op": "cache_evict", "keep": keep, "recent": recent, **heads_of})
             self.kernels.append(self.k_evict)
-            self.weights, self.next_weights = alloc(cache, "fp32"), alloc(cache, "fp32")
+            # the weights with those of the step that is not committed yet, as of the last commit, and the eviction's
+            self.weights, self.committed_weights, self.next_weights = (alloc(cache, "fp32") for _ in range(3))
+            self.k_copy = rt.compile({"op": "copy", "bytes": 4 * cache, "direction": "d2d"})
+            self.kernels.append(self.k_copy)
             self.next_k, self.next_v, self.kept = alloc(cache * dim), alloc(cache * dim), alloc(batch * kv_heads * keep, "i32")
-            self.buffers += [self.weights, self.next_weights, self.next_k, self.next_v, self.kept]
+            self.buffers += [self.weights, self.committed_weights, self.next_weights, self.next_k, self.next_v, self.kept]
         rt.upload(self.tree, causal_tree(batch, seq))
 
     def release(self) -> None:
@@ -103,14 +109,16 @@ class CachedAttention:
     # -- jobs, for use in a larger batch
     def step_jobs(self):
         accumulated = [self.weights] if self.keep else []
-        return [(self.k_qkv, [self.x, self.wqkv, self.qkv]),
+        back = [(self.k_copy, [self.committed_weights, self.weights])] if self.keep else []
+        return [*back, (self.k_qkv, [self.x, self.wqkv, self.qkv]),
                 (self.k_rope, [self.qkv, *self.norm_weights, self.positions, self.lengths, self.q, self.k, self.v]),
                 (self.k_attend, [self.q, self.k, self.v, self.lengths, self.tree, self.out, *accumulated]),
                 (self.k_out, [self.out, self.wo, self.x, self.y])]
 
     def commit_jobs(self):
         accumulated = [self.weights] if self.keep else []
-        return [(self.k_commit, [self.path, self.counts, self.lengths, self.k, self.v, *accumulated, self.next_lengths])]
+        hold = [(self.k_copy, [self.weights, self.committed_weights])] if self.keep else []
+        return [(self.k_commit, [self.path, self.counts, self.lengths, self.k, self.v, *accumulated, self.next_lengths]), *hold]
 
     # -- host side
     def _to_dtype(self, x) -> np.ndarray:
@@ -149,12 +157,12 @@ class CachedAttention:
         return self.rt.download(self.lengths)
 
     def evict(self) -> np.ndarray:
-        """Keeps ``keep`` committed entries a head. Returns the slots that they had
-        [batch, kv_heads, keep], -1 where a sequence has fewer."""
+        """Keeps ``keep`` committed entries a head, by their weights as of the last commit.
+        Returns the slots that they had [batch, kv_heads, keep], -1 where a sequence has fewer."""
         if not self.keep:
             raise ValueError("this layer accumulates no weights (keep=0)")
-        self.rt.execute([(self.k_evict, [self.k, self.v, self.weights, self.lengths, self.next_k, self.next_v, self.next_weights, self.kept,
-                                         self.next_lengths])])
+        self.rt.execute([(self.k_evict, [self.k, self.v, self.committed_weights, self.lengths, self.next_k, self.next_v, self.next_weights, self.kept,
+                                         self.next_lengths]), (self.k_copy, [self.next_weights, self.committed_weights])])
         for name in ("k", "v", "weights", "lengths"):
             new = "next_" + name
             old = getattr(self, name)

@@ -81,3 +81,33 @@ def test_load_wants_the_norm_weights_that_the_layer_has(rt):
         with pytest.raises(ValueError, match="norm weights"):
             layer.load(wqkv, wo, *weights)
         layer.release()
+def test_step_that_is_not_committed_leaves_no_weight(rt):
+    # a step over again, with other tokens, as a server makes it after a failed draft
+    rng = np.random.default_rng(6)
+    layer = make(rt, keep=16, recent=2)
+    try:
+        lengths, expected = np.zeros(B, int), np.zeros((B, HK, C))
+        for n in range(6):
+            at = lengths[:, None] + np.arange(T)
+            for tries in range(1 + n % 3):
+                layer.step(rng.standard_normal((B, T, WIDTH)), at, causal_tree(B, T))
+            working = expected + added_weights(rt, layer, lengths, CAUSAL)
+            near(held_weights(rt, layer), working)
+            counts = np.array([T, T - n % 2])
+            layer.commit(counts=counts)
+            for b in range(B):
+                working[b, :, lengths[b] + counts[b]:] = 0
+            expected, lengths = working, lengths + counts
+            near(held_weights(rt, layer), expected)
+        layer.step(rng.standard_normal((B, T, WIDTH)), lengths[:, None] + np.arange(T))
+        kept = layer.evict()  # of the committed entries by their committed weights
+        for b in range(B):
+            for h in range(HK):
+                slots = kept[b, h][kept[b, h] >= 0]
+                near(held_weights(rt, layer)[b, h, :len(slots)], expected[b, h, slots])
+                older = np.delete(np.arange(lengths[b] - 2), slots[slots < lengths[b] - 2])
+                assert expected[b, h, older].max() <= expected[b, h, slots[slots < lengths[b] - 2]].min() * (1 + 2e-4)
+    finally:
+        layer.release()
+
+
