@@ -15,7 +15,8 @@ accepted branch. The step's tokens stay behind the committed entries until ``com
 names the ones to keep, so an uncommitted step is simply overwritten by the next. The
 same holds for the accumulated weights: a step adds its own to those of the last commit.
 A committed step counts whole, drafts that its commit leaves out included (they have
-attended to the committed entries; their own entries go with them).
+attended to the committed entries; their own entries go with them); places without a
+draft count nothing.
 
 Weights are FP32 host arrays in the reference's K x N layout; activations and the
 cache are BF16 or FP16, sums FP32.
@@ -68,7 +69,7 @@ class CachedAttention:
         self.k_qkv = rt.compile({**gemm, "n": packed, "k": width})
         norm = rotation.get("norm", True)
         self.k_rope = rt.compile({"op": "qk_norm_rope", "seq": seq, "heads": heads, "epsilon": eps, **heads_of, **rotation})
-        self.k_attend = rt.compile({"op": "attention_tree", "seq": seq, "heads": heads, "weights": keep > 0, **heads_of})
+        self.k_attend = rt.compile({"op": "attention_tree", "seq": seq, "heads": heads, "weights": keep > 0, **({"drafts_only": True} if keep else {}), **heads_of})
         self.k_out = rt.compile({**gemm, "n": width, "k": heads * dim, "epilogue": "residual"})
         self.k_commit = rt.compile({"op": "cache_commit", "seq": seq, "weights": keep > 0, **heads_of})
         self.kernels = [self.k_qkv, self.k_rope, self.k_attend, self.k_out, self.k_commit]

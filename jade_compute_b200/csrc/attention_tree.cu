@@ -6,7 +6,8 @@
 //   drafted tokens in slots lengths[b] + i, those whose bit i of tree[b, t] is set.
 //   out[b, t, h] = sum_j p_j v_j,  p = softmax_j(q k_j / sqrt(dim)) over what it sees
 //   (0 where it sees nothing); weights[b, hk, j] += sum of p_j over the group's heads
-//   and the tokens.
+//   and the tokens (with drafts_only: those that see a draft, as every token sees itself;
+//   a place of a step that holds no token has no bits and leaves no weight).
 //
 // The group's heads and tokens of a (sequence, kv head) are M = group * seq rows of q
 // that lie together and share its keys. Keys are split over blocks; each split keeps
@@ -355,7 +356,7 @@ __device__ __forceinline__ void add_weights(const TreeArgs &a, int splits, int f
         for (int s = part; s < splits; s += 4) l = fmaf(ml[s].y, exp2f((ml[s].x - shift) * a.scale_log2), l);
 #pragma unroll
         for (int x = 1; x < 4; x <<= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-        if (part == 0) stats[threadIdx.x >> 2] = make_float2(shift, l > 0.0f || l != l ? 1.0f / l : 0.0f);
+        if (part == 0) stats[threadIdx.x >> 2] = make_float2(shift, adds_weight(a, b, row) && (l > 0.0f || l != l) ? 1.0f / l : 0.0f);
     };
     uint64_t x[4][2 * kPieces];
     auto load_keys = [&](int block) {

@@ -87,11 +87,12 @@ struct Layout {
 
 // Stats of an item: x of every row, p_j = 2^(s_j scale_log2 + x) (the row's sum folded
 // into the exponent: one constant per column for the weights' pass to read), -inf for
-// rows that see nothing and up to whole groups of 32 columns of that pass's MMA.
+// rows that see nothing or add no weight, and up to whole groups of 32 columns of that
+// pass's MMA.
 __host__ __device__ constexpr size_t stats_stride(int rows) { return ((size_t)rows + 31) / 32 * 32; }
 __device__ __forceinline__ void store_stats(const TreeArgs &t, size_t item, int row, float m, float inv) {
     float *x = t.row_exponents + item * stats_stride(t.rows) + row;
-    *x = log2f(inv) - (m == -INFINITY ? 0.0f : m);
+    *x = adds_weight(t, (int)(item / t.kv_heads), row) ? log2f(inv) - (m == -INFINITY ? 0.0f : m) : -INFINITY;
     if (row == t.rows - 1)
         for (int r = t.rows; r < (int)stats_stride(t.rows); ++r) *++x = -INFINITY;
 }
@@ -199,11 +200,6 @@ __device__ __forceinline__ Segments open_range(const TcArgs &a, int *plan, long 
 }
 
 // ------------------------------------------------------------------ masks
-// The bits of word w that stand for drafts: bits beyond them may be anything.
-__device__ __forceinline__ uint32_t draft_bits(int w, int seq) {
-    const int n = seq - 32 * w;
-    return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1;
-}
 // Bit c of the result: the row sees column c of the tile whose first key lies `off`
 // slots before the first draft (off may be negative: the tile starts among the drafts).
 __device__ __forceinline__ void column_mask(const uint32_t (&bits)[4], int off, uint32_t (&mask)[4]) {

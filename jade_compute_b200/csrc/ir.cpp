@@ -251,6 +251,7 @@ Spec parse_spec(const Json &j) {
         s.heads = get_u32(j, "heads"); s.kv_heads = get_u32(j, "kv_heads"); s.seq = get_u32(j, "seq"); s.dim = get_u32(j, "dim");
         s.capacity = get_u32(j, "capacity");
         if (j.has("weights")) s.weights = get_bool(j, "weights");
+        if (j.has("drafts_only")) s.drafts_only = get_bool(j, "drafts_only");
     } else if (op == "cache_evict") {
         s.op = Op::CacheEvict;
         s.kv_heads = get_u32(j, "kv_heads"); s.dim = get_u32(j, "dim"); s.capacity = get_u32(j, "capacity");
@@ -349,6 +350,7 @@ Json spec_to_json(const Spec &s) {
         case Op::AttentionTree:
             j.set("op", Json::str("attention_tree")).set("heads", U(s.heads)).set("kv_heads", U(s.kv_heads)).set("seq", U(s.seq)).set("dim", U(s.dim))
                 .set("capacity", U(s.capacity)).set("weights", Json::boolean(s.weights));
+            if (s.drafts_only) j.set("drafts_only", Json::boolean(true));
             break;
         case Op::CacheEvict:
             j.set("op", Json::str("cache_evict")).set("kv_heads", U(s.kv_heads)).set("dim", U(s.dim)).set("capacity", U(s.capacity)).set("keep", U(s.keep))
@@ -402,6 +404,7 @@ void validate_cached_attention(const Spec &s) {
         ensure(s.scaling != "yarn" || s.original >= 1, "yarn scaling needs the original context length");
         ensure(s.op == Op::QkNormRope || !s.capacity, "qk_norm_rope_grad has no cache (capacity)");
     }
+    ensure(!s.drafts_only || s.weights, "drafts_only chooses the rows that add weights");
     if (s.op == Op::CacheCommit) ensure(s.seq >= 1 && s.seq <= 128, "cache_commit sequence must be 1..=128");
     if (s.op == Op::CacheEvict) {
         ensure(s.keep >= 1 && s.keep <= s.capacity, "keep must be 1..=capacity");

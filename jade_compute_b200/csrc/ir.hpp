@@ -99,6 +99,7 @@ struct Spec {
     float factor = 1.0f;           // how many times longer the scaled context is
     uint32_t original = 0;         // yarn: the context length before scaling
     bool weights = false;          // accumulated attention weight of every cache slot
+    bool drafts_only = false;      // attention_tree: rows that see no draft add no weight
     uint32_t keep = 0, recent = 0; // cache_evict: entries kept, of which the newest always
     bool extended() const;
 };

@@ -6,6 +6,7 @@ import pytest
 import jade_compute_b200 as jc
 from jade_compute_b200.cached_attention import CachedAttention, causal_tree, tree_words
 from tests import cached_reference as R
+from tests import test_gpu_cached_attention as base
 
 pytestmark = pytest.mark.gpu
 B, T, WIDTH, H, HK, D, C = 2, 4, 64, 4, 2, 32, 60
@@ -111,3 +112,44 @@ def test_step_that_is_not_committed_leaves_no_weight(rt):
         layer.release()
 
 
+def test_places_without_a_draft_add_no_weight(rt):
+    # the last piece of a prompt, a tree smaller than the step: their rows are no tokens
+    rng = np.random.default_rng(7)
+    layer = make(rt, keep=16, recent=2)
+    try:
+        layer.step(rng.standard_normal((B, T, WIDTH)), np.tile(np.arange(T), (B, 1)), causal_tree(B, T))
+        expected = added_weights(rt, layer, [0] * B, CAUSAL)
+        layer.commit()
+        words = tree_words([[-1, 0, -2, -2], [-1, 0, 0, -2]])
+        layer.step(rng.standard_normal((B, T, WIDTH)), T + np.tile(np.arange(T), (B, 1)), words)
+        sees = (words[:, :, 0, None] >> np.arange(T) & 1).astype(bool)
+        rows = sees.any(-1)
+        assert rows.tolist() == [[True, True, False, False], [True, True, True, False]]
+        near(held_weights(rt, layer), expected + added_weights(rt, layer, [T] * B, sees, rows))
+    finally:
+        layer.release()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("case", [1, 3, 4, 5, 7, 12, 13, 14])
+def test_drafts_only_leaves_out_rows_that_see_no_draft(rt, case, dtype):
+    case = base.TREES[case]
+    x, sees = base.tree_inputs(case, dtype, 80)
+    rng = np.random.default_rng(81)
+    sees &= (rng.random(sees.shape[:2]) < 0.6)[:, :, None]
+    sees[0, 0] = False
+    words = R.tree_words(sees)
+    if case["seq"] % 32:  # bits beyond the drafts are none
+        words[..., -1] = (words[..., -1].view(np.uint32) | np.uint32(0xffffffff) << np.uint32(case["seq"] % 32)).view(np.int32)
+    x["tree"] = words
+    got = R.run(rt, {**base.tree_spec(case, dtype), "drafts_only": True}, x)
+    base.check_tree(got, case, x, sees, dtype, weights=False)
+    hk, group = case["kv_heads"], case["heads"] // case["kv_heads"]
+    added = np.zeros_like(x["weights"], np.float64)
+    for b, n in enumerate(case["lengths"]):
+        mask, live = np.concatenate([np.ones((case["seq"], n), bool), sees[b]], 1), slice(0, n + case["seq"])
+        for h in range(hk):
+            q = x["q"][b, h * group:(h + 1) * group].reshape(-1, case["dim"])
+            p = R.attention(q, x["k"][b, h, live], x["v"][b, h, live], np.tile(mask, (group, 1)))[2]
+            added[b, h, live] = p[np.tile(sees[b].any(-1), group)].sum(0)
+    base.close(got["weights"].reshape(added.shape), x["weights"] + added, added, 2.0 ** -23, 2e-5 if dtype == "fp32" else 1e-4)

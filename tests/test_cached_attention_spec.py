@@ -76,3 +76,11 @@ def test_outputs_must_not_alias():
     jc.spec_validate_bindings(COMMIT, lengths, list(range(6)))
     with pytest.raises(JadeError, match="alias"):
         jc.spec_validate_bindings(COMMIT, lengths, [0, 1, 2, 3, 4, 2])  # lengths_out on lengths
+
+
+def test_drafts_only_goes_with_weights():
+    spec = {**TREE, "weights": True, "drafts_only": True}
+    assert json.loads(jc.canonical(spec))["drafts_only"] is True and jc.spec_bindings(spec) == jc.spec_bindings({**TREE, "weights": True})
+    assert jc.canonical({**spec, "drafts_only": False}) == jc.canonical({**TREE, "weights": True})
+    with pytest.raises(JadeError, match="drafts_only"):
+        jc.spec_validate({**TREE, "drafts_only": True})
