@@ -25,7 +25,7 @@ from __future__ import annotations
 
 import numpy as np
 
-from .runtime import Runtime, f32_to_bf16
+from .runtime import JR_EINVAL, JadeError, Runtime, f32_to_bf16
 
 
 def tree_words(parents) -> np.ndarray:
@@ -151,8 +151,15 @@ class CachedAttention:
         """Keeps drafts path[b, :counts[b]] (ascending) of the last step, all of them by
         default. Returns the sequences' new lengths."""
         everything = np.tile(np.arange(self.seq), (self.batch, 1))
-        self.rt.upload(self.path, np.asarray(everything if path is None else path, np.int32).ravel())
-        self.rt.upload(self.counts, np.full(self.batch, self.seq, np.int32) if counts is None else np.asarray(counts, np.int32))
+        path = np.asarray(everything if path is None else path, np.int32).reshape(self.batch, self.seq)
+        counts = np.full(self.batch, self.seq, np.int32) if counts is None else np.asarray(counts, np.int32).reshape(self.batch)
+        # refused here for all sequences: the operator leaves out a bad one and moves the others
+        taken = np.arange(self.seq) < counts[:, None]
+        ascends = np.diff(path, axis=1, prepend=-1) > 0
+        if (counts < 0).any() or (counts > self.seq).any() or not ascends[taken].all() or (path[taken] >= self.seq).any():
+            raise JadeError(JR_EINVAL, "commit: a path must ascend within the step's tokens, its count be at most their number")
+        self.rt.upload(self.path, path.ravel())
+        self.rt.upload(self.counts, counts)
         self.rt.execute(self.commit_jobs())
         self.lengths, self.next_lengths = self.next_lengths, self.lengths
         return self.rt.download(self.lengths)

@@ -153,3 +153,25 @@ def test_drafts_only_leaves_out_rows_that_see_no_draft(rt, case, dtype):
             p = R.attention(q, x["k"][b, h, live], x["v"][b, h, live], np.tile(mask, (group, 1)))[2]
             added[b, h, live] = p[np.tile(sees[b].any(-1), group)].sum(0)
     base.close(got["weights"].reshape(added.shape), x["weights"] + added, added, 2.0 ** -23, 2e-5 if dtype == "fp32" else 1e-4)
+
+
+@pytest.mark.parametrize("path,counts", [([[1, 3, 0, 0], [2, 1, 0, 0]], [2, 2]), ([[1, 3, 0, 0], [0, 4, 0, 0]], [2, 2]), ([[1, 3, 0, 0], [-1, 1, 0, 0]], [2, 1]),
+                                         ([[1, 3, 0, 0], [0, 0, 0, 0]], [2, 5]), ([[1, 3, 0, 0], [0, 0, 0, 0]], [2, -1])])
+def test_commit_that_is_refused_moves_nothing(rt, path, counts):
+    # a path that is none in one sequence: no other sequence's drafts move either, so that the
+    # right commit that follows finds them where the step left them
+    rng = np.random.default_rng(9)
+    layer = make(rt, keep=16, recent=2)
+    try:
+        layer.step(rng.standard_normal((B, T, WIDTH)), np.tile(np.arange(T), (B, 1)))
+        k = rt.download_f32(layer.k).reshape(B, HK, C, D)[:, :, :T].copy()
+        weights = held_weights(rt, layer)
+        with pytest.raises(jc.JadeError, match="path must ascend"):
+            layer.commit(path, counts)
+        np.testing.assert_array_equal(rt.download_f32(layer.k).reshape(B, HK, C, D)[:, :, :T], k)
+        assert layer.commit([[1, 3, 0, 0], [1, 2, 0, 0]], [2, 2]).tolist() == [2, 2]
+        for b, rows in enumerate(([1, 3], [1, 2])):
+            np.testing.assert_array_equal(rt.download_f32(layer.k).reshape(B, HK, C, D)[b, :, :2], k[b][:, rows])
+            np.testing.assert_array_equal(held_weights(rt, layer)[b, :, :2], weights[b][:, rows])
+    finally:
+        layer.release()
