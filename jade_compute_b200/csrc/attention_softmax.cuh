@@ -41,6 +41,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+// The same, NaN if any of them is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float mufu_exp2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -54,7 +60,8 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 // 2^f by a cubic (relative-error least-squares fit on [-1/2, 1/2], max relative
 // error 7.5e-5, below the 16-bit rounding of P), 2^n added to the exponent field.
 // x is clamped to -125 so the exponent stays in the normal range (results below
-// 2^-125 are returned as about 2^-125 instead of smaller values).
+// 2^-125 are returned as about 2^-125 instead of smaller values). NaN comes out finite
+// like them: a caller looks for it in the row's maximum.
 __device__ __forceinline__ uint64_t poly_exp2_pair(uint64_t x) {
     float x0, x1;
     unpack2f(x, x0, x1);

@@ -334,14 +334,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
                 float mx[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) mx[e] = max3(sv[e], sv[e + 8], sv[e + 16]);
+                for (int e = 0; e < 8; ++e) mx[e] = max3_nan(sv[e], sv[e + 8], sv[e + 16]);
 #pragma unroll
                 for (int i = 24; i < 120; i += 16)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) mx[e] = max3(mx[e], sv[i + e], sv[i + 8 + e]);
+                    for (int e = 0; e < 8; ++e) mx[e] = max3_nan(mx[e], sv[i + e], sv[i + 8 + e]);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) mx[e] = fmaxf(mx[e], sv[120 + e]);
-                const float mraw = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7]));
+                for (int e = 0; e < 8; e += 2) mx[e] = max3_nan(mx[e], sv[120 + e], sv[121 + e]);
+                const float mraw = max3_nan(max3_nan(mx[0], mx[1], mx[2]), max3_nan(mx[3], mx[4], mx[5]), max3_nan(mx[6], mx[7], mx[7]));
                 const float m_tile = mraw * c;
                 // lazy rescale: keep the old maximum unless it grew by more than 2^8
                 float m_new = m_used, alpha = 1.0f;
@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_st32f(to + oc, ov);
                     }
                 }
-                l_run = l_run * alpha + psum;
+                // a NaN or +inf score makes the row NaN; the polynomial alone would drop it
+                l_run = l_run * alpha + (m_tile < INFINITY ? psum : NAN);
                 tmem_wait_st();
                 tc_fence_before();
                 mbar_arrive(&p_full[t]);
