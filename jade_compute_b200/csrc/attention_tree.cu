@@ -14,8 +14,10 @@
 // a running maximum m and sum l per row (FP32) and an unnormalised FP32 sum of
 // e^(s - m) v, and the splits are joined by rescaling to the common maximum in split
 // order, so results do not depend on timing. Entries that a row does not see are
-// never multiplied (a NaN or infinity there cannot reach the row), slots from
-// lengths[b] + seq on are not read.
+// never multiplied (a NaN or infinity there cannot reach the row), nor is anything in slots
+// from lengths[b] + seq on (the tcgen05 form's last tile loads what lies there and masks it).
+// Entries that a row does see count as they are: a NaN, or a score of +inf, makes the row
+// NaN, a score of -inf weighs nothing, an infinity in v reaches its column.
 //
 // This file: FP32, and 16-bit types with dim above 128, on FFMA; weights; dispatch.
 // attention_tree_tc.cu: 16-bit types with dim up to 128, on tcgen05.

@@ -33,9 +33,9 @@
 // chains'.
 // Measured on B200, 8 kv heads of 128: 16 sequences of 1,000 to 8,000 keys, one token of 4
 // heads each (295 MB), 63 us with the join = 4.7 TB/s; 4 of 9,000 to 16,000, 128 rows, 56 us
-// (28 more for the weights); one of 131,000 in FP16, 256 rows, 153 us = 900 TFLOP/s at 1965
-// MHz (175 to 180 under the power cap), 2.2 us per pair of row tiles and key tile: bound by
-// the chain of S, its softmax and P V, not by HBM. Copies: 4 rows of 64 elements, 43.7 us
+// (28 more for the weights); one of 131,000 in FP16, 256 rows, 152 to 157 us = 900 TFLOP/s at
+// 1965 MHz (175 to 180 under the power cap), 2.2 us per pair of row tiles and key tile: bound
+// by the chain of S, its softmax and P V, not by HBM. Copies: 4 rows of 64 elements, 43.7 us
 // with four copies and 49.3 with none.
 //
 // A tile that reaches beyond the committed slots is masked per row by the drafts'
@@ -65,7 +65,8 @@ struct Exponents {
 // Measured on B200, 4 rows, 128 items of 9 to 63 tiles: 73.8 us with 0, 67.3 with 2,
 // 65.7 with 4, 64.6 with 6, 64.5 with 8, 67.0 with 12; 128 rows, 32 items of 72 to 126
 // tiles: 60.3 us with 6, 56.8 with 10, 55.8 with 12, 55.4 with 16. Two row tiles
-// (twice the time per tile): 73.6 us with 6, 74.9 with 10.
+// (twice the time per tile): 73.6 us with 6, 74.9 with 10. Row counts between (4 to 128,
+// three mixes of lengths from 100 to 16,000 keys): within 5 % of the best of 4, 8, 12 and 16.
 constexpr int boundary_tiles(int rows) { return rows > 128 ? 6 : 6 + rows / 20; }
 
 template <int DP, bool kTwoTiles, int kCopies>
